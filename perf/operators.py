@@ -1,0 +1,431 @@
+"""The operators of a preference-tuned ranker's training step, as they are measured: embedding lookup with its gradient,
+token log probabilities with their gradient, the preference loss with its gradient, and the AdamW step.
+
+`run` computes them in their plain form (elementary torch operations in 32 bits, in 64 where a long sum or a value next to a
+rounding border needs it), or, where `own` is true, by the calls that a user makes of ranking_amd."""
+import math
+
+import torch
+
+own = False
+
+_DTYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+_BYTES = {'fp32': 4, 'bf16': 2, 'fp16': 2}
+_QBLOCK = 128                      # elements that share one scale of an 8-bit optimizer state
+_BETA1, _BETA2, _EPS, _LR, _DECAY, _STEP = 0.9, 0.999, 1e-8, 1e-3, 0.01, 100
+
+
+def listed():
+    return [
+        # one new token of each of four running requests: latency only
+        dict(name='embed_decode', op='embed', rows=65536, dim=1024, bags=4, tokens=1, pool='none', dtype='bf16', ids='int64', scale=32.0, grad=False),
+        # text features of ranked documents, averaged (512 lists of 50 documents, 20-wide embeddings), trained in fp32
+        dict(name='embed_pooled_documents', op='embed', rows=30011, dim=20, bags=25600, tokens=32, pool='mean', dtype='fp32', ids='int32', scale=1.0, grad=True),
+        # one micro-batch of a language model
+        dict(name='embed_train', op='embed', rows=65536, dim=1024, bags=16384, tokens=1, pool='none', dtype='bf16', ids='int64', scale=32.0, grad=True),
+        # a large batch on a large table
+        dict(name='embed_train_large', op='embed', rows=131072, dim=2048, bags=262144, tokens=1, pool='none', dtype='bf16', ids='int64', scale=1.0, grad=True),
+        # two candidate answers' next token scored while decoding: two rows share the card
+        dict(name='logprob_decode', op='logprob', rows=2, vocab=131072, dtype='bf16', temperature=0.7, grad=False),
+        # a policy over the items of ranked lists (headline sizes: 16384 lists of 200), trained in fp32
+        dict(name='logprob_items', op='logprob', rows=16384, vocab=200, dtype='fp32', temperature=1.0, grad=True),
+        # the answers of a preference batch over an odd-sized vocabulary
+        dict(name='logprob_train', op='logprob', rows=8192, vocab=50021, dtype='bf16', temperature=1.0, grad=True),
+        # one small batch of answer pairs
+        dict(name='preference_pairs', op='preference', lists=8, answers=2, tokens=777, kind='logistic', average=False),
+        # graded answers to many prompts, long answers
+        dict(name='preference_graded', op='preference', lists=512, answers=6, tokens=8192, kind='logistic', average=True),
+        # the scorer tower of the training benchmarks (136-512-512-512-1 with batch norm)
+        dict(name='adamw_tower', op='adamw', model='tower', width=512, layers=3, dtype='fp32', bits=32),
+        # a small language model's weights: many matrices and vectors
+        dict(name='adamw_layers', op='adamw', model='layers', width=1000, layers=12, dtype='fp32', bits=32),
+        # a larger one in bf16, with 8-bit states
+        dict(name='adamw_layers_8bit', op='adamw', model='layers', width=1280, layers=12, dtype='bf16', bits=8),
+    ]
+
+
+def _between(rng, low, high):
+    """A size between low and high, spread over its logarithm."""
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(['embed', 'logprob', 'preference', 'adamw'])
+    if op == 'embed':
+        grad = rng.random() < 0.75
+        pool = rng.choice(['none', 'none', 'sum', 'mean'])
+        tokens = 1 if pool == 'none' else _between(rng, 1, 200)
+        dim = _between(rng, 8, 4096)
+        lookups = _between(rng, 1, min(1 << 20, (1 << 28) // dim))
+        return dict(op=op, rows=_between(rng, 100, min(1 << 20, (1 << 28) // dim)), dim=dim, bags=max(1, lookups // tokens), tokens=tokens, pool=pool,
+                    dtype=rng.choice(['fp32', 'bf16', 'fp16']), ids=rng.choice(['int32', 'int64']), scale=rng.choice([1.0, 0.5, 20.0]), grad=grad)
+    if op == 'logprob':
+        vocab = _between(rng, 3, 200000)
+        return dict(op=op, rows=_between(rng, 1, min(65536, (1 << 28) // vocab)), vocab=vocab, dtype=rng.choice(['fp32', 'bf16', 'fp16']),
+                    temperature=rng.choice([1.0, 0.7, 2.0]), grad=rng.random() < 0.75)
+    if op == 'preference':
+        answers = rng.choice([2, 2, 3, 4, 8, 16])
+        tokens = _between(rng, 1, 32768)
+        return dict(op=op, lists=_between(rng, 1, max(1, (1 << 24) // (answers * tokens))), answers=answers, tokens=tokens,
+                    kind=rng.choice(['logistic', 'logistic', 'hinge', 'squared']), average=rng.random() < 0.5)
+    bits = rng.choice([8, 32])
+    return dict(op=op, model=rng.choice(['tower', 'layers']), width=_between(rng, 64, 1000), layers=rng.randint(2, 12), dtype=rng.choice(['fp32', 'bf16', 'fp16']), bits=bits)
+
+
+# ------------------------------------------------------------------------------------------------ sizes
+def _shapes(case):
+    """The parameter shapes of a model: a scorer tower, or the layers of a language model with its embedding."""
+    w = case['width']
+    if case['model'] == 'tower':
+        dims = [136] + [w] * case['layers']
+        shapes = [s for a, b in zip(dims, dims[1:]) for s in ((b, a), (b,), (b,), (b,))]
+        return shapes + [(1, w), (1,)]
+    layer = [(w,), (w, w), (w, w), (w, w), (w, w), (w,), (4 * w, w), (w, 4 * w)]
+    return [(8011, w)] + layer * case['layers'] + [(w,)]
+
+
+def _offsets(shapes):
+    """Where each tensor starts in a flat buffer (every start on a multiple of the quantisation block), and its length."""
+    sizes = [math.prod(s) for s in shapes]
+    starts = [0]
+    for n in sizes:
+        starts.append(starts[-1] + -(-n // _QBLOCK) * _QBLOCK)
+    return sizes, starts
+
+
+def work(case):
+    b = _BYTES.get(case.get('dtype'))
+    if case['op'] == 'embed':
+        n, d = case['bags'] * case['tokens'], case['dim']
+        idb = 4 if case['ids'] == 'int32' else 8
+        bytes_ = n * idb + min(n, case['rows']) * d * b + case['bags'] * d * b     # a row that many tokens name is read once
+        flops = n * d
+        if case['grad']:
+            bytes_ += n * idb + case['bags'] * d * b + case['rows'] * d * b
+            flops += n * d
+        return {'bytes': bytes_, 'flops': flops}
+    if case['op'] == 'logprob':
+        n = case['rows'] * case['vocab']
+        bytes_, flops = n * b + case['rows'] * 12, 4 * n
+        if case['grad']:
+            bytes_ += 2 * n * b + case['rows'] * 12
+            flops += 4 * n
+        return {'bytes': bytes_, 'flops': flops}
+    if case['op'] == 'preference':
+        n = case['lists'] * case['answers'] * case['tokens']
+        return {'bytes': 13 * n, 'flops': 3 * n}
+    n = sum(math.prod(s) for s in _shapes(case))
+    if case['bits'] == 32:
+        return {'bytes': n * (3 * b + 16), 'flops': 14 * n}
+    # the states are read and written in 8 bits, with their scales, and given back as the values they stand for
+    return {'bytes': n * (3 * b + 4 + 8) + n // _QBLOCK * 16, 'flops': 24 * n}
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _common_ids(g, n, rows):
+    """Token ids as text has them: a few very common, most rare (probability ~ 1 / rank), every fortieth a padding."""
+    u = torch.rand(n, generator=g, device='cuda', dtype=torch.float64)
+    rank = (torch.exp(u * math.log(rows + 1.0)).to(torch.int64) - 1).clamp_(0, rows - 1)
+    ids = (rank * 7919 + 13) % rows
+    pad = torch.rand(n, generator=g, device='cuda') < 0.025
+    return torch.where(pad, -1, ids)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+
+    def normal(*shape, dtype=torch.float32, times=1.0):
+        return (torch.randn(*shape, generator=g, device='cuda') * times).to(dtype)
+
+    s = {'case': case}
+    if case['op'] == 'embed':
+        dt = _DTYPES[case['dtype']]
+        ids = _common_ids(g, case['bags'] * case['tokens'], case['rows'])
+        if case['pool'] != 'none':
+            ids = ids.reshape(case['bags'], case['tokens'])
+        s['ids'] = ids.to(torch.int32 if case['ids'] == 'int32' else torch.int64)
+        s['table'] = normal(case['rows'], case['dim'], dtype=dt, times=0.02)
+        if case['grad']:
+            s['upstream'] = normal(case['bags'], case['dim'], dtype=dt)
+    elif case['op'] == 'logprob':
+        n, v = case['rows'], case['vocab']
+        logits = normal(n, v, dtype=_DTYPES[case['dtype']], times=3.0)
+        target = torch.randint(0, v, (n,), generator=g, device='cuda')
+        if v <= 1000:                                       # ranked lists are padded: items behind a list's end are masked
+            length = torch.randint(max(1, v // 2), v + 1, (n, 1), generator=g, device='cuda')
+            logits.masked_fill_(torch.arange(v, device='cuda') >= length, -math.inf)
+            target = torch.minimum(target, length[:, 0] - 1)
+        else:                                               # prompt tokens are no targets
+            target = torch.where(torch.rand(n, generator=g, device='cuda') < 0.1, -1, target) if n > 8 else target
+        s['logits'], s['target'] = logits, target
+        if case['grad']:
+            s['upstream'] = normal(n)
+    elif case['op'] == 'preference':
+        b, l, t = case['lists'], case['answers'], case['tokens']
+        s['log_probs'] = -normal(b, l, t).abs_()
+        s['reference'] = s['log_probs'] + normal(b, l, t, times=0.3)
+        length = torch.randint(0, t + 1, (b, l, 1), generator=g, device='cuda')
+        s['mask'] = torch.arange(t, device='cuda') < length
+        s['log_probs'].masked_fill_(~s['mask'], math.nan)      # what stands in padded places is never read
+        grade = torch.randint(-1 if l > 2 else 0, 5, (b, l), generator=g, device='cuda').float()   # -1: an answer that is not there
+        if l == 2:
+            grade = torch.tensor([1.0, 0.0], device='cuda').expand(b, l).contiguous()
+        s['grade'] = grade
+        s['weight'] = torch.rand(b, generator=g, device='cuda') + 0.5
+    else:
+        dt = _DTYPES[case['dtype']]
+        shapes = _shapes(case)
+        sizes, starts = _offsets(shapes)
+        n = starts[-1]
+        held = torch.zeros(n, dtype=torch.bool, device='cuda')
+        for at, size in zip(starts, sizes):
+            held[at:at + size] = True
+
+        def flat(dtype, times, square=False):
+            x = torch.randn(n, generator=g, device='cuda') * times
+            return (x * x if square else x).mul_(held).to(dtype)
+
+        s['param'], s['grad'] = flat(dt, 0.02), flat(dt, 1e-3)
+        cut = lambda x: [x[a:a + k].view(sh) for a, k, sh in zip(starts, sizes, shapes)]   # noqa: E731
+        if case['bits'] == 32:
+            s['m'], s['v'] = flat(torch.float32, 3e-4), flat(torch.float32, 1e-3, square=True)
+            s['tensors'] = [cut(s[k]) for k in ('param', 'grad', 'm', 'v')]
+        else:
+            blocks = n // _QBLOCK
+            s['m'] = torch.randint(-127, 128, (n,), generator=g, device='cuda').mul_(held).to(torch.int8)
+            s['v'] = torch.randint(1, 256, (n,), generator=g, device='cuda').mul_(held).to(torch.uint8)
+            s['m_scale'] = torch.rand(blocks, generator=g, device='cuda') * 4e-6 + 4e-6
+            s['v_scale'] = torch.rand(blocks, generator=g, device='cuda') * 4e-6 + 4e-6
+            whole = [(a, b) for a, b in zip(starts, starts[1:])]
+            s['tensors'] = [cut(s['param']), cut(s['grad'])] + [
+                [(s[k][a:b], s[k + '_scale'][a // _QBLOCK:b // _QBLOCK]) for a, b in whole] for k in ('m', 'v')]
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def _embed(s):
+    c, ids, table = s['case'], s['ids'].to(torch.int64), s['table']
+    there = ids >= 0
+    rows = table[ids.clamp(min=0)].to(torch.float32) * there.unsqueeze(-1)
+    share = None
+    if c['pool'] != 'none':
+        rows = rows.sum(1)
+        if c['pool'] == 'mean':
+            share = 1.0 / there.sum(1, keepdim=True).clamp(min=1).to(torch.float32)
+            rows = rows * share
+    out = [(rows * c['scale']).to(table.dtype)]
+    if c['grad']:
+        flat = ids.reshape(-1)
+        up = s['upstream'].to(torch.float32) if share is None else s['upstream'].to(torch.float32) * share
+        if table.dtype == torch.float32:
+            # common tokens are sums over many thousand rows: differences of a running sum in 64 bits over the sorted tokens
+            sorted_ids, order = flat.sort()
+            runs = torch.zeros(c['dim'], -(-flat.numel() // 1024) * 1024, dtype=torch.float64, device='cuda')
+            runs[:, :flat.numel()] = up[order // c['tokens']].t()
+            runs = runs.view(c['dim'], -1, 1024).cumsum(2)
+            total = runs[:, :, -1].cumsum(1)
+            runs[:, 1:] += total[:, :-1].unsqueeze(2)
+            runs = torch.cat([torch.zeros_like(total[:, :1]), runs.view(c['dim'], -1)], 1)
+            ends = torch.searchsorted(sorted_ids, torch.arange(-1, c['rows'], device='cuda'), right=True)
+            grad = (runs[:, ends[1:]] - runs[:, ends[:-1]]).t()
+        else:
+            grad = torch.zeros(c['rows'] + 1, c['dim'], device='cuda')            # the last row takes the padding
+            at = torch.where(flat >= 0, flat, c['rows'])
+            grad.index_add_(0, at, up if c['pool'] == 'none' else up.repeat_interleave(c['tokens'], 0))
+            grad = grad[:-1]
+        out.append((grad * c['scale']).to(table.dtype))
+    return out
+
+
+def _logprob(s):
+    c, target = s['case'], s['target']
+    there = target >= 0
+    at = target.clamp(min=0).unsqueeze(1)
+    z = s['logits'].to(torch.float32) / c['temperature']
+    z = z - z.amax(1, keepdim=True)
+    e = torch.exp(z)
+    total = e.sum(1, keepdim=True)
+    logp = (z.gather(1, at) - torch.log(total)).squeeze(1)
+    out = [torch.where(there, logp, 0.0)]
+    if c['grad']:
+        up = torch.where(there, s['upstream'], 0.0).unsqueeze(1) / c['temperature']
+        grad = e.mul_(-up / total)
+        grad.scatter_add_(1, at, up)
+        out.append(grad.to(s['logits'].dtype))
+    return out
+
+
+_CONFIDENCE, _SMOOTHING = 0.1, 0.05          # beta and label smoothing of the preference loss
+
+
+def _preference(s):
+    c, mask = s['case'], s['mask']
+    ratio = torch.where(mask, s['log_probs'] - s['reference'], 0.0).sum(2, dtype=torch.float64)
+    share = _CONFIDENCE / mask.sum(2).clamp(min=1) if c['average'] else torch.full_like(ratio, _CONFIDENCE)
+    score, grade = ratio * share, s['grade']
+    pair = (grade.unsqueeze(2) > grade.unsqueeze(1)) & (grade.unsqueeze(1) >= 0)
+    h = score.unsqueeze(2) - score.unsqueeze(1)
+    if c['kind'] == 'logistic':
+        loss = (1 - _SMOOTHING) * torch.log1p(torch.exp(-h.abs())) + (1 - _SMOOTHING) * (-h).clamp(min=0)
+        loss = loss + _SMOOTHING * (torch.log1p(torch.exp(-h.abs())) + h.clamp(min=0))
+        slope = 1 / (1 + torch.exp(-h)) - (1 - _SMOOTHING)
+    elif c['kind'] == 'hinge':
+        loss, slope = (1 - h).clamp(min=0), -(h < 1).to(h.dtype)
+    else:
+        loss, slope = (h - 0.5) * (h - 0.5), 2 * h - 1
+    pairs = pair.sum((1, 2)).clamp(min=1)
+    weight = s['weight'] / c['lists']
+    loss = (loss * pair).sum((1, 2)) / pairs * weight
+    slope = slope * pair
+    to_score = (slope.sum(2) - slope.sum(1)) / pairs.unsqueeze(1) * weight.unsqueeze(1)
+    grad = (to_score * share).unsqueeze(2) * mask
+    return [loss.sum().to(torch.float32), grad.to(torch.float32)]
+
+
+def _adamw(s):
+    c = s['case']
+    fix1, fix2 = 1 - _BETA1 ** _STEP, 1 - _BETA2 ** _STEP
+    grad = s['grad'].to(torch.float32)
+    if c['bits'] == 32:
+        s['m'].mul_(_BETA1).add_(grad * (1 - _BETA1))
+        s['v'].mul_(_BETA2).add_(grad * grad * (1 - _BETA2))
+        m, v, out = s['m'], s['v'], [s['m'], s['v']]
+    else:
+        # values next to a rounding border: the states' update and their rounding in 64 bits
+        deep = grad.to(torch.float64).view(-1, _QBLOCK)
+        m = s['m'].view(-1, _QBLOCK).to(torch.float64) * s['m_scale'].unsqueeze(1)
+        r = s['v'].view(-1, _QBLOCK).to(torch.float64) * s['v_scale'].unsqueeze(1)
+        m = _BETA1 * m + (1 - _BETA1) * deep
+        v = _BETA2 * (r * r) + (1 - _BETA2) * (deep * deep)
+        s['m_scale'].copy_(m.to(torch.float32).abs().amax(1) / 127)
+        s['v_scale'].copy_(torch.sqrt(v.to(torch.float32).amax(1)) / 255)
+        by_m, by_v = s['m_scale'].unsqueeze(1).to(torch.float64), s['v_scale'].unsqueeze(1).to(torch.float64)
+        code = torch.where(by_m > 0, m / by_m, 0.0).round().clamp(-127, 127)
+        root = torch.where((by_v > 0) & (v > 0), (torch.sqrt(v) / by_v).round().clamp(1, 255), 0.0)
+        s['m'].copy_(code.view(-1))
+        s['v'].copy_(root.view(-1))
+        r = root.to(torch.float32) * s['v_scale'].unsqueeze(1)
+        out = [(code.to(torch.float32) * s['m_scale'].unsqueeze(1)).view(-1), (r * r).view(-1)]
+        m, v = m.to(torch.float32).view(-1), v.to(torch.float32).view(-1)
+    step = m * (_LR / fix1) / (torch.sqrt(v) / math.sqrt(fix2) + _EPS)
+    s['param'].copy_(s['param'].to(torch.float32) * (1 - _LR * _DECAY) - step)
+    return [s['param']] + out
+
+
+def run(state):
+    c = state['case']
+    if not own:
+        return {'embed': _embed, 'logprob': _logprob, 'preference': _preference, 'adamw': _adamw}[c['op']](state)
+    if c['op'] == 'embed':
+        from ranking_amd.embedding import embedding_grad, embedding_lookup
+        how = dict(scale=c['scale'], combiner=None if c['pool'] == 'none' else c['pool'])
+        out = [embedding_lookup(state['table'], state['ids'], **how)]
+        if c['grad']:
+            out.append(embedding_grad(state['upstream'], state['ids'], c['rows'], **how))
+        return out
+    if c['op'] == 'logprob':
+        from ranking_amd.preference import token_log_probs, token_log_probs_grad, token_log_probs_with_stats
+        if not c['grad']:
+            return [token_log_probs(state['logits'], state['target'], temperature=c['temperature'])]
+        logp, stats = token_log_probs_with_stats(state['logits'], state['target'], temperature=c['temperature'])
+        return [logp, token_log_probs_grad(state['upstream'], state['logits'], state['target'], stats, temperature=c['temperature'])]
+    if c['op'] == 'preference':
+        from ranking_amd.keras.losses import PreferenceLoss
+        loss = PreferenceLoss(beta=_CONFIDENCE, kind=c['kind'], length_normalized=c['average'],
+                              label_smoothing=_SMOOTHING if c['kind'] == 'logistic' else 0.0)
+        return list(loss.loss_and_grad(state['grade'], state['log_probs'], state['weight'], reference=state['reference'], mask=state['mask']))
+    from ranking_amd import optim
+    params, grads, m, v = state['tensors']
+    optim.adamw_step(params, grads, m, v, step=_STEP, lr=_LR, betas=(_BETA1, _BETA2), eps=_EPS, weight_decay=_DECAY)
+    if c['bits'] == 32:
+        return [state['param'], state['m'], state['v']]
+    return [state['param'], optim.dequantize_exp_avg(state['m'], state['m_scale']), optim.dequantize_exp_avg_sq(state['v'], state['v_scale'])]
+
+
+# ------------------------------------------------------------------------------------------------ in 64 bits
+def exact(case, seed):
+    s = prepare(case, seed)
+    wide = torch.float64
+    if case['op'] == 'embed':
+        ids = s['ids'].to(torch.int64).view(case['bags'], case['tokens'])
+        per = (ids >= 0).sum(1).to(wide)
+        factor = torch.full_like(per, case['scale']) if case['pool'] != 'mean' else case['scale'] / torch.where(per > 0, per, 1.0)
+        pooled = torch.zeros(case['bags'], case['dim'], dtype=wide, device='cuda')
+        for t in range(case['tokens']):
+            here = (ids[:, t] >= 0).nonzero().squeeze(1)
+            pooled[here] += s['table'][ids[here, t]].to(wide)
+        out = [pooled * factor.unsqueeze(1)]
+        del pooled
+        if case['grad']:
+            grad = torch.zeros(case['rows'], case['dim'], dtype=wide, device='cuda')
+            up = s['upstream'].to(wide) * factor.unsqueeze(1)
+            for t in range(case['tokens']):
+                here = (ids[:, t] >= 0).nonzero().squeeze(1)
+                grad.index_put_((ids[here, t],), up[here], accumulate=True)
+            out.append(grad)
+        return out
+    if case['op'] == 'logprob':
+        n, there = case['rows'], s['target'] >= 0
+        logp, grads = torch.zeros(n, dtype=wide, device='cuda'), []
+        for a in range(0, n, 1024):
+            z = s['logits'][a:a + 1024].to(wide) / case['temperature']
+            k = z.shape[0]
+            lse = torch.logsumexp(z, 1)
+            t = s['target'][a:a + k]
+            row = torch.arange(k, device='cuda')
+            ok = there[a:a + k]
+            logp[a:a + k] = torch.where(ok, z[row, t.clamp(min=0)] - lse, 0.0)
+            if case['grad']:
+                p = -torch.exp(z - lse.unsqueeze(1))
+                p[row, t.clamp(min=0)] += 1.0
+                p *= torch.where(ok, s['upstream'][a:a + k].to(wide), 0.0).unsqueeze(1) / case['temperature']
+                grads.append(p)
+        return [logp, torch.cat(grads)] if case['grad'] else [logp]
+    if case['op'] == 'preference':
+        m = s['mask']
+        x = torch.nan_to_num(s['log_probs'].to(wide)).requires_grad_()
+        total = torch.zeros((), dtype=wide, device='cuda')
+        score = _CONFIDENCE * ((x - s['reference'].to(wide)) * m).sum(2)
+        if case['average']:
+            score = score / torch.where(m.any(2), m.sum(2), 1)
+        y = s['grade']
+        count = torch.zeros(case['lists'], dtype=wide, device='cuda')
+        loss = torch.zeros(case['lists'], dtype=wide, device='cuda')
+        for i in range(case['answers']):
+            for j in range(case['answers']):
+                use = ((y[:, i] > y[:, j]) & (y[:, j] >= 0)).to(wide)
+                h = score[:, i] - score[:, j]
+                if case['kind'] == 'logistic':
+                    value = -(1 - _SMOOTHING) * torch.nn.functional.logsigmoid(h) - _SMOOTHING * torch.nn.functional.logsigmoid(-h)
+                elif case['kind'] == 'hinge':
+                    value = torch.relu(1 - h)
+                else:
+                    value = (h - 0.5) ** 2
+                loss = loss + use * value
+                count = count + use
+        total = (loss / torch.where(count > 0, count, 1.0) * s['weight'].to(wide)).sum() / case['lists']
+        total.backward()
+        return [total.detach(), x.grad]
+    p, g = s['param'].to(wide), s['grad'].to(wide)
+    if case['bits'] == 32:
+        m0, v0 = s['m'].to(wide), s['v'].to(wide)
+    else:
+        m0 = s['m'].to(wide) * s['m_scale'].to(wide).repeat_interleave(_QBLOCK)
+        v0 = torch.square(s['v'].to(wide) * s['v_scale'].to(wide).repeat_interleave(_QBLOCK))
+    m1 = m0 * _BETA1 + g * (1 - _BETA1)
+    v1 = v0 * _BETA2 + g.square() * (1 - _BETA2)
+    p1 = p - _LR * _DECAY * p - _LR * (m1 / (1 - _BETA1 ** _STEP)) / ((v1 / (1 - _BETA2 ** _STEP)).sqrt() + _EPS)
+    if case['bits'] == 32:
+        return [p1, m1, v1]
+    held = []                        # the scales are held in 32 bits, the codes are the nearest to the values they stand for
+    for x, top in ((m1, 127), (v1.sqrt(), 255)):
+        x = x.view(-1, _QBLOCK)
+        if top == 127:
+            scale = (x.abs().amax(1).float() / top).to(wide).unsqueeze(1)
+        else:
+            scale = (torch.sqrt(x.square().amax(1).float()) / top).to(wide).unsqueeze(1)
+        code = torch.where(scale > 0, torch.round(x / torch.where(scale > 0, scale, 1.0)), 0.0)
+        if top == 255:
+            code = torch.where((x > 0) & (scale > 0), code.clamp(1, 255), 0.0)
+        held.append((code * scale).view(-1))
+    return [p1, held[0], held[1].square()]
