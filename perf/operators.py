@@ -297,8 +297,8 @@ def _adamw(s):
         r = s['v'].view(-1, _QBLOCK).to(torch.float64) * s['v_scale'].unsqueeze(1)
         m = _BETA1 * m + (1 - _BETA1) * deep
         v = _BETA2 * (r * r) + (1 - _BETA2) * (deep * deep)
-        s['m_scale'].copy_(m.to(torch.float32).abs().amax(1) / 127)
-        s['v_scale'].copy_(torch.sqrt(v.to(torch.float32).amax(1)) / 255)
+        s['m_scale'].copy_(m.to(torch.float32).abs().amax(1).to(torch.float64) / 127)
+        s['v_scale'].copy_(torch.sqrt(v.to(torch.float32).amax(1).to(torch.float64)) / 255)
         by_m, by_v = s['m_scale'].unsqueeze(1).to(torch.float64), s['v_scale'].unsqueeze(1).to(torch.float64)
         code = torch.where(by_m > 0, m / by_m, 0.0).round().clamp(-127, 127)
         root = torch.where((by_v > 0) & (v > 0), (torch.sqrt(v) / by_v).round().clamp(1, 255), 0.0)
@@ -420,10 +420,8 @@ def exact(case, seed):
     held = []                        # the scales are held in 32 bits, the codes are the nearest to the values they stand for
     for x, top in ((m1, 127), (v1.sqrt(), 255)):
         x = x.view(-1, _QBLOCK)
-        if top == 127:
-            scale = (x.abs().amax(1).float() / top).to(wide).unsqueeze(1)
-        else:
-            scale = (torch.sqrt(x.square().amax(1).float()) / top).to(wide).unsqueeze(1)
+        most = x.abs().amax(1).float().to(wide) if top == 127 else x.square().amax(1).float().to(wide).sqrt()
+        scale = (most / top).float().to(wide).unsqueeze(1)
         code = torch.where(scale > 0, torch.round(x / torch.where(scale > 0, scale, 1.0)), 0.0)
         if top == 255:
             code = torch.where((x > 0) & (scale > 0), code.clamp(1, 255), 0.0)
