@@ -605,6 +605,84 @@ int tfr_group_scatter_avg_bwd_f32(const float* dlogits, const float* counts, con
                                   const uint8_t* gmask, int B, int L, int G, int group_size,
                                   float* dscores_out, void* stream);
 
+/* ---- training on token features and preferences --------------------------------------------------------------------
+ * The entry points below take fp32, bf16 or fp16 tensors; arithmetic is fp32 (fp64 where said), results are rounded once. */
+#define TFR_DTYPE_F32 0
+#define TFR_DTYPE_BF16 1
+#define TFR_DTYPE_F16 2
+#define TFR_IDS_I32 0
+#define TFR_IDS_I64 1
+#define TFR_COMBINER_NONE 0   /* tokens == 1: one row of the table a lookup */
+#define TFR_COMBINER_SUM 1
+#define TFR_COMBINER_MEAN 2   /* over the ids >= 0 of a bag */
+
+/* Embedding lookup: out[b] = f_b * sum_t table[ids[b, t]], f_b = scale, with TFR_COMBINER_MEAN scale / #{t : ids[b, t] >= 0}.
+ * ids < 0 are padding (nothing is added); ids >= rows add NaN.
+ *   table [rows, dim] with row pitch ld (elements), ids [bags, tokens] dense, out [bags, dim] dense, both of `dtype`.
+ * rows, bags and bags * tokens at most 2^25. */
+int tfr_embedding_lookup(const void* table, long ld, long rows, int dim, int dtype, const void* ids, int id_type,
+                         long bags, int tokens, int combiner, float scale, void* out, void* stream);
+/* Its gradient: grad_table[v] = sum over (b, t) with ids[b, t] == v of f_b * grad[b], every row of it written once.  Sums are
+ * fp32 in an order that depends on the ids alone: the same ids and gradients give the same bits.
+ *   grad [bags, dim], grad_table [rows, dim] dense, both of `dtype`; workspace: 16-byte aligned. */
+long tfr_embedding_grad_workspace_bytes(long rows, int dim, long bags, int tokens, int combiner);
+int tfr_embedding_grad(const void* grad, int dtype, const void* ids, int id_type, long bags, int tokens, int combiner,
+                       float scale, long rows, int dim, void* grad_table, void* workspace, long workspace_bytes,
+                       void* stream);
+
+/* logp[n] = (x[n, y_n] - lse_n) with x = logits / temperature and lse_n = log sum_v exp x[n, v]; n = (b, t), the row at
+ * logits + b * stride_b + t * stride_t (elements; t < per).  target < 0: logp 0 and the row is not read; target >= vocab: NaN.
+ *   stats nullable [n, 2]: (max of the row, sum of exponentials) for the gradient
+ *   dlogits [n, vocab] dense = upstream[n] / temperature * (1{v = y_n} - softmax), rows without a target are zero.
+ * n below 2^24, vocab at most 2^28; workspace: tfr_token_logprob_workspace_bytes (0 where rows are not split). */
+long tfr_token_logprob_workspace_bytes(long n, int vocab);
+int tfr_token_logprob(const void* logits, int dtype, long per, long stride_b, long stride_t, const int64_t* target, long n,
+                      int vocab, float temperature, float* logp, float* stats, void* workspace, long workspace_bytes,
+                      void* stream);
+int tfr_token_logprob_grad(const void* logits, int dtype, long per, long stride_b, long stride_t, const int64_t* target,
+                           const float* stats, const float* upstream, long n, int vocab, float temperature, void* dlogits,
+                           void* stream);
+
+/* Preference loss of lists of L answers (at most 64) of T tokens: with s_i = beta * sum_t m (log_probs - reference), divided by
+ * the answer's number of tokens when `normalize`, the mean over the pairs y_i > y_j >= 0 of a list of
+ *   TFR_PREFERENCE_LOGISTIC (1 - smoothing) softplus(-(s_i - s_j)) + smoothing softplus(s_i - s_j)   (0 <= smoothing < 1/2)
+ *   TFR_PREFERENCE_HINGE    max(0, 1 - (s_i - s_j))
+ *   TFR_PREFERENCE_SQUARED  (s_i - s_j - 1/2)^2
+ * times scale and the list's weight.  Sums are fp64.  reference, mask (uint8 [B, L, T]), list_weights ([B]) are nullable.
+ *   loss [B];  coef [B, L] = d loss[b] / d (any unmasked log prob of the answer); the gradient spreads it over the tokens,
+ *   times upstream[b] (nullable).  B * L below 2^24, T at most 2^28; workspace: 8-byte aligned. */
+#define TFR_PREFERENCE_LOGISTIC 0
+#define TFR_PREFERENCE_HINGE 1
+#define TFR_PREFERENCE_SQUARED 2
+long tfr_preference_workspace_bytes(int B, int L, int T);
+int tfr_preference_loss_f32(const float* log_probs, const float* reference, const uint8_t* mask, const float* labels,
+                            const float* list_weights, int B, int L, int T, int kind, float beta, float smoothing,
+                            int normalize, float scale, float* loss, float* coef, void* workspace, long workspace_bytes, void* stream);
+int tfr_preference_grad_f32(const float* coef, const float* upstream, const uint8_t* mask, int B, int L, int T,
+                            float* dlog_probs, void* stream);
+
+/* AdamW (decoupled weight decay) on up to TFR_ADAMW_MAX_TENSORS tensors in one launch; the arrays named _host live in host
+ * memory and hold device pointers and element counts.  Parameters and gradients of `dtype`, moments fp32; `step` counts from
+ * 1; with `now` (device, from tfr_adamw_advance) the step's coefficients come from the device and lr / step are not used. */
+#define TFR_ADAMW_MAX_TENSORS 88
+#define TFR_ADAMW8_MAX_TENSORS 64
+#define TFR_ADAMW_QBLOCK 128
+int tfr_adamw(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+              void* const* exp_avg_sqs_host, const int64_t* sizes_host, double lr, double beta1, double beta2, double eps,
+              double weight_decay, int64_t step, const float* now, void* stream);
+/* The same with 8-bit moments: TFR_ADAMW_QBLOCK consecutive elements share a scale.  exp_avg = code * scale with codes -127 ..
+ * 127 (-128: NaN), exp_avg_sq = (code * scale)^2 with codes 0 .. 255; codes in tensors of whole blocks, 8-byte aligned. */
+int tfr_adamw8(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+               float* const* exp_avg_scales_host, void* const* exp_avg_sqs_host, float* const* exp_avg_sq_scales_host,
+               const int64_t* sizes_host, double lr, double beta1, double beta2, double eps, double weight_decay,
+               int64_t step, const float* now, void* stream);
+/* step[0] += 1 on the device, then now[3] = (1 - lr * weight_decay, lr / (1 - beta1^step), 1 / sqrt(1 - beta2^step)); lr from
+ * lr_device when given: a step that is replayed from a hipGraph keeps counting and follows its learning rate. */
+int tfr_adamw_advance(int64_t* step, const float* lr_device, double lr, double beta1, double beta2, double weight_decay,
+                      float* now, void* stream);
+/* out[i] = codes[i] * scale (square: its square): what the 8-bit moments stand for; n a multiple of TFR_ADAMW_QBLOCK. */
+int tfr_adamw_dequantize(const void* codes, const float* scales, long n, int square, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,9 @@ from . import losses_impl     # noqa: F401
 from . import metrics_impl    # noqa: F401
 from . import losses          # noqa: F401
 from . import metrics         # noqa: F401
+from . import embedding       # noqa: F401
+from . import preference      # noqa: F401
+from . import optim           # noqa: F401
 from . import keras           # noqa: F401
 
 __version__ = '0.1.0'

@@ -18,7 +18,12 @@ LIB_PATH = os.path.join(CSRC, 'libtfr_hip.so')
 STAMP_PATH = LIB_PATH + '.stamp'                           # fingerprint of what LIB_PATH was built from
 PROF_LIB_PATH = os.path.join(CSRC, 'libtfr_hip_prof.so')     # developer aid: -DTFR_PROFILE_STAMPS build
 SOURCES = ['sort_metrics.hip', 'approx_ndcg.hip', 'pairwise.hip', 'softmax_gumbel.hip', 'tower.hip', 'listwise.hip',
-           'neural_sort.hip', 'pointwise.hip', 'groupwise.hip', 'gemm_f32.hip']
+           'neural_sort.hip', 'pointwise.hip', 'groupwise.hip', 'gemm_f32.hip', 'embedding.hip', 'token_logprob.hip',
+           'preference.hip', 'adamw.hip']
+# Per-source additions: hipcc forms packed fp32 instructions from plain float code, some of which have given wrong results; the
+# kernels that do not write such code on purpose are compiled without them.
+_NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+SOURCE_FLAGS = {s: _NO_PACKED_FP32 for s in ('embedding.hip', 'token_logprob.hip', 'preference.hip', 'adamw.hip')}
 HIPCC_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-ffp-contract=off', '-fPIC', '-shared',
                '-fvisibility=default']
 
@@ -161,6 +166,29 @@ _SIGNATURES = {
     'tfr_group_scatter_avg_f32': (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int] * 4 + [ctypes.c_void_p] * 3),
     'tfr_group_scatter_avg_bwd_f32': (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int] * 4
                                       + [ctypes.c_void_p] * 2),
+    # token features, token log probabilities, preferences (embedding.hip, token_logprob.hip, preference.hip)
+    'tfr_embedding_lookup': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                            ctypes.c_int, ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_float]
+                             + [ctypes.c_void_p] * 2),
+    'tfr_embedding_grad_workspace_bytes': (ctypes.c_long, [ctypes.c_long, ctypes.c_int, ctypes.c_long, ctypes.c_int, ctypes.c_int]),
+    'tfr_embedding_grad': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_int,
+                                          ctypes.c_int, ctypes.c_float, ctypes.c_long, ctypes.c_int, ctypes.c_void_p] + _WS),
+    'tfr_token_logprob_workspace_bytes': (ctypes.c_long, [ctypes.c_long, ctypes.c_int]),
+    'tfr_token_logprob': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_long] * 3 + [ctypes.c_void_p, ctypes.c_long, ctypes.c_int,
+                                         ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p] + _WS),
+    'tfr_token_logprob_grad': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_long] * 3 + [ctypes.c_void_p] * 3
+                               + [ctypes.c_long, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]),
+    'tfr_preference_workspace_bytes': (ctypes.c_long, [ctypes.c_int] * 3),
+    'tfr_preference_loss_f32': (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int] * 4 + [ctypes.c_float] * 2
+                                + [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p] + _WS),
+    'tfr_preference_grad_f32': (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2),
+    # optimizer (adamw.hip): pointer tables live in host memory
+    'tfr_adamw': (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_void_p] * 5 + [ctypes.c_double] * 5
+                  + [ctypes.c_int64] + [ctypes.c_void_p] * 2),
+    'tfr_adamw8': (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_void_p] * 7 + [ctypes.c_double] * 5
+                   + [ctypes.c_int64] + [ctypes.c_void_p] * 2),
+    'tfr_adamw_advance': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_double] * 4 + [ctypes.c_void_p] * 2),
+    'tfr_adamw_dequantize': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_long, ctypes.c_int] + [ctypes.c_void_p] * 2),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -184,7 +212,7 @@ def _deps():
 def _fingerprint() -> str:
     """sha256 over the sources, the public header and the compiler flags: what the in-tree .so was built from."""
     import hashlib
-    h = hashlib.sha256(' '.join(HIPCC_FLAGS).encode())
+    h = hashlib.sha256((' '.join(HIPCC_FLAGS) + repr(sorted(SOURCE_FLAGS.items()))).encode())
     for d in _deps():
         h.update(os.path.basename(d).encode())
         with open(d, 'rb') as f:
@@ -231,7 +259,7 @@ class _BuildLock:
 def _source_fingerprint(src: str) -> str:
     """What one object file depends on: its source, the shared headers and the compile flags."""
     import hashlib
-    h = hashlib.sha256(' '.join(COMPILE_FLAGS).encode())
+    h = hashlib.sha256(' '.join(COMPILE_FLAGS + SOURCE_FLAGS.get(src, [])).encode())
     deps = [os.path.join(CSRC, src)] + [d for d in _deps() if d.endswith('.h')]
     for d in deps:
         h.update(os.path.basename(d).encode())
@@ -251,7 +279,7 @@ def _compile_one(hipcc: str, src: str, verbose: bool) -> str:
     except OSError:
         pass
     tmp = '%s.%d.tmp' % (obj, os.getpid())
-    cmd = [hipcc] + COMPILE_FLAGS + ['-I', INCLUDE, '-c', os.path.join(CSRC, src), '-o', tmp]
+    cmd = [hipcc] + COMPILE_FLAGS + SOURCE_FLAGS.get(src, []) + ['-I', INCLUDE, '-c', os.path.join(CSRC, src), '-o', tmp]
     if verbose:
         print(' '.join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,0 +1,346 @@
+// AdamW over many tensors in one launch, with the moments held in 32 or in 8 bits (gfx950).
+//
+//   m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2
+//   p <- p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// HBM-bound: with fp32 parameters and moments 16 bytes are read and 12 written an element.  The addresses and lengths of up to
+// TFR_ADAMW_MAX_TENSORS (TFR_ADAMW8_MAX_TENSORS) tensors travel in the kernel's arguments: no table in device memory that a
+// step would have to copy first (the gradients' addresses change from step to step), and a captured launch holds its own.
+//
+// 8 bits: QBLOCK consecutive elements share two scales.  m is held as a signed code of -127 .. 127, the root of v as an unsigned
+// code of 0 .. 255; the root halves the exponent range that 255 steps have to cover.  Codes are the nearest to the updated
+// value, but the code of a positive v is at least 1: a denominator is never rounded down to eps, so small second moments slow
+// an element down and never blow it up.  The update and the choice of the codes run in fp64: a code is one of 255 steps, and
+// which one a value next to a border gets must not hang on fp32 rounding (~25 fp64 operations an element: a third of the memory
+// time).  The parameter's own update uses the moments before they are rounded to codes.  An element whose moments are no longer
+// finite keeps the code -128, which stands for NaN, and does not touch its neighbours' scale.
+#include "common.h"
+#include "elem.h"
+
+using namespace tfr;
+
+namespace {
+
+constexpr int QBLOCK = TFR_ADAMW_QBLOCK;
+
+struct Coef {
+  double b1, c1, b2, c2;               // beta and 1 - beta
+  float decay, step, root, eps;        // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  const float* now;                    // device (decay, step, root) of a step that is counted on the device, or null
+};
+
+template <int CAP, bool Q>
+struct Table {
+  Coef coef;
+  int count;
+  int first[CAP + 1];                  // first workgroup of each tensor
+  void* p[CAP];
+  const void* g[CAP];
+  void* m[CAP];
+  void* v[CAP];
+  float* ms[Q ? CAP : 1];
+  float* vs[Q ? CAP : 1];
+  long n[CAP];
+};
+typedef Table<TFR_ADAMW_MAX_TENSORS, false> Table32;
+typedef Table<TFR_ADAMW8_MAX_TENSORS, true> Table8;
+static_assert(sizeof(Table32) <= 4096 && sizeof(Table8) <= 4096, "kernel arguments hold 4 KB");
+
+template <typename Tab>
+__device__ __forceinline__ int tensor_of(const Tab& t, int block) {
+  int lo = 0, hi = t.count;            // t.first[lo] <= block < t.first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.first[mid] <= block) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+struct Now { float decay, step, root; };
+__device__ __forceinline__ Now now_of(const Coef& c) {
+  Now w = {c.decay, c.step, c.root};
+  if (c.now) w = {c.now[0], c.now[1], c.now[2]};
+  return w;
+}
+
+__device__ __forceinline__ float updated(float p, float m, float v, const Now& w, float eps) {
+  return p * w.decay - m * w.step / (sqrtf(v) * w.root + eps);
+}
+
+constexpr int BLOCK32 = 4096;          // elements of a workgroup
+constexpr int BLOCK8 = 4096;
+
+template <typename T>
+__global__ __launch_bounds__(256) void adamw_kernel(const Table32 t) {
+  const int i = tensor_of(t, blockIdx.x);
+  const long n = t.n[i], base = (long)(blockIdx.x - t.first[i]) * BLOCK32;
+  T* __restrict__ p = (T*)t.p[i] + base;
+  const T* __restrict__ g = (const T*)t.g[i] + base;
+  float* __restrict__ m = (float*)t.m[i] + base;
+  float* __restrict__ v = (float*)t.v[i] + base;
+  const Now w = now_of(t.coef);
+  const float b1 = (float)t.coef.b1, c1 = (float)t.coef.c1, b2 = (float)t.coef.b2, c2 = (float)t.coef.c2, eps = t.coef.eps;
+  const int left = (int)(n - base < BLOCK32 ? n - base : BLOCK32);
+  const bool wide = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0;
+  if (wide && left == BLOCK32) {
+#pragma unroll
+    for (int k = 0; k < BLOCK32 / 1024; ++k) {
+      const int at = k * 1024 + threadIdx.x * 4;
+      float pe[4], ge[4], me[4], ve[4];
+      load_pack<T, 4>(p + at, pe);
+      load_pack<T, 4>(g + at, ge);
+      load_pack<float, 4>(m + at, me);
+      load_pack<float, 4>(v + at, ve);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        me[e] = b1 * me[e] + c1 * ge[e];
+        ve[e] = b2 * ve[e] + c2 * (ge[e] * ge[e]);
+        pe[e] = updated(pe[e], me[e], ve[e], w, eps);
+      }
+      store_pack<float, 4>(m + at, me);
+      store_pack<float, 4>(v + at, ve);
+      store_pack<T, 4>(p + at, pe);
+    }
+    return;
+  }
+  for (int at = threadIdx.x; at < left; at += 256) {
+    const float ge = (float)g[at];
+    const float me = b1 * m[at] + c1 * ge, ve = b2 * v[at] + c2 * (ge * ge);
+    m[at] = me;
+    v[at] = ve;
+    p[at] = (T)updated((float)p[at], me, ve, w, eps);
+  }
+}
+
+// A thread takes 8 consecutive elements, 16 lanes a scale.  The codes lie in whole blocks (their tensors are padded), the
+// parameters and gradients end where they end.
+template <typename T>
+__global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
+  const int i = tensor_of(t, blockIdx.x);
+  const long n = t.n[i], base = (long)(blockIdx.x - t.first[i]) * BLOCK8;
+  T* __restrict__ p = (T*)t.p[i];
+  const T* __restrict__ g = (const T*)t.g[i];
+  int8_t* __restrict__ m = (int8_t*)t.m[i];
+  uint8_t* __restrict__ v = (uint8_t*)t.v[i];
+  float* __restrict__ ms = t.ms[i];
+  float* __restrict__ vs = t.vs[i];
+  const Now w = now_of(t.coef);
+  const double b1 = t.coef.b1, c1 = t.coef.c1, b2 = t.coef.b2, c2 = t.coef.c2;
+  const float eps = t.coef.eps;
+  constexpr int W = sizeof(T) == 4 ? 4 : 8;                    // elements of a 16-byte access
+  const bool wide = (((uintptr_t)p | (uintptr_t)g) & 15) == 0;
+  const long padded = (n + QBLOCK - 1) / QBLOCK * QBLOCK;
+  for (int k = 0; k < BLOCK8 / 2048; ++k) {
+    const long at = base + k * 2048 + threadIdx.x * 8;
+    if (at >= padded) return;                                   // whole groups of 16 lanes
+    float pe[8], ge[8];
+    const bool whole = wide && at + 8 <= n;
+    if (whole) {
+#pragma unroll
+      for (int q = 0; q < 8; q += W) {
+        load_pack<T, W>(p + at + q, *reinterpret_cast<float(*)[W]>(pe + q));
+        load_pack<T, W>(g + at + q, *reinterpret_cast<float(*)[W]>(ge + q));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pe[e] = at + e < n ? (float)p[at + e] : 0.f;
+        ge[e] = at + e < n ? (float)g[at + e] : 0.f;
+      }
+    }
+    const uint2 mw = *reinterpret_cast<const uint2*>(m + at), vw = *reinterpret_cast<const uint2*>(v + at);
+    const double sm = (double)ms[at / QBLOCK], sv = (double)vs[at / QBLOCK];
+    double md[8], vd[8];
+    float most_m = 0.f, most_v = 0.f;
+    unsigned lost = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int mc = (int)(int8_t)((e < 4 ? mw.x : mw.y) >> (8 * (e & 3)));
+      const int vc = (int)(((e < 4 ? vw.x : vw.y) >> (8 * (e & 3))) & 255u);
+      const double gd = (double)ge[e], r = (double)vc * sv;
+      md[e] = b1 * ((double)mc * sm) + c1 * gd;
+      vd[e] = b2 * (r * r) + c2 * (gd * gd);
+      float m32 = (float)md[e];
+      const float v32 = (float)vd[e];
+      if (mc == -128) m32 = __builtin_nanf("");
+      pe[e] = updated(pe[e], m32, v32, w, eps);
+      const bool bad = !(fabsf(m32) < INFINITY) || !(v32 < INFINITY);
+      lost |= bad ? 1u << e : 0u;
+      most_m = fmaxf(most_m, bad ? 0.f : fabsf(m32));
+      most_v = fmaxf(most_v, bad ? 0.f : v32);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      most_m = fmaxf(most_m, __shfl_xor(most_m, o, 64));
+      most_v = fmaxf(most_v, __shfl_xor(most_v, o, 64));
+    }
+    // in fp64 and rounded once, so that the scale is the same wherever it is computed
+    const float new_sm = (float)((double)most_m / 127.0), new_sv = (float)(sqrt((double)most_v) / 255.0);
+    const double over_m = new_sm > 0.f ? 1.0 / (double)new_sm : 0.0, over_v = new_sv > 0.f ? 1.0 / (double)new_sv : 0.0;
+    const double wide_v = (double)new_sv;
+    uint2 mo = make_uint2(0u, 0u), vo = make_uint2(0u, 0u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int mc = (int)fmin(fmax(rint(md[e] * over_m), -127.0), 127.0);
+      // nearest code of the root without a root in fp64: the fp32 one is off by at most a step, two squares decide
+      double kd = fmin(rint((double)sqrtf((float)vd[e]) * over_v), 255.0);
+      const double lo = (kd - 0.5) * wide_v, hi = (kd + 0.5) * wide_v;
+      kd += vd[e] < lo * lo && kd > 0.0 ? -1.0 : vd[e] > hi * hi ? 1.0 : 0.0;
+      int vc = (int)fmin(fmax(kd, 1.0), 255.0);
+      if (!(vd[e] > 0.0) || !(new_sv > 0.f)) vc = 0;
+      if (lost & (1u << e)) {
+        mc = -128;
+        vc = 255;
+      }
+      const unsigned mb = ((unsigned)mc & 255u) << (8 * (e & 3)), vb = (unsigned)vc << (8 * (e & 3));
+      if (e < 4) {
+        mo.x |= mb;
+        vo.x |= vb;
+      } else {
+        mo.y |= mb;
+        vo.y |= vb;
+      }
+    }
+    *reinterpret_cast<uint2*>(m + at) = mo;
+    *reinterpret_cast<uint2*>(v + at) = vo;
+    if ((threadIdx.x & 15) == 0) {
+      ms[at / QBLOCK] = new_sm;
+      vs[at / QBLOCK] = new_sv;
+    }
+    if (whole) {
+#pragma unroll
+      for (int q = 0; q < 8; q += W) store_pack<T, W>(p + at + q, *reinterpret_cast<float(*)[W]>(pe + q));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (at + e < n) p[at + e] = (T)pe[e];
+    }
+  }
+}
+
+// The values that codes stand for: 8 a thread.
+template <bool SQUARE>
+__global__ __launch_bounds__(256) void adamw_dequantize_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, long n,
+                                                               float* __restrict__ out) {
+  const long at = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= n) return;
+  const uint2 c = *reinterpret_cast<const uint2*>(codes + at);
+  const float s = scales[at / QBLOCK];
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const unsigned b = ((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 255u;
+    if (SQUARE) {
+      const float r = (float)b * s;
+      v[e] = r * r;
+    } else {
+      v[e] = b == 128u ? __builtin_nanf("") : (float)(int8_t)b * s;
+    }
+  }
+  store_pack<float, 4>(out + at, *reinterpret_cast<float(*)[4]>(v));
+  store_pack<float, 4>(out + at + 4, *reinterpret_cast<float(*)[4]>(v + 4));
+}
+
+// One more step, counted on the device: coefficients of the launch behind it.
+__global__ void adamw_advance_kernel(long* __restrict__ count, const float* __restrict__ lr_now, double lr, double b1, double b2, double decay,
+                                     float* __restrict__ now) {
+  const long t = count[0] + 1;
+  count[0] = t;
+  if (lr_now) lr = (double)lr_now[0];
+  now[0] = (float)(1.0 - lr * decay);
+  now[1] = (float)(lr / (1.0 - pow(b1, (double)t)));
+  now[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+}
+
+bool bad_betas(double b1, double b2) { return !(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0); }
+
+template <typename Tab, int PER>
+int fill(Tab& t, int cap, int count, void* const* p, const void* const* g, void* const* m, void* const* v, const int64_t* n, double lr,
+         double b1, double b2, double eps, double decay, int64_t step, const float* now) {
+  if (count < 1 || count > cap || !p || !g || !m || !v || !n || bad_betas(b1, b2)) return TFR_EINVAL;
+  if (!now && step < 1) return TFR_EINVAL;
+  t.coef.b1 = b1;
+  t.coef.c1 = 1.0 - b1;
+  t.coef.b2 = b2;
+  t.coef.c2 = 1.0 - b2;
+  t.coef.eps = (float)eps;
+  t.coef.now = now;
+  t.coef.decay = (float)(1.0 - lr * decay);
+  t.coef.step = now ? 0.f : (float)(lr / (1.0 - __builtin_pow(b1, (double)step)));
+  t.coef.root = now ? 0.f : (float)(1.0 / __builtin_sqrt(1.0 - __builtin_pow(b2, (double)step)));
+  t.count = count;
+  long at = 0;
+  for (int i = 0; i < count; ++i) {
+    if (n[i] < 0 || (n[i] > 0 && (!p[i] || !g[i] || !m[i] || !v[i]))) return TFR_EINVAL;
+    t.first[i] = (int)at;
+    t.p[i] = p[i];
+    t.g[i] = g[i];
+    t.m[i] = m[i];
+    t.v[i] = v[i];
+    t.n[i] = n[i];
+    at += (n[i] + PER - 1) / PER;
+    if (at >= (1l << 24)) return TFR_EINVAL;                    // no grid of 2^32 threads
+  }
+  t.first[count] = (int)at;
+  return TFR_OK;
+}
+
+}  // namespace
+
+extern "C" int tfr_adamw(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+                         void* const* exp_avg_sqs_host, const int64_t* sizes_host, double lr, double beta1, double beta2, double eps,
+                         double weight_decay, int64_t step, const float* now, void* stream) {
+  if (!elem_known(dtype)) return TFR_EINVAL;
+  Table32 t;
+  const int rc = fill<Table32, BLOCK32>(t, TFR_ADAMW_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_sqs_host, sizes_host,
+                                        lr, beta1, beta2, eps, weight_decay, step, now);
+  if (rc != TFR_OK) return rc;
+  const int blocks = t.first[count];
+  if (blocks == 0) return TFR_OK;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == TFR_DTYPE_F32) adamw_kernel<float><<<blocks, 256, 0, st>>>(t);
+  else if (dtype == TFR_DTYPE_BF16) adamw_kernel<__bf16><<<blocks, 256, 0, st>>>(t);
+  else adamw_kernel<_Float16><<<blocks, 256, 0, st>>>(t);
+  return (int)hipGetLastError();
+}
+
+extern "C" int tfr_adamw8(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+                          float* const* exp_avg_scales_host, void* const* exp_avg_sqs_host, float* const* exp_avg_sq_scales_host,
+                          const int64_t* sizes_host, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                          const float* now, void* stream) {
+  if (!elem_known(dtype) || !exp_avg_scales_host || !exp_avg_sq_scales_host) return TFR_EINVAL;
+  Table8 t;
+  const int rc = fill<Table8, BLOCK8>(t, TFR_ADAMW8_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_sqs_host, sizes_host,
+                                      lr, beta1, beta2, eps, weight_decay, step, now);
+  if (rc != TFR_OK) return rc;
+  for (int i = 0; i < count; ++i) {
+    t.ms[i] = exp_avg_scales_host[i];
+    t.vs[i] = exp_avg_sq_scales_host[i];
+    if (t.n[i] > 0 && (!t.ms[i] || !t.vs[i] || (((uintptr_t)t.m[i] | (uintptr_t)t.v[i]) & 7))) return TFR_EINVAL;
+  }
+  const int blocks = t.first[count];
+  if (blocks == 0) return TFR_OK;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == TFR_DTYPE_F32) adamw8_kernel<float><<<blocks, 256, 0, st>>>(t);
+  else if (dtype == TFR_DTYPE_BF16) adamw8_kernel<__bf16><<<blocks, 256, 0, st>>>(t);
+  else adamw8_kernel<_Float16><<<blocks, 256, 0, st>>>(t);
+  return (int)hipGetLastError();
+}
+
+extern "C" int tfr_adamw_advance(int64_t* step, const float* lr_device, double lr, double beta1, double beta2, double weight_decay, float* now,
+                                 void* stream) {
+  if (!step || !now || bad_betas(beta1, beta2)) return TFR_EINVAL;
+  adamw_advance_kernel<<<1, 1, 0, (hipStream_t)stream>>>((long*)step, lr_device, lr, beta1, beta2, weight_decay, now);
+  return (int)hipGetLastError();
+}
+
+extern "C" int tfr_adamw_dequantize(const void* codes, const float* scales, long n, int square, float* out, void* stream) {
+  if (n < 0 || n % QBLOCK || n > (1l << 33)) return TFR_EINVAL;
+  if (n == 0) return TFR_OK;
+  if (!codes || !scales || !out || ((uintptr_t)codes & 7) || ((uintptr_t)out & 15)) return TFR_EINVAL;
+  const unsigned blocks = (unsigned)((n + 2047) / 2048);
+  hipStream_t st = (hipStream_t)stream;
+  if (square) adamw_dequantize_kernel<true><<<blocks, 256, 0, st>>>((const uint8_t*)codes, scales, n, out);
+  else adamw_dequantize_kernel<false><<<blocks, 256, 0, st>>>((const uint8_t*)codes, scales, n, out);
+  return (int)hipGetLastError();
+}

@@ -83,6 +83,38 @@ def create_tower(hidden_layer_dims: List[int], output_units: int, activation: Op
     return _LayerStack(*layers)
 
 
+class Embedding(nn.Module):
+    """Table of ``num_embeddings`` rows of ``embedding_dim`` numbers for id features (the role of an embedding column with its
+    ``combiner``: the ids of the last axis are averaged, added, or kept apart with ``combiner=None``).
+
+    Ids are int32 or int64, or float32 as the parsers of ``ranking_amd.data`` deliver integer features (exact up to 2^24).
+    Below 0 they are padding: zeros, no gradient.  ``embedding_lookup`` runs it (``ranking_amd.embedding``)."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, combiner: Optional[str] = 'mean', scale: float = 1.0,
+                 dtype: torch.dtype = torch.float32):
+        super().__init__()
+        if int(num_embeddings) < 1 or int(embedding_dim) < 1:
+            raise ValueError('num_embeddings and embedding_dim must be positive, got %s and %s' % (num_embeddings, embedding_dim))
+        if combiner not in (None, 'sum', 'mean'):
+            raise ValueError("combiner must be None, 'sum' or 'mean', got %r" % (combiner,))
+        self.num_embeddings, self.embedding_dim = int(num_embeddings), int(embedding_dim)
+        self.combiner, self.scale = combiner, float(scale)
+        self.weight = nn.Parameter(torch.empty(self.num_embeddings, self.embedding_dim, dtype=dtype))
+        nn.init.normal_(self.weight, std=1.0 / math.sqrt(self.embedding_dim))
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        from ..embedding import embedding_lookup
+        if ids.dtype == torch.float32:
+            if self.num_embeddings > 1 << 24:
+                raise ValueError('float32 ids are exact up to 2^24; the table has %d rows' % self.num_embeddings)
+            ids = ids.to(torch.int64)
+        return embedding_lookup(self.weight, ids, self.scale, self.combiner)
+
+    def get_config(self):
+        return {'num_embeddings': self.num_embeddings, 'embedding_dim': self.embedding_dim, 'combiner': self.combiner,
+                'scale': self.scale}
+
+
 class FlattenList(nn.Module):
     """keras/layers.py:81-182."""
 

@@ -19,6 +19,7 @@ import torch
 
 from .. import _ops
 from .. import losses_impl
+from .. import preference as _preference
 from .. import utils as _tfr_utils
 from . import utils
 
@@ -58,6 +59,7 @@ class RankingLossKey(object):
     APPROX_MRR_LOSS = 'approx_mrr_loss'
     GUMBEL_APPROX_NDCG_LOSS = 'gumbel_approx_ndcg_loss'
     COUPLED_RANKDISTIL_LOSS = 'coupled_rankdistil_loss'
+    PREFERENCE_LOSS = 'preference_loss'            # not in the reference: PreferenceLoss below
 
     @classmethod
     def all_keys(cls) -> List[str]:
@@ -78,6 +80,7 @@ def get(loss: str, reduction: str = Reduction.AUTO, lambda_weight=None, name: Op
         RankingLossKey.APPROX_NDCG_LOSS: ApproxNDCGLoss,
         RankingLossKey.APPROX_MRR_LOSS: ApproxMRRLoss,
         RankingLossKey.GUMBEL_APPROX_NDCG_LOSS: GumbelApproxNDCGLoss,
+        RankingLossKey.PREFERENCE_LOSS: PreferenceLoss,
     }
     key_to_cls_with_lambda = {
         RankingLossKey.PAIRWISE_HINGE_LOSS: PairwiseHingeLoss,
@@ -769,3 +772,95 @@ class MeanSquaredLoss(_PointwiseLoss):
     def __init__(self, reduction=Reduction.AUTO, name=None, ragged=False):
         super().__init__(reduction, name, ragged)
         self._loss = losses_impl.MeanSquaredLoss(name='{}_impl'.format(name) if name else None, ragged=ragged)
+
+
+# ---------------------------------------------------------------- preferences
+@utils.register_keras_serializable()
+class PreferenceLoss(_RankingLoss):
+    """Preference loss on paired log ratios (not in the reference): answers of a list that are graded higher should gain
+    more log probability over the reference model than answers graded lower.
+
+    ``y_true`` ``[B, L]``: grades of at most 64 answers a list; below 0 the answer is not there.  ``y_pred``: token log
+    probabilities ``[B, L, T]`` of the trained model (``preference.token_log_probs``), or one number an answer
+    ``[B, L]``.  ``reference``: the same of the reference model (None: 0).  ``mask`` ``[B, L, T]``: the answers' tokens; what
+    stands elsewhere is never used and gets no gradient.  ``sample_weight``: a number, or one a list (``[B]``, ``[B, 1]``).
+
+        s_i = beta sum_t (y_pred - reference)_it      (divided by the answer's number of tokens if length_normalized)
+        a list's loss = mean over its pairs y_i > y_j >= 0 of l(s_i - s_j), 0 without a pair
+        kind 'logistic': l(h) = (1 - label_smoothing) softplus(-h) + label_smoothing softplus(h)
+             'hinge'   : max(0, 1 - h)         'squared': (h - 1/2)^2
+
+    The scalar is the weighted sum over the lists divided by their number (``AUTO``, ``SUM_OVER_BATCH_SIZE``), or the sum."""
+
+    def __init__(self, reduction=Reduction.AUTO, name=None, beta=0.1, kind='logistic', label_smoothing=0.0,
+                 length_normalized=False):
+        super().__init__(reduction, name)
+        if not 0.0 < float(beta) < 1e30:
+            raise ValueError('beta must be positive, got {}'.format(beta))
+        if kind not in _preference.KINDS:
+            raise ValueError('Invalid kind: {}. Expected "{}"'.format(kind, tuple(_preference.KINDS)))
+        if not 0.0 <= float(label_smoothing) < 0.5 or (label_smoothing and kind != 'logistic'):
+            raise ValueError('label_smoothing must be in [0, 0.5) and needs kind "logistic", got {}'.format(label_smoothing))
+        self._beta, self._kind = float(beta), kind
+        self._label_smoothing, self._length_normalized = float(label_smoothing), bool(length_normalized)
+
+    def get_config(self) -> Dict[str, Any]:
+        return {'reduction': self.reduction, 'name': self.name, 'beta': self._beta, 'kind': self._kind,
+                'label_smoothing': self._label_smoothing, 'length_normalized': self._length_normalized}
+
+    def _args(self, y_true, y_pred, sample_weight, reference, mask):
+        """(y_pred [B, L, T] fp32, arguments of preference.preference_loss)."""
+        _ops.require_device(y_pred, 'y_pred')
+        if y_pred.dim() not in (2, 3):
+            raise ValueError('y_pred must be [batch, answers] or [batch, answers, tokens], got shape %s' % (tuple(y_pred.shape),))
+        shape = tuple(y_pred.shape)
+        flat = len(shape) == 2
+        y_pred = y_pred.to(torch.float32).contiguous()
+        y_true = torch.as_tensor(y_true, dtype=torch.float32, device=y_pred.device).detach().contiguous()
+        if tuple(y_true.shape) != shape[:2]:
+            raise ValueError('y_true of shape %s does not fit y_pred of shape %s' % (tuple(y_true.shape), shape))
+        if not 1 <= shape[1] <= _preference.MAX_ANSWERS:
+            raise ValueError('between 1 and %d answers a list, got %d' % (_preference.MAX_ANSWERS, shape[1]))
+        for name, t in (('reference', reference), ('mask', mask)):
+            if t is not None and (tuple(_ops.require_device(t, name).shape) != shape or t.device != y_pred.device):
+                raise ValueError('%s of shape %s on %s does not fit y_pred of shape %s on %s'
+                                 % (name, tuple(t.shape), t.device, shape, y_pred.device))
+        if reference is not None:
+            reference = _ops._f32(reference.detach(), 'reference')
+        if mask is not None:
+            mask = _ops._u8(mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0, 'mask')
+        scale = 1.0 if self.reduction in (Reduction.SUM, Reduction.NONE) else 1.0 / max(1, shape[0])
+        if sample_weight is not None:
+            if not torch.is_tensor(sample_weight) and not hasattr(sample_weight, '__len__'):
+                scale, sample_weight = scale * float(sample_weight), None
+            else:
+                sample_weight = torch.as_tensor(sample_weight, dtype=torch.float32, device=y_pred.device).detach()
+                if sample_weight.dim() == 0:
+                    sample_weight = sample_weight.expand(shape[0])
+                if tuple(sample_weight.shape) not in ((shape[0],), (shape[0], 1)):
+                    raise ValueError('sample_weight of shape %s: one weight a list is wanted (%d)' % (tuple(sample_weight.shape), shape[0]))
+                sample_weight = sample_weight.reshape(-1).contiguous()
+        how = dict(kind=self._kind, beta=self._beta, label_smoothing=self._label_smoothing,
+                   length_normalized=self._length_normalized, scale=scale)
+        return (y_pred.unsqueeze(2) if flat else y_pred), y_true, reference, mask, sample_weight, how
+
+    def __call__(self, y_true, y_pred, sample_weight=None, reference=None, mask=None):
+        y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred, sample_weight, reference, mask)
+        losses = _preference._PreferenceFn.apply(y_pred, y_true, reference, mask, weight, how)
+        return losses if self.reduction == Reduction.NONE else losses.sum()
+
+    def call(self, y_true, y_pred):
+        """The unreduced losses, one a list."""
+        y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred, None, None, None)
+        return _preference._PreferenceFn.apply(y_pred, y_true, reference, mask, weight, dict(how, scale=1.0))
+
+    def loss_and_grad(self, y_true, y_pred, sample_weight=None, reference=None, mask=None):
+        """(scalar loss, d loss / d y_pred in y_pred's shape, float32) without an autograd graph."""
+        if self.reduction == Reduction.NONE:
+            raise ValueError('loss_and_grad needs a scalar reduction')
+        shape = tuple(y_pred.shape) if torch.is_tensor(y_pred) else None
+        y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred.detach() if shape is not None else y_pred, sample_weight,
+                                                                  reference, mask)
+        losses, coef = _preference.preference_loss(y_pred, y_true, reference, mask, weight, **how)
+        grad = _preference.preference_grad(coef, mask, y_pred.shape[2])
+        return (_ops.list_dot(losses) if losses.numel() else losses.sum()), grad.reshape(shape)

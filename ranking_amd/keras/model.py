@@ -33,10 +33,12 @@ class UnivariateScorer(nn.Module, metaclass=abc.ABCMeta):
 
 class DNNScorer(UnivariateScorer):
     """keras/model.py:780-817: features concatenated in sorted-name order (:803-813)
-    then ``create_tower`` (keras/layers.py:26-77)."""
+    then ``create_tower`` (keras/layers.py:26-77).  ``embeddings``: modules by feature name (``layers.Embedding``) that
+    turn id features ``[B, T]`` (context) or ``[B, L, T]`` (example) into dense columns first; ``input_dim`` counts those."""
 
-    def __init__(self, input_dim: int, **dnn_kwargs):
+    def __init__(self, input_dim: int, embeddings: Optional[Dict[str, nn.Module]] = None, **dnn_kwargs):
         super().__init__()
+        self._embeddings = nn.ModuleDict(embeddings or {})
         self._dnn_kwargs = dict(dnn_kwargs)
         self._dnn_kwargs.setdefault('output_units', 1)
         self._tower = layers.create_tower(input_dim=input_dim, **self._dnn_kwargs)
@@ -45,6 +47,9 @@ class DNNScorer(UnivariateScorer):
         """keras/model.py:712-777.  With the fused tower and one dense example feature the flatten step's
         circular-padding gather (a full copy of the [B, L, F] tensor) is folded into the tower's input cast."""
         from ..tower import FusedTower
+        if self._embeddings:
+            context_features = self._embed(context_features or {}, 1)
+            example_features = self._embed(example_features, 2)
         _feed = (torch.float32, torch.bfloat16)               # (bf16: features the parser already rounded, data.py)
         if not context_features and len(example_features) > 1 and all(
                 torch.is_tensor(v) and v.dim() >= 2 and v.dtype in _feed for v in example_features.values()) and len(
@@ -68,6 +73,10 @@ class DNNScorer(UnivariateScorer):
                 flat_logits = self._tower(x.reshape(b * l, x.shape[2]), row_index=rows)
                 return self._restore((flat_logits, mask))
         return super().forward(context_features, example_features, mask)
+
+    def _embed(self, features, lead):
+        """The features with the embedded ones as [..., width]: `lead` leading axes (batch, or batch and list) are kept."""
+        return {k: self._embeddings[k](v).flatten(lead) if k in self._embeddings else v for k, v in features.items()}
 
     def _score_flattened(self, context_features, example_features):
         ctx = [context_features[k].reshape(context_features[k].shape[0], -1)

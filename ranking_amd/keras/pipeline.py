@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import abc
 import dataclasses
+import functools
 import os
 from typing import Any, Callable, Dict, Iterator, List, Optional, Tuple, Union
 
@@ -25,6 +26,8 @@ import torch
 
 from .. import data as data_lib
 from .. import distributed as dist_lib
+from .. import optim as optim_lib
+from . import layers as layers_lib
 from . import losses as losses_lib
 from . import metrics as metrics_lib
 from . import model as model_lib
@@ -159,19 +162,31 @@ class SimpleDatasetBuilder(AbstractDatasetBuilder):
 class SimpleModelBuilder:
     """The role of ``model.ModelBuilder`` (keras/model.py:316-399) for numeric features: example (and
     context) features are concatenated in sorted-name order (keras/model.py:803-813) and scored by a
-    ``DNNScorer``; ``build()`` returns ``fn(features) -> logits [B, L]``."""
+    ``DNNScorer``; ``build()`` returns ``fn(features) -> logits [B, L]``.  ``embeddings``: for id features, the arguments of
+    ``layers.Embedding`` by feature name."""
 
-    def __init__(self, context_feature_spec, example_feature_spec, mask_feature_name, **dnn_kwargs):
+    def __init__(self, context_feature_spec, example_feature_spec, mask_feature_name, embeddings=None, **dnn_kwargs):
         self._context_names = sorted(context_feature_spec or {})
         self._example_names = sorted(example_feature_spec)
         self._mask_feature_name = mask_feature_name
-        width = sum(data_lib._spec_width(example_feature_spec[n]) for n in self._example_names)
-        width += sum(data_lib._spec_width(context_feature_spec[n]) for n in self._context_names)
+        self._embeddings = dict(embeddings or {})
+        unknown = set(self._embeddings) - set(self._example_names) - set(self._context_names)
+        if unknown:
+            raise ValueError('embeddings for features that no spec has: {}'.format(sorted(unknown)))
+
+        def columns(name, spec):
+            width, how = data_lib._spec_width(spec), self._embeddings.get(name)
+            if how is None:
+                return width
+            return how['embedding_dim'] * (width if how.get('combiner', 'mean') is None else 1)
+        width = sum(columns(n, example_feature_spec[n]) for n in self._example_names)
+        width += sum(columns(n, context_feature_spec[n]) for n in self._context_names)
         self._input_dim = width
         self._dnn_kwargs = dnn_kwargs
 
     def build(self) -> torch.nn.Module:
-        scorer = model_lib.DNNScorer(input_dim=self._input_dim, **self._dnn_kwargs)
+        embeddings = {n: layers_lib.Embedding(**how) for n, how in self._embeddings.items()}
+        scorer = model_lib.DNNScorer(input_dim=self._input_dim, embeddings=embeddings, **self._dnn_kwargs)
         builder = self
 
         class _Model(torch.nn.Module):
@@ -187,7 +202,8 @@ class SimpleModelBuilder:
 
 
 _OPTIMIZERS = {'adam': torch.optim.Adam, 'adagrad': torch.optim.Adagrad, 'sgd': torch.optim.SGD,
-               'rmsprop': torch.optim.RMSprop}
+               'rmsprop': torch.optim.RMSprop, 'adamw': optim_lib.AdamW,
+               'adamw_8bit': functools.partial(optim_lib.AdamW, state_bits=8)}
 
 
 class AbstractPipeline(metaclass=abc.ABCMeta):

@@ -1,0 +1,286 @@
+"""AdamW over many tensors at once, with the moments in 32 or in 8 bits (``csrc/adamw.hip``).
+
+``AdamW`` is the optimizer object (``keras.pipeline``'s ``'adamw'`` and ``'adamw_8bit'``), ``adamw_step`` the same update as
+a plain call on lists of tensors.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from . import _ops
+from ._ops import _ptr, _stream, require_device
+
+QBLOCK = 128                          # TFR_ADAMW_QBLOCK: elements that share a scale
+_MAX_TENSORS, _MAX_TENSORS_8 = 88, 64  # TFR_ADAMW_MAX_TENSORS, TFR_ADAMW8_MAX_TENSORS: tensors of one launch
+_MAX_LAUNCH = 1 << 35                 # elements of one launch
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # TFR_DTYPE_*
+
+
+def quantized_size(numel: int) -> Tuple[int, int]:
+    """(codes, scales) of an 8-bit moment of ``numel`` elements: whole blocks."""
+    blocks = -(-int(numel) // QBLOCK)
+    return blocks * QBLOCK, blocks
+
+
+def _check_hyper(lr, betas, eps, weight_decay):
+    if not torch.is_tensor(lr) and not lr >= 0.0:
+        raise ValueError('Invalid learning rate: {}'.format(lr))
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError('Invalid betas: {}'.format(betas))
+    if not eps >= 0.0:
+        raise ValueError('Invalid epsilon value: {}'.format(eps))
+    if not weight_decay >= 0.0:
+        raise ValueError('Invalid weight_decay value: {}'.format(weight_decay))
+
+
+def _check_dense(t, like, numel, dtype, name):
+    if t.dtype != dtype or t.numel() != numel or not t.is_contiguous() or t.device != like.device:
+        raise ValueError('%s must be a dense %s tensor of %d elements on %s, got %s of shape %s on %s'
+                         % (name, dtype, numel, like.device, t.dtype, tuple(t.shape), t.device))
+
+
+def _array(values):
+    return (ctypes.c_void_p * len(values))(*values)
+
+
+def _launch(items, bits, code, hyper, step, now):
+    """One launch: items = [(param, grad, exp_avg, exp_avg_sq)], their checks done."""
+    lr, (b1, b2), eps, decay = hyper
+    p, g, m, v = zip(*items)
+    addr = lambda ts: _array([t.data_ptr() for t in ts])                    # noqa: E731
+    sizes = (ctypes.c_int64 * len(p))(*[t.numel() for t in p])
+    lib = _lib.load()
+    tail = (sizes, float(lr), float(b1), float(b2), float(eps), float(decay), int(step), _ptr(now), _stream())
+    if bits == 32:
+        _lib.check(lib.tfr_adamw(code, len(p), addr(p), addr(g), addr(m), addr(v), *tail), 'tfr_adamw')
+    else:
+        _lib.check(lib.tfr_adamw8(code, len(p), addr(p), addr(g), addr([x[0] for x in m]), addr([x[1] for x in m]), addr([x[0] for x in v]),
+                                  addr([x[1] for x in v]), *tail), 'tfr_adamw8')
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence, exp_avg_sqs: Sequence, *, step: int,
+               lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+               now: Optional[torch.Tensor] = None) -> None:
+    """One AdamW step, in place, on all tensors: ``TFR_ADAMW_MAX_TENSORS`` tensors a launch.
+
+    ``params`` / ``grads``: dense tensors of one type (float32, bfloat16, float16) a pair.  ``exp_avgs`` / ``exp_avg_sqs``:
+    float32 tensors of the parameter's size, or all of them pairs ``(codes, scales)``: int8 / uint8 codes and float32 scales
+    of ``quantized_size(param.numel())`` elements.  ``step`` counts from 1.  ``now``: float32 ``[3]`` on the device, written
+    by ``AdamW`` when the step is counted there (``step`` and ``lr`` are then not used)."""
+    n = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n):
+        raise ValueError('lists of %d params, %d grads, %d exp_avgs and %d exp_avg_sqs' % (n, len(grads), len(exp_avgs), len(exp_avg_sqs)))
+    _check_hyper(lr, betas, eps, weight_decay)
+    if torch.is_tensor(lr) and now is None:
+        raise ValueError('lr must be a number: a learning rate on the device needs a step that is counted there')
+    if now is None and step < 1:
+        raise ValueError('step counts from 1, got %r' % (step,))
+    if n == 0:
+        return
+    if len({p.data_ptr() for p in params if p.numel()}) != sum(1 for p in params if p.numel()):
+        raise ValueError('the same parameter twice')
+    eight = isinstance(exp_avgs[0], (tuple, list))
+    launches = {}
+    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+        require_device(p, 'params')
+        if p.dtype not in _DTYPES:
+            raise ValueError('params must be float32, bfloat16 or float16, got %s' % p.dtype)
+        numel = p.numel()
+        if not p.is_contiguous():
+            raise ValueError('params must be dense, got strides %s' % (p.stride(),))
+        _check_dense(g, p, numel, p.dtype, 'grads')
+        if isinstance(m, (tuple, list)) != eight or isinstance(v, (tuple, list)) != eight:
+            raise ValueError('moments of 8 and of 32 bits in one call')
+        if eight:
+            codes, blocks = quantized_size(numel)
+            _check_dense(m[0], p, codes, torch.int8, 'exp_avgs codes')
+            _check_dense(m[1], p, blocks, torch.float32, 'exp_avgs scales')
+            _check_dense(v[0], p, codes, torch.uint8, 'exp_avg_sqs codes')
+            _check_dense(v[1], p, blocks, torch.float32, 'exp_avg_sqs scales')
+            if (m[0].data_ptr() | v[0].data_ptr()) & 7:
+                raise ValueError('codes must be 8-byte aligned')
+        else:
+            _check_dense(m, p, numel, torch.float32, 'exp_avgs')
+            _check_dense(v, p, numel, torch.float32, 'exp_avg_sqs')
+        if numel >= _MAX_LAUNCH:
+            raise ValueError('params of at most %d elements, got %d' % (_MAX_LAUNCH - 1, numel))
+        if numel:
+            launches.setdefault((p.device, p.dtype), []).append((p, g, m, v))
+    cap = _MAX_TENSORS_8 if eight else _MAX_TENSORS
+    hyper = (0.0 if torch.is_tensor(lr) else lr, betas, eps, weight_decay)
+    for (device, dtype), items in launches.items():
+        with torch.cuda.device(device):
+            part, size = [], 0
+            for it in items:
+                if len(part) == cap or size + it[0].numel() >= _MAX_LAUNCH:
+                    _launch(part, 8 if eight else 32, _DTYPES[dtype], hyper, step, now)
+                    part, size = [], 0
+                part.append(it)
+                size += it[0].numel()
+            _launch(part, 8 if eight else 32, _DTYPES[dtype], hyper, step, now)
+
+
+def _dequantize(codes, scales, dtype, square):
+    require_device(codes, 'codes')
+    if codes.dtype != dtype or codes.numel() % QBLOCK or not codes.is_contiguous():
+        raise ValueError('codes must be dense %s in whole blocks of %d, got %s of shape %s' % (dtype, QBLOCK, codes.dtype, tuple(codes.shape)))
+    _check_dense(scales, codes, codes.numel() // QBLOCK, torch.float32, 'scales')
+    if codes.data_ptr() & 7:
+        raise ValueError('codes must be 8-byte aligned')
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    _lib.check(_lib.load().tfr_adamw_dequantize(_ptr(codes), _ptr(scales), codes.numel(), int(square), _ptr(out), _stream()),
+               'tfr_adamw_dequantize')
+    return out
+
+
+@_ops.device_guarded
+def dequantize_exp_avg(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The float32 first moments that int8 codes stand for: code * scale (-128: NaN)."""
+    return _dequantize(codes, scales, torch.int8, False)
+
+
+@_ops.device_guarded
+def dequantize_exp_avg_sq(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The float32 second moments that uint8 codes stand for: (code * scale)^2."""
+    return _dequantize(codes, scales, torch.uint8, True)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) over dense float32, bfloat16 or float16 parameters, one launch per
+    ``TFR_ADAMW_MAX_TENSORS`` tensors.
+
+    ``state_bits=8`` holds the moments in 8 bits (2.06 bytes an element for both instead of 8).  ``capturable=True`` counts the
+    step on the device (one small launch more), so that a step recorded in a hipGraph keeps counting when it is replayed;
+    ``lr`` may then be a float32 device tensor of one element.  The state is made by the first eager step (or by
+    ``init_state()``); a capture needs it to be there."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
+        _check_hyper(lr, betas, eps, weight_decay)
+        if state_bits not in (8, 32):
+            raise ValueError('state_bits must be 8 or 32, got {}'.format(state_bits))
+        if torch.is_tensor(lr) and not capturable:
+            raise ValueError('lr as a tensor needs capturable=True')
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      capturable=capturable))
+
+    def _state_of(self, p, group):
+        s = self.state[p]
+        if 'exp_avg' in s:
+            return s
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('AdamW: the state must be there before a stream capture (run a step or init_state() first)')
+        require_device(p, 'params')
+        if group['state_bits'] == 32:
+            s['exp_avg'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            s['exp_avg_sq'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        else:
+            codes, blocks = quantized_size(p.numel())
+            s['exp_avg'] = torch.zeros(codes, dtype=torch.int8, device=p.device)
+            s['exp_avg_sq'] = torch.zeros(codes, dtype=torch.uint8, device=p.device)
+            s['exp_avg_scale'] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+            s['exp_avg_sq_scale'] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        if not group['capturable']:
+            s['step'] = 0
+        return s
+
+    def _counter(self, group, device):
+        """(step count, coefficients) on the device, of a capturable group."""
+        if group.get('step_count') is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('AdamW: the state must be there before a stream capture (run a step or init_state() first)')
+            group['step_count'] = torch.zeros(1, dtype=torch.int64, device=device)
+            group['coefficients'] = torch.zeros(3, dtype=torch.float32, device=device)
+        return group['step_count'], group['coefficients']
+
+    def init_state(self) -> None:
+        """Makes the state of every parameter (before a stream capture without an eager step)."""
+        for group in self.param_groups:
+            for p in group['params']:
+                self._state_of(p, group)
+            if group['capturable'] and group['params']:
+                self._counter(group, group['params'][0].device)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            eight = group['state_bits'] == 8
+            runs = {}                                          # by step count: parameters that were frozen for a while have their own
+            for p in group['params']:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError('AdamW does not take sparse gradients')
+                s = self._state_of(p, group)
+                if group['capturable']:
+                    t = 1
+                else:
+                    t = s['step'] = s['step'] + 1
+                m, v = s['exp_avg'], s['exp_avg_sq']
+                runs.setdefault(t, []).append((p, p.grad.contiguous(), (m, s['exp_avg_scale']) if eight else m,
+                                               (v, s['exp_avg_sq_scale']) if eight else v))
+            if not runs:
+                continue
+            lr, now = group['lr'], None
+            if group['capturable']:
+                now = self._advance(group, next(iter(runs.values()))[0][0].device)
+            elif torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('AdamW: a step inside a stream capture needs capturable=True (the step count would be frozen)')
+            for t, items in runs.items():
+                p, g, m, v = zip(*items)
+                adamw_step(p, g, m, v, step=t, lr=lr, betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'], now=now)
+        return loss
+
+    def _advance(self, group, device):
+        count, now = self._counter(group, device)
+        if any(p.device != count.device for p in group['params']):
+            raise ValueError('AdamW: a capturable group lives on one device')
+        lr, lr_device = group['lr'], None
+        if torch.is_tensor(lr):
+            if not (lr.is_cuda and lr.dtype == torch.float32 and lr.numel() == 1 and lr.device == count.device):
+                raise ValueError('lr must be a float32 tensor of one element on %s' % (count.device,))
+            lr, lr_device = 0.0, lr
+        with torch.cuda.device(count.device):
+            rc = _lib.load().tfr_adamw_advance(_ptr(count), _ptr(lr_device), float(lr), group['betas'][0], group['betas'][1],
+                                               group['weight_decay'], _ptr(now), _stream())
+        _lib.check(rc, 'tfr_adamw_advance')
+        return now
+
+    def load_state_dict(self, state_dict) -> None:
+        """Loads what ``state_dict`` gave.  Moments keep their own types (the base class would cast them to the
+        parameter's), and tensors that are there already are filled in place: a captured step goes on with them."""
+        mine = {p: dict(s) for p, s in self.state.items()}
+        counters = [(g.get('step_count'), g.get('coefficients')) for g in self.param_groups]
+        saved = [(g.get('step_count'), g['params']) for g in state_dict['param_groups']]
+        super().load_state_dict(state_dict)
+        for group, (count, ids), (old, coef) in zip(self.param_groups, saved, counters):
+            for p, i in zip(group['params'], ids):
+                given = state_dict['state'].get(i)
+                if given is None:
+                    continue
+                codes, blocks = quantized_size(p.numel())
+                sizes = {'exp_avg': codes, 'exp_avg_sq': codes, 'exp_avg_scale': blocks, 'exp_avg_sq_scale': blocks}
+                s = self.state[p] = {}
+                for key, value in given.items():
+                    if not torch.is_tensor(value):
+                        s[key] = value
+                        continue
+                    want = sizes.get(key) if group['state_bits'] == 8 else p.numel()
+                    if value.numel() != want:
+                        raise ValueError('state %s of %d elements does not fit a parameter of %d' % (key, value.numel(), p.numel()))
+                    have = mine.get(p, {}).get(key)
+                    if have is not None and have.dtype == value.dtype and have.shape == value.shape:
+                        s[key] = have.copy_(value)
+                    else:
+                        s[key] = value.to(p.device, copy=True)
+            if count is not None and group['params']:
+                device = group['params'][0].device
+                group['step_count'] = count.to(device, copy=True) if old is None else old.copy_(count)
+                group['coefficients'] = torch.zeros(3, dtype=torch.float32, device=device) if coef is None else coef

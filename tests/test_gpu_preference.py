@@ -1,0 +1,177 @@
+"""Preference loss and gradient (csrc/preference.hip, keras.losses.PreferenceLoss) on the GPU against the plain 64-bit form.
+
+The kernels sum in fp64 and round once to fp32 (the gradient: the coefficient once, times the upstream once more), so a loss or
+a gradient is off by 2 U of itself; fp64 roundings, e^x to 1e-15 of them, are counted by 1e-12 of the sums of absolute values."""
+import pytest
+import torch
+
+from tests import training_ops as T
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+def K():
+    from ranking_amd.keras import losses
+    return losses
+
+
+def make(B, L, tokens, seed=0, graded=True):
+    g = torch.Generator().manual_seed(seed + L + tokens)
+    lp = -torch.rand(B, L, tokens, generator=g) * 3
+    ref = lp + torch.randn(B, L, tokens, generator=g) * 0.2
+    mask = torch.rand(B, L, tokens, generator=g) < 0.7
+    y = torch.randint(-1, 4, (B, L), generator=g).float() if graded else torch.tensor([1.0, 0.0]).expand(B, 2).contiguous()
+    return y, lp, ref, mask, torch.rand(B, generator=g) + 0.1
+
+
+def check(y, lp, ref, mask, w, kind='logistic', beta=0.3, smoothing=0.0, normalize=False, reduction='auto'):
+    loss = K().PreferenceLoss(reduction=reduction, beta=beta, kind=kind, label_smoothing=smoothing, length_normalized=normalize)
+    on = lambda t: None if t is None else t.to(DEV)                        # noqa: E731
+    total, grad = loss.loss_and_grad(on(y), on(lp), on(w), reference=on(ref), mask=on(mask))
+    B = lp.shape[0]
+    # beta and the smoothing are handed over as fp32
+    f32 = lambda v: torch.tensor(v, dtype=torch.float32).item()            # noqa: E731
+    scale = f32(1.0 / max(1, B)) if reduction != 'sum' else 1.0
+    want, want_grad, size = T.preference(y, lp, ref, mask, w, kind, f32(beta), f32(smoothing), normalize, scale)
+    slack = 1e-12 * (1 + size.sum()) ** 2
+    T.assert_within(grad, want_grad, 2 * T.U * want_grad.abs() + 1e-12 * (1 + size.amax()) + 2.0 ** -149, 'gradient')
+    # the lists' losses are rounded once and added in fp32
+    T.assert_within(total, want.sum(), (B + 2) * T.U * want.abs().sum() + slack, 'loss')
+    p = on(lp).requires_grad_()
+    out = loss(on(y), p, on(w), reference=on(ref), mask=on(mask))
+    T.assert_within(out, want.sum(), (B + 2) * T.U * want.abs().sum() + slack, 'loss of the autograd path')
+    (out * 2.0).backward()
+    assert torch.equal(p.grad, grad * 2.0)
+    return total, grad
+
+
+@pytest.mark.parametrize('kind,smoothing', [('logistic', 0.0), ('logistic', 0.1), ('hinge', 0.0), ('squared', 0.0)])
+@pytest.mark.parametrize('normalize', [False, True])
+@pytest.mark.parametrize('B,L,tokens', [(1, 2, 1), (5, 3, 17), (3, 5, 300), (2, 64, 9)])
+def test_kinds(kind, smoothing, normalize, B, L, tokens):
+    check(*make(B, L, tokens), kind=kind, smoothing=smoothing, normalize=normalize)
+
+
+@pytest.mark.parametrize('B,L,tokens', [(1, 1, 5), (7, 2, 255), (2, 2, 8191), (2, 3, 8193), (1, 2, 40001), (300, 2, 64), (3, 2, 0)])
+def test_sizes(B, L, tokens):
+    check(*make(B, L, tokens))
+
+
+def test_optional_arguments():
+    y, lp, ref, mask, w = make(4, 3, 50)
+    check(y, lp, None, None, None)
+    check(y, lp, ref, None, None)
+    check(y, lp, None, mask, w, reduction='sum')
+    loss = K().PreferenceLoss()
+    a = loss.loss_and_grad(y.to(DEV), lp.to(DEV), w.unsqueeze(1).to(DEV), mask=mask.float().to(DEV))
+    b = loss.loss_and_grad(y.to(DEV), lp.to(DEV), w.to(DEV), mask=mask.to(torch.uint8).to(DEV))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    a, b = loss.loss_and_grad(y.to(DEV), lp.to(DEV), 2.0), loss.loss_and_grad(y.to(DEV), lp.to(DEV), torch.tensor(2.0, device=DEV))
+    assert torch.allclose(a[0], b[0], rtol=4 * T.U) and torch.allclose(a[1], b[1], rtol=4 * T.U)
+
+
+def test_scores_of_whole_answers():
+    """[B, L] log probabilities of whole answers = answers of one token; unreduced losses."""
+    y, lp, ref, _, w = make(6, 4, 1)
+    loss = K().PreferenceLoss(reduction='none')
+    got = loss(y.to(DEV), lp[:, :, 0].to(DEV), w.to(DEV), reference=ref[:, :, 0].to(DEV))
+    f32 = torch.tensor(0.1, dtype=torch.float32).item()
+    want, _, _ = T.preference(y, lp, ref, None, w, 'logistic', f32, 0.0, False)
+    T.assert_within(got, want, 2 * T.U * want.abs() + 1e-12)
+    T.assert_within(loss.call(y.to(DEV), lp[:, :, 0].to(DEV)), T.preference(y, lp, None, None, None, 'logistic', f32, 0.0, False)[0],
+                    1e-6 * want.abs().max())
+    total, grad = K().PreferenceLoss().loss_and_grad(y.to(DEV), lp[:, :, 0].to(DEV))
+    assert grad.shape == (6, 4)
+
+
+def test_masked_places_are_never_used():
+    y, lp, ref, mask, w = make(5, 4, 100)
+    y[0] = torch.tensor([2.0, -1.0, 0.0, 1.0])
+    clean = check(y, lp, ref, mask, w, normalize=True)
+    off = ~mask
+    off[0, 1] = True                                                       # an answer that is not there
+    for bad in (float('nan'), float('inf'), -float('inf')):
+        lp2, ref2 = lp.masked_fill(off, bad), ref.masked_fill(off, bad)
+        got = K().PreferenceLoss(beta=0.3, length_normalized=True).loss_and_grad(y.to(DEV), lp2.to(DEV), w.to(DEV), reference=ref2.to(DEV), mask=mask.to(DEV))
+        assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
+    assert not got[1][off.to(DEV)].any()
+
+
+def test_lists_without_pairs_and_empty_answers():
+    y, lp, ref, mask, w = make(4, 3, 20)
+    y[0], y[1], y[2] = 1.0, -1.0, torch.tensor([-1.0, 3.0, -1.0])          # ties, nothing there, one answer
+    y[3] = torch.tensor([2.0, 1.0, 0.0])
+    mask[3, 1] = False                                                     # an answer of no tokens
+    _, grad = check(y, lp, ref, mask, w, normalize=True)
+    assert not grad[:3].any() and not grad[3, 1].any() and grad[3, 0].any()
+    total, grad = check(y[:3], lp[:3], ref[:3], mask[:3], w[:3])
+    assert total == 0 and not grad.any()
+    nan = torch.full_like(y, float('nan'))
+    total, grad = K().PreferenceLoss().loss_and_grad(nan.to(DEV), lp.to(DEV))
+    assert total == 0 and not grad.any()
+
+
+def test_large_margins_and_infinities():
+    """Margins far beyond what an exponential takes; an infinite log probability of a token that counts."""
+    y = torch.tensor([[1.0, 0.0], [1.0, 0.0]])
+    lp = torch.tensor([[[-1.0], [-5e4]], [[-5e4], [-1.0]]])
+    total, grad = check(y, lp, None, None, None, beta=1.0)
+    assert torch.isfinite(grad).all() and grad[0].abs().max() < 1e-30 and grad[1, 0, 0] == -0.5
+    lp[1, 0, 0] = -float('inf')
+    total, grad = K().PreferenceLoss(beta=1.0).loss_and_grad(y.to(DEV), lp.to(DEV))
+    assert total == float('inf') and grad[1, 0, 0] == -0.5
+
+
+def test_strides_types_and_empty_batch():
+    y, lp, ref, mask, w = make(6, 4, 30)
+    want = K().PreferenceLoss().loss_and_grad(y[::2, :3].contiguous().to(DEV), lp[::2, :3, 5:].contiguous().to(DEV),
+                                              mask=mask[::2, :3, 5:].contiguous().to(DEV))
+    got = K().PreferenceLoss().loss_and_grad(y.to(DEV)[::2, :3], lp.to(DEV)[::2, :3, 5:], mask=mask.to(DEV)[::2, :3, 5:])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    half = lp.to(torch.bfloat16).to(DEV).requires_grad_()
+    K().PreferenceLoss()(y.to(DEV), half).backward()
+    assert half.grad.dtype == torch.bfloat16
+    full = K().PreferenceLoss().loss_and_grad(y.to(DEV), half.detach().float())[1]
+    T.assert_within(half.grad, full.double(), T.half(torch.bfloat16) * full.double().abs() + 1e-40)
+    total, grad = K().PreferenceLoss().loss_and_grad(torch.zeros(0, 3, device=DEV), torch.zeros(0, 3, 7, device=DEV))
+    assert total == 0 and grad.shape == (0, 3, 7)
+
+
+@pytest.mark.parametrize('tokens', [40, 20000])
+def test_other_stream_and_graphs(tokens):
+    y, lp, ref, mask, w = (t.to(DEV) for t in make(3, 2, tokens, graded=False))
+    loss = K().PreferenceLoss(label_smoothing=0.1)
+    step = lambda: loss.loss_and_grad(y, lp, w, reference=ref, mask=mask)   # noqa: E731
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graphs = []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for _ in range(3):
+        lp.uniform_(-4, 0)
+        for g, _ in graphs:
+            g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_refusals():
+    y, lp, ref, mask, w = (t.to(DEV) for t in make(4, 3, 5))
+    loss = K().PreferenceLoss()
+    for bad in (lambda: loss(y[:3], lp), lambda: loss(y, lp[0, 0]), lambda: loss(y, lp, reference=ref[:, :, :4]), lambda: loss(y, lp, mask=mask[:2]),
+                lambda: loss(y, lp, w[:3]), lambda: loss(y, lp, y), lambda: loss(y.new_zeros(1, 65), lp.new_zeros(1, 65, 2)),
+                lambda: loss(y.new_zeros(1, 0), lp.new_zeros(1, 0, 2)), lambda: K().PreferenceLoss(reduction='none').loss_and_grad(y, lp)):
+        with pytest.raises(ValueError):
+            bad()
