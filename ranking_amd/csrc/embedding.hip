@@ -6,12 +6,13 @@
 // An id below 0 is padding: a zero row, no gradient.  An id beyond the table gives a row of NaN and no gradient: nothing
 // outside the table is read.
 //
-// The gradient writes every row of dW exactly once and adds in an order that depends on the ids alone: the occurrences are
-// sorted by id (stable radix sort, least significant digit first), a row's occurrences are then a run of the sorted list, and
-// the wave that owns the row finds the run by a search.  No atomics on floating point, no separate zero fill.  Runs of common
-// tokens are cut: every aligned chunk of CHUNK sorted occurrences that holds one single token is summed by a workgroup of its
-// own beforehand, and the row adds those sums and the loose ends (a token that is 6 % of 262 144 costs its row 120 sums
-// instead of 16 000 rows).
+// The gradient writes every row of dW exactly once and adds in an order that depends on the ids alone: no atomics on floating
+// point, no separate zero fill of rows that are written anyway.
+//   1. The occurrences are sorted by id (stable radix sort, least significant digit first, at most 10 bits a pass).
+//   2. A group of lanes walks a chunk of the sorted list (32 .. 128 occurrences) and adds the rows of each run of equal ids: a run
+//      that lies inside its chunk is a finished row of dW; the part of a run that crosses a chunk's border is left as a partial
+//      sum.  The work is cut by occurrences and not by rows, so a token that is 6 % of the batch costs what the others cost.
+//   3. Runs that cross borders are joined from their partial sums, and rows without an occurrence are filled with zeros.
 #include "common.h"
 #include "elem.h"
 
@@ -19,10 +20,9 @@ using namespace tfr;
 
 namespace {
 
-constexpr int CHUNK = 128;              // sorted occurrences per chunk sum
-constexpr int HEAVY = 64;               // occurrences from which the whole workgroup adds a row
+constexpr int LONG_RUN = 16;            // partial sums from which the whole workgroup joins a run
 constexpr int SMALL_SORT = 4096;        // lookups that one workgroup sorts in LDS
-constexpr int ITEMS = 8;                // sorted items per thread and pass of the large sort
+constexpr int ITEMS = 8;                // items a thread of the large sort holds
 
 template <typename Id>
 __device__ __forceinline__ int id_key(const Id* __restrict__ ids, long i, int rows) {
@@ -135,18 +135,6 @@ __global__ __launch_bounds__(256) void embedding_bag_kernel(const T* __restrict_
   }
 }
 
-// Per-bag factor of the mean combiner's gradient: scale / #{t : id >= 0}.
-template <typename Id>
-__global__ __launch_bounds__(256) void embedding_factor_kernel(const Id* __restrict__ ids, long bags, int tokens, float scale,
-                                                               float* __restrict__ factor) {
-  const long bag = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (bag >= bags) return;
-  int count = 0;
-  for (int t = threadIdx.x & 63; t < tokens; t += 64) count += ids[bag * tokens + t] >= 0 ? 1 : 0;
-  count = wave_sum_i(count);
-  if ((threadIdx.x & 63) == 0) factor[bag] = scale / (float)(count > 0 ? count : 1);
-}
-
 // ------------------------------------------------------------------------------------------------ sort
 // Lanes of the wave whose digit equals this lane's (`live` lanes only).
 __device__ __forceinline__ uint64_t same_digit(int digit, int bits, bool live) {
@@ -170,8 +158,8 @@ __device__ __forceinline__ int wave_place(int digit, int bits, bool live, int* c
   return before + __popcll(peers & ((1ull << lane) - 1ull));
 }
 
-// Exclusive prefix sum over `n` (<= 1024) values, one a thread, of a 1024-thread workgroup; `red` holds 16 ints.
-__device__ __forceinline__ int block_exclusive_1024(int v, int* red) {
+// Exclusive prefix sum over one value a thread; `red` holds 16 ints.
+__device__ __forceinline__ int block_exclusive(int v, int* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
 #pragma unroll
@@ -187,10 +175,37 @@ __device__ __forceinline__ int block_exclusive_1024(int v, int* red) {
   return base + x - v;
 }
 
-// One workgroup sorts up to SMALL_SORT (id, position) pairs, 8 bits a pass.
+// What the first launch of a gradient does beside sorting, on workgroups of its own: every row's first occurrence is set to
+// "none", and the mean combiner's factor of every bag, scale / #{t : id >= 0}, is counted.
+struct Prepare {
+  int* first;
+  float* factor;
+  long bags;
+  int rows, tokens;
+  float scale;
+};
+
 template <typename Id>
-__global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __restrict__ ids, int n, int rows, int bits,
+__device__ __forceinline__ void prepare_rows(const Prepare& p, const Id* __restrict__ ids, int block, int blocks) {
+  for (long r = (long)block * blockDim.x + threadIdx.x; r < p.rows; r += (long)blocks * blockDim.x) p.first[r] = -1;
+  if (!p.factor) return;
+  const int waves = blockDim.x >> 6;
+  for (long bag = (long)block * waves + (threadIdx.x >> 6); bag < p.bags; bag += (long)blocks * waves) {
+    int count = 0;
+    for (int t = threadIdx.x & 63; t < p.tokens; t += 64) count += ids[bag * p.tokens + t] >= 0 ? 1 : 0;
+    count = wave_sum_i(count);
+    if ((threadIdx.x & 63) == 0) p.factor[bag] = p.scale / (float)(count > 0 ? count : 1);
+  }
+}
+
+// Workgroup 0 sorts up to SMALL_SORT (id, position) pairs, 8 bits a pass; the others prepare the rows.
+template <typename Id>
+__global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __restrict__ ids, int n, int rows, int bits, const Prepare prep,
                                                                     int* __restrict__ keys_out, int* __restrict__ pos_out) {
+  if (blockIdx.x > 0) {
+    prepare_rows(prep, ids, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
   __shared__ uint64_t s_item[SMALL_SORT];
   __shared__ int s_count[16 * 256];
   __shared__ int s_red[16];
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __
         total += c;
       }
     }
-    const int base = block_exclusive_1024(tid < 256 ? total : 0, s_red);
+    const int base = block_exclusive(tid < 256 ? total : 0, s_red);
     if (tid < 256)
       for (int w = 0; w < 16; ++w) s_count[w * 256 + tid] += base;
     __syncthreads();
@@ -242,241 +257,282 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __
   }
 }
 
-// The large sort, one pass = digit counts of every tile, then the scatter; a tile is 1024 * ITEMS consecutive items.
-// FIRST: the keys are the ids themselves, and the positions their indexes.
+// The large sort.  One pass = the digit counts of every tile (a workgroup's `subs` * blockDim.x * ITEMS consecutive items), then
+// the scatter, in which a tile adds up the counts of the tiles before it by itself.  FIRST: the keys are the ids themselves, the
+// positions their indexes, and the workgroups behind the tiles prepare the rows.
 template <typename Id, bool FIRST>
-__global__ __launch_bounds__(1024) void embedding_digits_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, int n,
-                                                                int rows, int shift, int bits, int* __restrict__ counts) {
+__global__ __launch_bounds__(1024) void embedding_digits_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, int n, int rows, int tiles,
+                                                                int subs, int shift, int bits, const Prepare prep, int* __restrict__ counts) {
+  if (FIRST && (int)blockIdx.x >= tiles) {
+    prepare_rows(prep, ids, blockIdx.x - tiles, gridDim.x - tiles);
+    return;
+  }
   extern __shared__ int s_bins[];
   const int bins = 1 << bits;
-  for (int i = threadIdx.x; i < bins; i += 1024) s_bins[i] = 0;
+  for (int i = threadIdx.x; i < bins; i += blockDim.x) s_bins[i] = 0;
   __syncthreads();
-  const long base = (long)blockIdx.x * (1024 * ITEMS);
+  for (int sub = 0; sub < subs; ++sub) {
+    const long base = ((long)blockIdx.x * subs + sub) * ((long)blockDim.x * ITEMS);
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const long i = base + k * 1024 + threadIdx.x;
-    if (i < n) atomicAdd(&s_bins[((FIRST ? id_key(ids, i, rows) : keys[i]) >> shift) & (bins - 1)], 1);
+    for (int k = 0; k < ITEMS; ++k) {
+      const long i = base + k * blockDim.x + threadIdx.x;
+      if (i < n) atomicAdd(&s_bins[((FIRST ? id_key(ids, i, rows) : keys[i]) >> shift) & (bins - 1)], 1);
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < bins; i += 1024) counts[(long)blockIdx.x * bins + i] = s_bins[i];
+  for (int i = threadIdx.x; i < bins; i += blockDim.x) counts[(long)blockIdx.x * bins + i] = s_bins[i];
 }
 
 template <typename Id, bool FIRST>
-__global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Id* __restrict__ ids, const int* __restrict__ keys,
-                                                                 const int* __restrict__ pos, int n, int rows, int shift,
-                                                                 int bits, const int* __restrict__ counts, int* __restrict__ keys_out,
-                                                                 int* __restrict__ pos_out) {
-  extern __shared__ int s_count[];                              // [16][bins], then the 16 ints of the prefix sum
-  const int bins = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int* red = s_count + 16 * bins;
-  for (int i = tid; i < 16 * bins; i += 1024) s_count[i] = 0;
-  __syncthreads();
-  const long base = (long)blockIdx.x * (1024 * ITEMS) + wave * (64 * ITEMS);
-  int key[ITEMS], place[ITEMS];
+__global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, const int* __restrict__ pos,
+                                                                 int n, int rows, int subs, int shift, int bits, const int* __restrict__ counts,
+                                                                 int* __restrict__ keys_out, int* __restrict__ pos_out) {
+  extern __shared__ int s_count[];                              // [waves][bins], the 16 ints of the prefix sum, the next place of each bin [bins]
+  const int bins = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  int* red = s_count + waves * bins;
+  int* next = red + 16;
+  const int per = bins > (int)blockDim.x ? bins / blockDim.x : 1;        // bins of a thread: 1, 2 or 4, neighbours
+  int before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0};
+  if (tid * per < bins) {
+    const int* c = counts + tid * per;
+    const int tiles = gridDim.x, mine = blockIdx.x;
+    for (int t0 = 0; t0 < tiles; t0 += 8) {
+      int v[8][4];
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const long i = base + k * 64 + lane;
-    key[k] = i < n ? (FIRST ? id_key(ids, i, rows) : keys[i]) : -1;
-  }
+      for (int u = 0; u < 8; ++u)
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) place[k] = wave_place((key[k] >> shift) & (bins - 1), bits, key[k] >= 0, s_count + wave * bins);
-  __syncthreads();
-  int before = 0, total = 0;
-  if (tid < bins) {
-    for (int t = 0; t < (int)gridDim.x; ++t) {
-      const int c = counts[(long)t * bins + tid];
-      before += t < (int)blockIdx.x ? c : 0;
-      total += c;
+        for (int j = 0; j < 4; ++j) v[u][j] = t0 + u < tiles && j < per ? c[(long)(t0 + u) * bins + j] : 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          before[j] += t0 + u < mine ? v[u][j] : 0;
+          total[j] += v[u][j];
+        }
     }
   }
-  before += block_exclusive_1024(total, red);
-  if (tid < bins) {
-    for (int w = 0; w < 16; ++w) {
-      const int c = s_count[w * bins + tid];
-      s_count[w * bins + tid] = before;
-      before += c;
+  int at = block_exclusive(total[0] + total[1] + total[2] + total[3], red);
+  if (tid * per < bins) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j < per) next[tid * per + j] = at + before[j];
+      at += total[j];
     }
   }
-  __syncthreads();
+  for (int sub = 0; sub < subs; ++sub) {
+    for (int i = tid; i < waves * bins; i += blockDim.x) s_count[i] = 0;
+    __syncthreads();
+    const long base = ((long)blockIdx.x * subs + sub) * ((long)blockDim.x * ITEMS) + wave * (64 * ITEMS);
+    int key[ITEMS], place[ITEMS];
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    if (key[k] < 0) continue;
-    const int to = s_count[wave * bins + ((key[k] >> shift) & (bins - 1))] + place[k];
-    keys_out[to] = key[k];
-    pos_out[to] = FIRST ? (int)(base + k * 64 + lane) : pos[base + k * 64 + lane];
+    for (int k = 0; k < ITEMS; ++k) {
+      const long i = base + k * 64 + lane;
+      key[k] = i < n ? (FIRST ? id_key(ids, i, rows) : keys[i]) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) place[k] = wave_place((key[k] >> shift) & (bins - 1), bits, key[k] >= 0, s_count + wave * bins);
+    __syncthreads();
+    for (int b = tid; b < bins; b += blockDim.x) {
+      int p = next[b];
+      for (int w = 0; w < waves; ++w) {
+        const int c = s_count[w * bins + b];
+        s_count[w * bins + b] = p;
+        p += c;
+      }
+      next[b] = p;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      if (key[k] < 0) continue;
+      const int to = s_count[wave * bins + ((key[k] >> shift) & (bins - 1))] + place[k];
+      keys_out[to] = key[k];
+      pos_out[to] = FIRST ? (int)(base + k * 64 + lane) : pos[base + k * 64 + lane];
+    }
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
 struct GradArgs {
-  const int* keys;                      // [n] sorted ids
+  const int* keys;                      // [n] sorted ids; rows: no gradient
   const int* pos;                       // [n] the lookup that each came from
   const float* factor;                  // [bags] or null: scale for all
-  float* chunks;                        // [n / CHUNK][dim] sums of the chunks that hold one token
-  int n, rows, dim, tokens, lanes_log2, wave_rows;
+  int* first;                           // [rows] where a row's run begins, -1: no occurrence
+  int* last;                            // [rows] where it ends (rows with an occurrence)
+  void* out;                            // [rows][dim]
+  float* parts;                         // [2 * chunks][dim]: of chunk q the run that began before it (2 q) and the one that goes on (2 q + 1)
+  int n, rows, dim, tokens, chunk_log2, lanes_log2, wave_rows;
   float scale;
 };
 
-// Adds f_b * g[b] of the sorted occurrences first, first + step, ... < end to acc.
+// Step 2: a group of lanes a chunk, gridDim.y column steps of the group.
 template <typename T, int E>
-__device__ __forceinline__ void add_rows(const GradArgs& a, const T* __restrict__ grad, int first, int end, int step, int c, float (&acc)[E]) {
-  for (int i = first; i < end; i += 4 * step) {
-    int b[4];
-    float v[4][E], f[4];
+__global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, const T* __restrict__ grad) {
+  const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
+  const long q = (long)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const long begin = q << a.chunk_log2;
+  if (begin >= a.n) return;
+  const int lo = (int)begin, hi = a.n - lo < (1 << a.chunk_log2) ? a.n : lo + (1 << a.chunk_log2);
+  const int c = (blockIdx.y << a.lanes_log2) + lane;
+  const bool on = c < a.dim / E, scribe = lane == 0 && blockIdx.y == 0;
+  int row = a.keys[lo], start = lo;
+  bool began_before = lo > 0 && a.keys[lo - 1] == row;
+  float acc[E];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int at = i + k * step;
-      b[k] = at < end ? a.pos[at] : -1;
-      if (a.tokens > 1 && b[k] >= 0) b[k] = (int)((unsigned)b[k] / (unsigned)a.tokens);
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  // Ends the run of `row` at sorted position `end`; `goes_on`: its next occurrence is the next chunk's first.
+  auto finish = [&](int end, bool goes_on) {
+    if (row >= a.rows) return;
+    if (scribe) {
+      if (!began_before) a.first[row] = start;
+      if (!goes_on) a.last[row] = end;
+    }
+    if (!on) return;
+    if (began_before || goes_on) {
+      store_pack<float, E>(a.parts + (2 * q + (began_before ? 0 : 1)) * a.dim + (long)c * E, acc);
+    } else {
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = a.factor ? acc[e] : acc[e] * a.scale;
+      store_pack<T, E>(static_cast<T*>(a.out) + (long)row * a.dim + (long)c * E, v);
+    }
+  };
+  for (int i = lo; i < hi; i += 8) {
+    int key[8], b[8];
+    float v[8][E], f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool in = i + k < hi;
+      key[k] = in ? a.keys[i + k] : a.rows;
+      b[k] = in ? a.pos[i + k] : 0;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (b[k] >= 0) {
+    for (int k = 0; k < 8; ++k) {
+      if (a.tokens > 1) b[k] = (int)((unsigned)b[k] / (unsigned)a.tokens);
+      if (key[k] < a.rows && on) {
         load_pack<T, E>(grad + (long)b[k] * a.dim + (long)c * E, v[k]);
         f[k] = a.factor ? a.factor[b[k]] : 1.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i + k >= hi) break;
+      if (key[k] != row) {
+        finish(i + k, false);
+        row = key[k];
+        start = i + k;
+        began_before = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      }
+      if (key[k] < a.rows && on) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(f[k], v[k][e], acc[e]);
+      }
+    }
+  }
+  finish(hi, hi < a.n && a.keys[hi] == row);
+}
+
+// Adds the partial sums of a run from sorted position s to e: that of its first chunk and those of the chunks behind it, the
+// `offset`th and every `step`th from there.
+template <int E>
+__device__ __forceinline__ void add_parts(const GradArgs& a, int s, int e, int offset, int step, int c, float (&acc)[E]) {
+  const long q0 = s >> a.chunk_log2, q1 = (e - 1) >> a.chunk_log2;
+  for (long q = q0 + offset; q <= q1; q += 4 * step) {
+    float v[4][E];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long p = q + k * step;
+      if (p <= q1) {
+        load_pack<float, E>(a.parts + (2 * p + (p == q0 ? 1 : 0)) * a.dim + (long)c * E, v[k]);
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[k][e] = 0.f;
-        f[k] = 0.f;
+        for (int x = 0; x < E; ++x) v[k][x] = 0.f;
       }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = b[k] >= 0 ? __builtin_fmaf(f[k], v[k][e], acc[e]) : acc[e];
-  }
-}
-
-// Joins the groups' sums through LDS in group order; the result is group 0's.
-template <int E>
-__device__ __forceinline__ void join_groups(float* s_acc, int lanes_log2, float (&acc)[E]) {
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_acc[e * 256 + threadIdx.x] = acc[e];
-  __syncthreads();
-  if ((threadIdx.x >> lanes_log2) == 0) {
-    for (int p = 1; p < (256 >> lanes_log2); ++p)
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += s_acc[e * 256 + threadIdx.x + (p << lanes_log2)];
+      for (int x = 0; x < E; ++x) acc[x] += v[k][x];
   }
 }
 
 template <typename T, int E>
-__global__ __launch_bounds__(256) void embedding_chunk_kernel(const GradArgs a, const T* __restrict__ grad) {
-  __shared__ float s_acc[256 * E];
-  const int first = blockIdx.x * CHUNK;
-  const int key = a.keys[first];
-  if (key >= a.rows || a.keys[first + CHUNK - 1] != key) return;         // the same for the whole workgroup
-  const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1), group = threadIdx.x >> a.lanes_log2;
-  const int packs = a.dim / E;
-  for (int c0 = 0; c0 < packs; c0 += 1 << a.lanes_log2) {
-    const int c = c0 + lane;
-    float acc[E];
+__device__ __forceinline__ void write_row(const GradArgs& a, int row, int c, float (&acc)[E]) {
+  if (!a.factor) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    if (c < packs) add_rows<T, E>(a, grad, first + group, first + CHUNK, 256 >> a.lanes_log2, c, acc);
-    join_groups<E>(s_acc, a.lanes_log2, acc);
-    if (group == 0 && c < packs) store_pack<float, E>(a.chunks + (long)blockIdx.x * a.dim + (long)c * E, acc);
+    for (int e = 0; e < E; ++e) acc[e] *= a.scale;
   }
+  store_pack<T, E>(static_cast<T*>(a.out) + (long)row * a.dim + (long)c * E, acc);
 }
 
-// First index of the sorted keys that is not below `row`: 64 probes a step, the whole wave together.
-__device__ __forceinline__ int wave_lower_bound(const int* __restrict__ keys, int n, int row) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, len = n;                                          // the answer is in [lo, lo + len]
-  while (len > 0) {
-    const int step = (len + 63) / 64;
-    const int at = lo + lane * step + step - 1;                 // the last key of this lane's part
-    const bool below = lane * step < len && keys[at < lo + len ? at : lo + len - 1] < row;
-    const int whole = __popcll(__ballot(below));                // parts that lie below as a whole
-    const int next = lo + whole * step;
-    if (next >= lo + len) return lo + len;
-    const int left = lo + len - next;
-    lo = next;
-    len = step == 1 ? 0 : (left < step ? left : step) - 1;      // the part's last key is not below
-  }
-  return lo;
-}
-
+// Step 3: the first `joins` workgroups join the runs that cross the borders of their chunks (a group of lanes a border; long
+// runs the whole workgroup, through LDS in a fixed order), the others fill the rows that have no occurrence.
 template <typename T, int E>
-__global__ __launch_bounds__(256) void embedding_rows_kernel(const GradArgs a, const T* __restrict__ grad, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void embedding_rows_kernel(const GradArgs a, int joins) {
   __shared__ float s_acc[256 * E];
-  __shared__ int s_bound[4][65];
-  __shared__ int s_heavy[4 * 64], s_heavies;
-  const int wave = threadIdx.x >> 6, wlane = threadIdx.x & 63;
-  const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
+  __shared__ int s_long[256], s_longs;
+  const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.lanes_log2, groups = 256 >> a.lanes_log2;
   const int packs = a.dim / E;
-  const long r0 = ((long)blockIdx.x * 4 + wave) * a.wave_rows;
-  if (threadIdx.x == 0) s_heavies = 0;
-  __syncthreads();
-  if (r0 < a.rows) {
+  if ((int)blockIdx.x >= joins) {
+    const long r0 = ((long)(blockIdx.x - joins) * 4 + (threadIdx.x >> 6)) * a.wave_rows;
+    if (r0 >= a.rows) return;
+    const int wlane = threadIdx.x & 63;
     const int many = (int)(a.rows - r0 < a.wave_rows ? a.rows - r0 : a.wave_rows);
-    const int lo = wave_lower_bound(a.keys, a.n, (int)r0);
-    const int hi = wave_lower_bound(a.keys + lo, a.n - lo, (int)r0 + many) + lo;
-    int b0 = lo, b1 = hi;                                       // first key of row r0 + wlane
-    while (b0 < b1) {
-      const int mid = (b0 + b1) >> 1;
-      if (a.keys[mid] < (int)r0 + wlane) b0 = mid + 1; else b1 = mid;
-    }
-    s_bound[wave][wlane] = wlane < many ? b0 : hi;
-    if (wlane == 0) s_bound[wave][64] = hi;
-  }
-  __syncthreads();
-  if (r0 < a.rows) {
-    const int many = (int)(a.rows - r0 < a.wave_rows ? a.rows - r0 : a.wave_rows);
+    const uint64_t empty = __ballot(wlane < many && (a.first == nullptr || a.first[r0 + wlane] < 0));
+    float zero[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) zero[e] = 0.f;
     for (int r = wlane >> a.lanes_log2; r < many; r += 64 >> a.lanes_log2) {
-      const int s = s_bound[wave][r], e = s_bound[wave][r + 1];
-      if (e - s > HEAVY) {
-        if (lane == 0) s_heavy[atomicAdd(&s_heavies, 1)] = wave * 64 + r;
-        continue;
-      }
-      T* row = out + (r0 + r) * a.dim;
-      for (int c = lane; c < packs; c += lanes) {
-        float acc[E];
+      if (!((empty >> r) & 1)) continue;
+      T* o = static_cast<T*>(a.out) + (r0 + r) * a.dim;
+      for (int c = lane; c < packs; c += lanes) store_pack<T, E>(o + (long)c * E, zero);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) s_longs = 0;
+  __syncthreads();
+  // the run of the last occurrence of chunk q, if it begins there and goes on
+  const long border = (((long)blockIdx.x * groups + group) + 1) << a.chunk_log2;
+  if (border < a.n) {
+    const int row = a.keys[border - 1];
+    if (row < a.rows && a.keys[border] == row) {
+      const int s = a.first[row], e = a.last[row];
+      if ((long)s >= border - (1l << a.chunk_log2)) {
+        if (((e - 1) >> a.chunk_log2) - (s >> a.chunk_log2) >= LONG_RUN) {
+          if (lane == 0) s_long[atomicAdd(&s_longs, 1)] = row;
+        } else {
+          for (int c = lane; c < packs; c += lanes) {
+            float acc[E];
 #pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] = 0.f;
-        add_rows<T, E>(a, grad, s, e, 1, c, acc);
-        if (!a.factor) {
-#pragma unroll
-          for (int k = 0; k < E; ++k) acc[k] *= a.scale;
+            for (int x = 0; x < E; ++x) acc[x] = 0.f;
+            add_parts<E>(a, s, e, 0, 1, c, acc);
+            write_row<T, E>(a, row, c, acc);
+          }
         }
-        store_pack<T, E>(row + (long)c * E, acc);
       }
     }
   }
   __syncthreads();
-  const int group = threadIdx.x >> a.lanes_log2, groups = 256 >> a.lanes_log2;
-  for (int h = 0; h < s_heavies; ++h) {                         // the list's order does not touch a row's own sum
-    const int w = s_heavy[h] >> 6, r = s_heavy[h] & 63;
-    const int s = s_bound[w][r], e = s_bound[w][r + 1];
-    const int whole0 = (s + CHUNK - 1) / CHUNK, whole1 = e / CHUNK;      // the chunks that lie inside
-    T* row = out + (((long)blockIdx.x * 4 + w) * a.wave_rows + r) * a.dim;
+  for (int h = 0; h < s_longs; ++h) {                           // the list's order does not touch a row's own sum
+    const int row = s_long[h], s = a.first[row], e = a.last[row];
     for (int c0 = 0; c0 < packs; c0 += lanes) {
       const int c = c0 + lane;
       float acc[E];
 #pragma unroll
-      for (int k = 0; k < E; ++k) acc[k] = 0.f;
-      if (c < packs) {
-        if (whole1 > whole0) {
-          add_rows<T, E>(a, grad, s + group, whole0 * CHUNK, groups, c, acc);
-          for (int q = whole0 + group; q < whole1; q += groups) {
-            float v[E];
-            load_pack<float, E>(a.chunks + (long)q * a.dim + (long)c * E, v);
+      for (int x = 0; x < E; ++x) acc[x] = 0.f;
+      if (c < packs) add_parts<E>(a, s, e, group, groups, c, acc);
+      __syncthreads();
 #pragma unroll
-            for (int k = 0; k < E; ++k) acc[k] += v[k];
-          }
-          add_rows<T, E>(a, grad, whole1 * CHUNK + group, e, groups, c, acc);
-        } else {
-          add_rows<T, E>(a, grad, s + group, e, groups, c, acc);
-        }
-      }
-      join_groups<E>(s_acc, a.lanes_log2, acc);
+      for (int x = 0; x < E; ++x) s_acc[x * 256 + threadIdx.x] = acc[x];
+      __syncthreads();
       if (group == 0 && c < packs) {
-        if (!a.factor) {
+        for (int p = 1; p < groups; ++p)
 #pragma unroll
-          for (int k = 0; k < E; ++k) acc[k] *= a.scale;
-        }
-        store_pack<T, E>(row + (long)c * E, acc);
+          for (int x = 0; x < E; ++x) acc[x] += s_acc[x * 256 + threadIdx.x + (p << a.lanes_log2)];
+        write_row<T, E>(a, row, c, acc);
       }
     }
   }
@@ -500,8 +556,8 @@ int pack_elems(int dtype, int dim, long ld, const void* p, const void* q) {
 }
 
 struct Sizes {
-  long keys, pos, keys2, pos2, counts, factor, chunks, total;   // byte offsets
-  int tiles, bits, passes;
+  long keys, pos, keys2, pos2, counts, factor, first, last, parts, total;   // byte offsets
+  int tiles, subs, threads, digit, passes, bits, chunk_log2;
 };
 
 Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
@@ -509,8 +565,15 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   s.bits = log2_ceil(rows + 1);
   if (s.bits < 1) s.bits = 1;
   s.passes = (s.bits + 9) / 10;
-  s.tiles = (int)((n + 1024 * ITEMS - 1) / (1024 * ITEMS));
-  const int digit = (s.bits + s.passes - 1) / s.passes;
+  s.digit = (s.bits + s.passes - 1) / s.passes;
+  // Tiles of 2048 up to 64 of them, of 8192 up to 128, then longer ones: every tile reads the counts of all.
+  s.threads = n <= 64 * 256 * ITEMS ? 256 : 1024;
+  const long sub = (long)s.threads * ITEMS;
+  s.subs = (int)((n + 128 * sub - 1) / (128 * sub));
+  if (s.subs < 1) s.subs = 1;
+  s.tiles = (int)((n + s.subs * sub - 1) / (s.subs * sub));
+  // A chunk is walked by one group of lanes: short ones while there are few, long ones leave fewer partial sums.
+  s.chunk_log2 = n <= 65536 ? 5 : n <= (1 << 20) ? 6 : 7;
   long at = 0;
   auto take = [&at](long bytes) { const long p = at; at += (bytes + 255) / 256 * 256; return p; };
   s.keys = take(4 * n);
@@ -518,9 +581,11 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   const bool large = n > SMALL_SORT;
   s.keys2 = take(large ? 4 * n : 0);
   s.pos2 = take(large ? 4 * n : 0);
-  s.counts = take(large ? 4l * s.tiles << digit : 0);
+  s.counts = take(large ? 4l * s.tiles << s.digit : 0);
   s.factor = take(mean ? 4 * bags : 0);
-  s.chunks = take(4 * (n / CHUNK) * (long)dim);
+  s.first = take(n > 0 ? 4 * rows : 0);
+  s.last = take(n > 0 ? 4 * rows : 0);
+  s.parts = take(8 * ((n + (1 << s.chunk_log2) - 1) >> s.chunk_log2) * (long)dim);
   s.total = at;
   return s;
 }
@@ -562,59 +627,60 @@ int launch_lookup_ids(const void* table, long ld, int rows, int dim, const void*
   return launch_lookup<T, E, int64_t>((const T*)table, ld, rows, dim, (const int64_t*)ids, bags, tokens, combiner, scale, (T*)out, stream);
 }
 
+template <typename Id, bool FIRST>
+int launch_pass(const Id* ids, const int* keys, const int* pos, long n, int rows, const Sizes& s, int shift, const Prepare& prep, int extra,
+                int* counts, int* keys_out, int* pos_out, hipStream_t stream) {
+  const size_t lds = ((s.threads / 64 + 1) * (size_t)(1 << s.digit) + 16) * sizeof(int);
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)embedding_scatter_kernel<Id, FIRST>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  embedding_digits_kernel<Id, FIRST><<<s.tiles + extra, s.threads, sizeof(int) << s.digit, stream>>>(ids, keys, (int)n, rows, s.tiles, s.subs, shift,
+                                                                                                     s.digit, prep, counts);
+  embedding_scatter_kernel<Id, FIRST><<<s.tiles, s.threads, lds, stream>>>(ids, keys, pos, (int)n, rows, s.subs, shift, s.digit, counts, keys_out, pos_out);
+  return (int)hipGetLastError();
+}
+
 template <typename Id>
-int launch_sort(const Id* ids, long n, int rows, const Sizes& s, char* ws, int** keys, int** pos, hipStream_t stream) {
+int launch_sort(const Id* ids, long n, int rows, const Sizes& s, char* ws, const Prepare& prep, int** keys, int** pos, hipStream_t stream) {
   int* k[2] = {(int*)(ws + s.keys), (int*)(ws + s.keys2)};
   int* p[2] = {(int*)(ws + s.pos), (int*)(ws + s.pos2)};
+  long extra = 1 + (prep.rows > prep.bags * (prep.factor ? 64 : 0) ? prep.rows : prep.bags * 64) / 16384;   // workgroups that prepare the rows
+  if (extra > 512) extra = 512;
   if (n <= SMALL_SORT) {
-    embedding_sort_small_kernel<Id><<<1, 1024, 0, stream>>>(ids, (int)n, rows, s.bits, k[0], p[0]);
+    embedding_sort_small_kernel<Id><<<1 + (unsigned)extra, 1024, 0, stream>>>(ids, (int)n, rows, s.bits, prep, k[0], p[0]);
     *keys = k[0];
     *pos = p[0];
     return (int)hipGetLastError();
   }
   int* counts = (int*)(ws + s.counts);
-  const int digit = (s.bits + s.passes - 1) / s.passes;
-  const size_t lds = (16 * (size_t)(1 << digit) + 16) * sizeof(int);
+  int rc = launch_pass<Id, true>(ids, nullptr, nullptr, n, rows, s, 0, prep, (int)extra, counts, k[0], p[0], stream);
   int from = 0;
-  for (int pass = 0; pass < s.passes; ++pass) {
-    const int shift = pass * digit, to = from ^ 1;
-    if (pass == 0) {
-      embedding_digits_kernel<Id, true><<<s.tiles, 1024, sizeof(int) << digit, stream>>>(ids, nullptr, (int)n, rows, shift, digit, counts);
-      if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)embedding_scatter_kernel<Id, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return (int)e;
-      }
-      embedding_scatter_kernel<Id, true><<<s.tiles, 1024, lds, stream>>>(ids, nullptr, nullptr, (int)n, rows, shift, digit, counts, k[0], p[0]);
-      from = 0;
-    } else {
-      embedding_digits_kernel<Id, false><<<s.tiles, 1024, sizeof(int) << digit, stream>>>(ids, k[from], (int)n, rows, shift, digit, counts);
-      if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)embedding_scatter_kernel<Id, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return (int)e;
-      }
-      embedding_scatter_kernel<Id, false><<<s.tiles, 1024, lds, stream>>>(ids, k[from], p[from], (int)n, rows, shift, digit, counts, k[to], p[to]);
-      from = to;
-    }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
+  for (int pass = 1; pass < s.passes && rc == TFR_OK; ++pass, from ^= 1)
+    rc = launch_pass<Id, false>(ids, k[from], p[from], n, rows, s, pass * s.digit, prep, 0, counts, k[from ^ 1], p[from ^ 1], stream);
   *keys = k[from];
   *pos = p[from];
-  return TFR_OK;
+  return rc;
 }
 
 template <typename T, int E>
-int launch_grad(GradArgs a, const void* grad, void* out, hipStream_t stream) {
+int launch_grad(GradArgs a, const void* grad, hipStream_t stream) {
   const int packs = a.dim / E;
   a.lanes_log2 = log2_ceil(packs < 64 ? packs : 64);
-  // A wave owns rows of about 8 KB in all: enough to hide its search, and the rows of a wide table still fill the card.
+  const int groups = 256 >> a.lanes_log2;
+  // A wave fills rows of about 8 KB in all.
   int wr = 4;
   while (wr < 64 && (long)(2 * wr) * a.dim * (long)sizeof(T) <= 8192) wr *= 2;
   if (wr < (64 >> a.lanes_log2)) wr = 64 >> a.lanes_log2;
   a.wave_rows = wr;
-  const int chunks = a.n / CHUNK;
-  if (chunks > 0) embedding_chunk_kernel<T, E><<<chunks, 256, 0, stream>>>(a, (const T*)grad);
-  embedding_rows_kernel<T, E><<<(unsigned)((a.rows + 4l * wr - 1) / (4l * wr)), 256, 0, stream>>>(a, (const T*)grad, (T*)out);
+  const long chunks = ((long)a.n + (1 << a.chunk_log2) - 1) >> a.chunk_log2;
+  if (chunks > 0) {
+    const int y = (packs + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
+    if (y > 65535) return TFR_EINVAL;
+    embedding_runs_kernel<T, E><<<dim3((unsigned)((chunks + groups - 1) / groups), y), 256, 0, stream>>>(a, (const T*)grad);
+  }
+  const unsigned joins = chunks > 1 ? (unsigned)((chunks - 1 + groups - 1) / groups) : 0;
+  embedding_rows_kernel<T, E><<<joins + (unsigned)((a.rows + 4l * wr - 1) / (4l * wr)), 256, 0, stream>>>(a, (int)joins);
   return (int)hipGetLastError();
 }
 
@@ -677,28 +743,28 @@ extern "C" int tfr_embedding_grad(const void* grad, int dtype, const void* ids, 
   a.scale = scale;
   char* ws = (char*)workspace;
   if (n > 0) {
-    if (mean) {
-      a.factor = (const float*)(ws + s.factor);
-      if (id_type == TFR_IDS_I32)
-        embedding_factor_kernel<int32_t><<<(unsigned)((bags + 3) / 4), 256, 0, st>>>((const int32_t*)ids, bags, tokens, scale, (float*)(ws + s.factor));
-      else
-        embedding_factor_kernel<int64_t><<<(unsigned)((bags + 3) / 4), 256, 0, st>>>((const int64_t*)ids, bags, tokens, scale, (float*)(ws + s.factor));
-    }
+    float* factor = mean ? (float*)(ws + s.factor) : nullptr;
+    a.factor = factor;
+    a.first = (int*)(ws + s.first);
+    a.last = (int*)(ws + s.last);
+    const Prepare prep = {a.first, factor, bags, a.rows, tokens, scale};
     int *keys = nullptr, *pos = nullptr;
-    rc = id_type == TFR_IDS_I32 ? launch_sort<int32_t>((const int32_t*)ids, n, a.rows, s, ws, &keys, &pos, st)
-                                : launch_sort<int64_t>((const int64_t*)ids, n, a.rows, s, ws, &keys, &pos, st);
+    rc = id_type == TFR_IDS_I32 ? launch_sort<int32_t>((const int32_t*)ids, n, a.rows, s, ws, prep, &keys, &pos, st)
+                                : launch_sort<int64_t>((const int64_t*)ids, n, a.rows, s, ws, prep, &keys, &pos, st);
     if (rc != TFR_OK) return rc;
     a.keys = keys;
     a.pos = pos;
-    a.chunks = (float*)(ws + s.chunks);
+    a.parts = (float*)(ws + s.parts);
+    a.chunk_log2 = s.chunk_log2;
   }
+  a.out = grad_table;
   const int e = pack_elems(dtype, dim, dim, n > 0 ? grad : grad_table, grad_table);
-  if (dtype == TFR_DTYPE_F32) return e == 4 ? launch_grad<float, 4>(a, grad, grad_table, st) : launch_grad<float, 1>(a, grad, grad_table, st);
+  if (dtype == TFR_DTYPE_F32) return e == 4 ? launch_grad<float, 4>(a, grad, st) : launch_grad<float, 1>(a, grad, st);
   if (dtype == TFR_DTYPE_BF16)
-    return e == 8   ? launch_grad<__bf16, 8>(a, grad, grad_table, st)
-           : e == 2 ? launch_grad<__bf16, 2>(a, grad, grad_table, st)
-                    : launch_grad<__bf16, 1>(a, grad, grad_table, st);
-  return e == 8   ? launch_grad<_Float16, 8>(a, grad, grad_table, st)
-         : e == 2 ? launch_grad<_Float16, 2>(a, grad, grad_table, st)
-                  : launch_grad<_Float16, 1>(a, grad, grad_table, st);
+    return e == 8   ? launch_grad<__bf16, 8>(a, grad, st)
+           : e == 2 ? launch_grad<__bf16, 2>(a, grad, st)
+                    : launch_grad<__bf16, 1>(a, grad, st);
+  return e == 8   ? launch_grad<_Float16, 8>(a, grad, st)
+         : e == 2 ? launch_grad<_Float16, 2>(a, grad, st)
+                  : launch_grad<_Float16, 1>(a, grad, st);
 }
