@@ -650,7 +650,7 @@ int tfr_token_logprob_grad(const void* logits, int dtype, long per, long stride_
  *   TFR_PREFERENCE_SQUARED  (s_i - s_j - 1/2)^2
  * times scale and the list's weight.  Sums are fp64.  reference, mask (uint8 [B, L, T]), list_weights ([B]) are nullable.
  *   loss [B];  coef [B, L] = d loss[b] / d (any unmasked log prob of the answer); the gradient spreads it over the tokens,
- *   times upstream[b] (nullable).  B * L below 2^24, T at most 2^28; workspace: 8-byte aligned. */
+ *   times upstream[b] (nullable).  B * L below 2^24 - 1, T at most 2^28; workspace: 8-byte aligned. */
 #define TFR_PREFERENCE_LOGISTIC 0
 #define TFR_PREFERENCE_HINGE 1
 #define TFR_PREFERENCE_SQUARED 2
@@ -660,6 +660,12 @@ int tfr_preference_loss_f32(const float* log_probs, const float* reference, cons
                             int normalize, float scale, float* loss, float* coef, void* workspace, long workspace_bytes, void* stream);
 int tfr_preference_grad_f32(const float* coef, const float* upstream, const uint8_t* mask, int B, int L, int T,
                             float* dlog_probs, void* stream);
+/* Both at once: total[0] = sum of the lists' losses, dlog_probs its gradient; lists of up to 8192 tokens in all go from their
+ * sums to their gradient inside one workgroup. */
+int tfr_preference_loss_and_grad_f32(const float* log_probs, const float* reference, const uint8_t* mask, const float* labels,
+                                     const float* list_weights, int B, int L, int T, int kind, float beta, float smoothing,
+                                     int normalize, float scale, float* total, float* dlog_probs, void* workspace,
+                                     long workspace_bytes, void* stream);
 
 /* AdamW (decoupled weight decay) on up to TFR_ADAMW_MAX_TENSORS tensors in one launch; the arrays named _host live in host
  * memory and hold device pointers and element counts.  Parameters and gradients of `dtype`, moments fp32; `step` counts from

@@ -6,6 +6,7 @@ current stream and returns freshly allocated outputs.  No CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -30,6 +31,11 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+# The handle of torch's current stream on a device as an int, without building a Stream object: the short form for entry points
+# whose calls are a few microseconds long.
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def require_device(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -786,6 +792,14 @@ def list_dot(x, w=None):
     return out
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_of(index: int):
+    """A context in which device ``index`` is the current one: nothing to do where it is already."""
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
 def device_guarded(fn):
     """Runs ``fn`` with the HIP device of its first device-tensor argument current, so that ``_stream()`` and every
     allocation inside land on the device the tensors live on (a caller holding cuda:1 tensors while cuda:0 is current
@@ -813,4 +827,4 @@ def _guard_module(namespace, module_name, skip=()):
             namespace[name] = device_guarded(obj)
 
 
-_guard_module(globals(), __name__, skip=('require_device', 'rank_table', 'device_guarded', 'order_cache', 'launch_order', 'tie_keys'))
+_guard_module(globals(), __name__, skip=('require_device', 'rank_table', 'device_guarded', 'device_of', 'order_cache', 'launch_order', 'tie_keys'))

@@ -10,9 +10,8 @@
 // 8 bits: QBLOCK consecutive elements share two scales.  m is held as a signed code of -127 .. 127, the root of v as an unsigned
 // code of 0 .. 255; the root halves the exponent range that 255 steps have to cover.  Codes are the nearest to the updated
 // value, but the code of a positive v is at least 1: a denominator is never rounded down to eps, so small second moments slow
-// an element down and never blow it up.  The update and the choice of the codes run in fp64: a code is one of 255 steps, and
-// which one a value next to a border gets must not hang on fp32 rounding (~25 fp64 operations an element: a third of the memory
-// time).  The parameter's own update uses the moments before they are rounded to codes.  An element whose moments are no longer
+// an element down and never blow it up.  Which code a value next to a border gets is decided in fp64 and does not hang on fp32
+// rounding.  The parameter's own update uses the moments before they are rounded to codes.  An element whose moments are no longer
 // finite keeps the code -128, which stands for NaN, and does not touch its neighbours' scale.
 #include "common.h"
 #include "elem.h"
@@ -112,8 +111,31 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table32 t) {
   }
 }
 
+// The updated moments of one 8-bit element: fp64, in this order, wherever they are needed.
+struct Moments {
+  double m, v;
+};
+__device__ __forceinline__ Moments moments(int mc, float vc, float g, double b1_sm, double b2_sv2, double c1, double c2) {
+  const double gd = (double)g;
+  return {__builtin_fma((double)mc, b1_sm, c1 * gd), __builtin_fma((double)(vc * vc), b2_sv2, c2 * (gd * gd))};
+}
+__device__ __forceinline__ int signed_code(uint2 w, int e) { return (int)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3))); }
+__device__ __forceinline__ float unsigned_code(uint2 w, int e) { return (float)(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 255u); }
+
+// Maximum over the 16 lanes of a row (lane / 16), for all of them: rotations of the row.
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true)));   // row_ror:8
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x124, 0xf, 0xf, true)));   // row_ror:4
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x122, 0xf, 0xf, true)));   // row_ror:2
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x121, 0xf, 0xf, true)));
+}
+
 // A thread takes 8 consecutive elements, 16 lanes a scale.  The codes lie in whole blocks (their tensors are padded), the
 // parameters and gradients end where they end.
+//
+// Codes are chosen in fp32 (the value over the scale is off by at most 255 * 5.5 * 2^-24 = 8.4e-5 of a step) and again in fp64 by the
+// few threads that hold a value within 1e-4 of a border: the same codes as fp64 throughout, at half the instructions (246 M
+// bf16 elements: 787 us with all of it in fp64, bound by instruction issue; 535 us so, 4.6 TB/s, near what a copy reaches).
 template <typename T>
 __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
   const int i = tensor_of(t, blockIdx.x);
@@ -125,15 +147,17 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
   float* __restrict__ ms = t.ms[i];
   float* __restrict__ vs = t.vs[i];
   const Now w = now_of(t.coef);
-  const double b1 = t.coef.b1, c1 = t.coef.c1, b2 = t.coef.b2, c2 = t.coef.c2;
+  const double c1 = t.coef.c1, c2 = t.coef.c2;
   const float eps = t.coef.eps;
-  constexpr int W = sizeof(T) == 4 ? 4 : 8;                    // elements of a 16-byte access
+  const bool tiny_eps = eps < 1e-12f;                          // the fast root takes v below 2^-126 as 0: far below any other eps
+  constexpr int W = 16 / sizeof(T);                            // elements of a 16-byte access
   const bool wide = (((uintptr_t)p | (uintptr_t)g) & 15) == 0;
   const long padded = (n + QBLOCK - 1) / QBLOCK * QBLOCK;
+#pragma unroll 1
   for (int k = 0; k < BLOCK8 / 2048; ++k) {
     const long at = base + k * 2048 + threadIdx.x * 8;
     if (at >= padded) return;                                   // whole groups of 16 lanes
-    float pe[8], ge[8];
+    float pe[8], ge[8], m32[8], root[8], low[8];
     const bool whole = wide && at + 8 <= n;
     if (whole) {
 #pragma unroll
@@ -150,55 +174,93 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
     }
     const uint2 mw = *reinterpret_cast<const uint2*>(m + at), vw = *reinterpret_cast<const uint2*>(v + at);
     const double sm = (double)ms[at / QBLOCK], sv = (double)vs[at / QBLOCK];
-    double md[8], vd[8];
+    const double b1_sm = t.coef.b1 * sm, b2_sv2 = t.coef.b2 * (sv * sv);
     float most_m = 0.f, most_v = 0.f;
-    unsigned lost = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int mc = (int)(int8_t)((e < 4 ? mw.x : mw.y) >> (8 * (e & 3)));
-      const int vc = (int)(((e < 4 ? vw.x : vw.y) >> (8 * (e & 3))) & 255u);
-      const double gd = (double)ge[e], r = (double)vc * sv;
-      md[e] = b1 * ((double)mc * sm) + c1 * gd;
-      vd[e] = b2 * (r * r) + c2 * (gd * gd);
-      float m32 = (float)md[e];
-      const float v32 = (float)vd[e];
-      if (mc == -128) m32 = __builtin_nanf("");
-      pe[e] = updated(pe[e], m32, v32, w, eps);
-      const bool bad = !(fabsf(m32) < INFINITY) || !(v32 < INFINITY);
-      lost |= bad ? 1u << e : 0u;
-      most_m = fmaxf(most_m, bad ? 0.f : fabsf(m32));
-      most_v = fmaxf(most_v, bad ? 0.f : v32);
+      const Moments d = moments(signed_code(mw, e), unsigned_code(vw, e), ge[e], b1_sm, b2_sv2, c1, c2);
+      m32[e] = (float)d.m;
+      root[e] = (float)d.v;
+      low[e] = d.v > 0.0 ? 1.f : 0.f;                           // the least code
+    }
+    unsigned lost = 0;                                          // bit e: the moments are no longer finite
+    const unsigned mx = mw.x ^ 0x80808080u, my = mw.y ^ 0x80808080u;     // a byte of 0 is the code -128
+    float all = 0.f;                                            // a gradient that is not finite shows in v
+#pragma unroll
+    for (int e = 0; e < 8; ++e) all += root[e];
+    if ((((mx - 0x01010101u) & ~mx) | ((my - 0x01010101u) & ~my)) & 0x80808080u || !(all < INFINITY)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (signed_code(mw, e) == -128) m32[e] = __builtin_nanf("");
+        const bool bad = !(fabsf(m32[e]) < INFINITY) || !(root[e] < INFINITY);
+        lost |= bad ? 1u << e : 0u;
+        most_m = fmaxf(most_m, bad ? 0.f : fabsf(m32[e]));
+        most_v = fmaxf(most_v, bad ? 0.f : root[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        most_m = fmaxf(most_m, fabsf(m32[e]));
+        most_v = fmaxf(most_v, root[e]);
+      }
+    }
+    if (tiny_eps) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) root[e] = sqrtf(root[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) root[e] = __builtin_amdgcn_sqrtf(root[e]);
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      most_m = fmaxf(most_m, __shfl_xor(most_m, o, 64));
-      most_v = fmaxf(most_v, __shfl_xor(most_v, o, 64));
-    }
+    for (int e = 0; e < 8; ++e)
+      pe[e] = __builtin_fmaf(-m32[e] * w.step, __builtin_amdgcn_rcpf(__builtin_fmaf(root[e], w.root, eps)), pe[e] * w.decay);
+    most_m = row_max(most_m);
+    most_v = row_max(most_v);
     // in fp64 and rounded once, so that the scale is the same wherever it is computed
-    const float new_sm = (float)((double)most_m / 127.0), new_sv = (float)(sqrt((double)most_v) / 255.0);
-    const double over_m = new_sm > 0.f ? 1.0 / (double)new_sm : 0.0, over_v = new_sv > 0.f ? 1.0 / (double)new_sv : 0.0;
-    const double wide_v = (double)new_sv;
+    const float new_sm = (float)((double)most_m * (1.0 / 127.0)), new_sv = (float)(sqrt((double)most_v) * (1.0 / 255.0));
+    const float over_m = __builtin_amdgcn_rcpf(new_sm), over_v = __builtin_amdgcn_rcpf(new_sv);
+    float km[8], kv[8], side = 0.f;                             // farthest from a code
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float ym = m32[e] * over_m, yv = root[e] * over_v;
+      km[e] = rintf(ym);
+      kv[e] = rintf(yv);
+      side = fmaxf(side, fmaxf(fabsf(ym - km[e]), fabsf(yv - kv[e])));
+      kv[e] = fmaxf(kv[e], low[e]);
+    }
+    // near a border, or scales that fp32 does not divide by
+    const bool near = !(side < 0.4999f) || most_m < 1e-30f || most_v < 1e-30f;
+    if (near) {
+      const double wide_m = new_sm > 0.f ? 1.0 / (double)new_sm : 0.0, wide_v = new_sv > 0.f ? 1.0 / (double)new_sv : 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Moments d = moments(signed_code(mw, e), unsigned_code(vw, e), ge[e], b1_sm, b2_sv2, c1, c2);
+        km[e] = (float)fmin(fmax(rint(d.m * wide_m), -127.0), 127.0);
+        kv[e] = fmaxf((float)fmin(rint(sqrt(d.v) * wide_v), 255.0), new_sv > 0.f ? low[e] : 0.f);
+      }
+    }
     uint2 mo = make_uint2(0u, 0u), vo = make_uint2(0u, 0u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int mc = (int)fmin(fmax(rint(md[e] * over_m), -127.0), 127.0);
-      // nearest code of the root without a root in fp64: the fp32 one is off by at most a step, two squares decide
-      double kd = fmin(rint((double)sqrtf((float)vd[e]) * over_v), 255.0);
-      const double lo = (kd - 0.5) * wide_v, hi = (kd + 0.5) * wide_v;
-      kd += vd[e] < lo * lo && kd > 0.0 ? -1.0 : vd[e] > hi * hi ? 1.0 : 0.0;
-      int vc = (int)fmin(fmax(kd, 1.0), 255.0);
-      if (!(vd[e] > 0.0) || !(new_sv > 0.f)) vc = 0;
-      if (lost & (1u << e)) {
-        mc = -128;
-        vc = 255;
-      }
-      const unsigned mb = ((unsigned)mc & 255u) << (8 * (e & 3)), vb = (unsigned)vc << (8 * (e & 3));
-      if (e < 4) {
-        mo.x |= mb;
-        vo.x |= vb;
-      } else {
-        mo.y |= mb;
-        vo.y |= vb;
+    for (int e = 0; e < 4; ++e) {
+      // bytes of code + 128: the sign's bit is turned for all at once
+      mo.x = __builtin_amdgcn_cvt_pk_u8_f32(km[e] + 128.f, e, mo.x);
+      mo.y = __builtin_amdgcn_cvt_pk_u8_f32(km[e + 4] + 128.f, e, mo.y);
+      vo.x = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e, vo.x);
+      vo.y = __builtin_amdgcn_cvt_pk_u8_f32(kv[e + 4], e, vo.y);
+    }
+    mo.x ^= 0x80808080u;
+    mo.y ^= 0x80808080u;
+    if (lost) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned byte = lost & (1u << e) ? 255u << (8 * (e & 3)) : 0u, sign = byte & 0x80808080u;
+        if (e < 4) {
+          mo.x = (mo.x & ~byte) | sign;
+          vo.x |= byte;
+        } else {
+          mo.y = (mo.y & ~byte) | sign;
+          vo.y |= byte;
+        }
       }
     }
     *reinterpret_cast<uint2*>(m + at) = mo;

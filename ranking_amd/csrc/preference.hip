@@ -17,7 +17,8 @@ using namespace tfr;
 namespace {
 
 constexpr int MAX_ANSWERS = 64;                      // one lane an answer
-constexpr int PART = 8192;                           // tokens of an answer that a workgroup sums
+constexpr int LONG_PART = 8192, SHORT_PART = 2048;   // tokens of an answer that a workgroup sums
+constexpr int SMALL_LIST = 8192;                     // tokens of a list that one workgroup takes from its sums to its gradient
 
 struct PrefArgs {
   const float* lp;
@@ -25,8 +26,8 @@ struct PrefArgs {
   const uint8_t* mask;
   const float* labels;
   const float* weights;
-  int B, L, T, parts, kind;
-  bool normalize;
+  int B, L, T, parts, part, kind;
+  bool normalize, wide;                              // wide: addresses allow 16-byte accesses (4 of the mask) at multiples of 4 tokens
   float beta, smoothing, scale;
 };
 
@@ -35,49 +36,97 @@ struct Sum {
   int n;
 };
 
-__device__ __forceinline__ Sum token_sum(const PrefArgs& a, long seq, int lo, int hi) {
+__device__ __forceinline__ void add_token(Sum& r, float lp, float ref, bool on) {
+  r.s += (double)(on ? lp : 0.f) - (double)(on ? ref : 0.f);     // fp64 holds the difference of two fp32 numbers of like size
+  r.n += on ? 1 : 0;
+}
+
+// Tokens lo .. hi of answer `seq`, by THREADS threads; 4 tokens an access between the first and the last multiple of 4 in memory.
+template <int THREADS>
+__device__ __forceinline__ Sum token_sum(const PrefArgs& a, long seq, int lo, int hi, int tid) {
   Sum r = {0.0, 0};
-  const float* lp = a.lp + seq * a.T;
-  const float* ref = a.ref ? a.ref + seq * a.T : nullptr;
-  const uint8_t* m = a.mask ? a.mask + seq * a.T : nullptr;
-  for (int t = lo + threadIdx.x; t < hi; t += 256) {
-    const bool on = m ? m[t] != 0 : true;
-    const double d = (double)lp[t] - (ref ? (double)ref[t] : 0.0);
-    r.s += on ? d : 0.0;
-    r.n += on ? 1 : 0;
+  const long at = seq * a.T + lo, end = seq * a.T + hi;
+  const auto one = [&](long t) { add_token(r, a.lp[t], a.ref ? a.ref[t] : 0.f, a.mask ? a.mask[t] != 0 : true); };
+  if (!a.wide) {
+    for (long t = at + tid; t < end; t += THREADS) one(t);
+    return r;
+  }
+  long head = (at + 3) & ~3l;
+  if (head > end) head = end;
+  const long tail = head + ((end - head) & ~3l);
+  if (tid < head - at) one(at + tid);
+  if (tid < end - tail) one(tail + tid);
+  for (long t = head + 4 * tid; t < tail; t += 16 * THREADS) {
+    float4 x[4], y[4];
+    uint32_t m[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long u = t + 4l * THREADS * k;
+      if (u < tail) {
+        x[k] = *reinterpret_cast<const float4*>(a.lp + u);
+        y[k] = a.ref ? *reinterpret_cast<const float4*>(a.ref + u) : make_float4(0.f, 0.f, 0.f, 0.f);
+        m[k] = a.mask ? *reinterpret_cast<const uint32_t*>(a.mask + u) : 0x01010101u;
+      } else {
+        x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[k] = 0u;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      add_token(r, x[k].x, y[k].x, (m[k] & 0xffu) != 0);
+      add_token(r, x[k].y, y[k].y, (m[k] & 0xff00u) != 0);
+      add_token(r, x[k].z, y[k].z, (m[k] & 0xff0000u) != 0);
+      add_token(r, x[k].w, y[k].w, (m[k] & 0xff000000u) != 0);
+    }
   }
   return r;
 }
 
-// Thread 0 gets the workgroup's sum (fixed order).
-__device__ __forceinline__ Sum block_sum_tokens(Sum v) {
-  __shared__ double s_s[4];
-  __shared__ int s_n[4];
+// out = m c on tokens lo .. hi of answer `seq`.
+template <int THREADS>
+__device__ __forceinline__ void token_fill(const uint8_t* __restrict__ mask, bool wide, long seq, int T, int lo, int hi, int tid, float c,
+                                           float* __restrict__ out) {
+  const long at = seq * T + lo, end = seq * T + hi;
+  const auto one = [&](long t) { out[t] = (mask ? mask[t] != 0 : true) ? c : 0.f; };
+  if (!wide) {
+    for (long t = at + tid; t < end; t += THREADS) one(t);
+    return;
+  }
+  long head = (at + 3) & ~3l;
+  if (head > end) head = end;
+  const long tail = head + ((end - head) & ~3l);
+  if (tid < head - at) one(at + tid);
+  if (tid < end - tail) one(tail + tid);
+#pragma unroll 4
+  for (long t = head + 4 * tid; t < tail; t += 4 * THREADS) {
+    const uint32_t m = mask ? *reinterpret_cast<const uint32_t*>(mask + t) : 0x01010101u;
+    *reinterpret_cast<float4*>(out + t) = make_float4(m & 0xffu ? c : 0.f, m & 0xff00u ? c : 0.f, m & 0xff0000u ? c : 0.f, m & 0xff000000u ? c : 0.f);
+  }
+}
+
+__device__ __forceinline__ Sum wave_sum_tokens(Sum v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     v.s += __shfl_xor(v.s, o, 64);
     v.n += __shfl_xor(v.n, o, 64);
   }
-  if ((threadIdx.x & 63) == 0) {
-    s_s[threadIdx.x >> 6] = v.s;
-    s_n[threadIdx.x >> 6] = v.n;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0)
-    for (int w = 1; w < 4; ++w) {
-      v.s += s_s[w];
-      v.n += s_n[w];
-    }
   return v;
 }
 
 __global__ __launch_bounds__(256) void preference_sum_kernel(const PrefArgs a, double* __restrict__ part_sum, int* __restrict__ part_n) {
+  __shared__ Sum s_part[4];
   const long seq = blockIdx.x;
-  const int lo = blockIdx.y * PART, hi = lo + PART < a.T ? lo + PART : a.T;
+  const int lo = blockIdx.y * a.part, hi = lo + a.part < a.T ? lo + a.part : a.T;
   Sum v = {0.0, 0};
-  if (a.labels[seq] >= 0.f) v = token_sum(a, seq, lo, hi);
-  v = block_sum_tokens(v);
+  if (a.labels[seq] >= 0.f) v = token_sum<256>(a, seq, lo, hi, threadIdx.x);
+  v = wave_sum_tokens(v);
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) {
+      v.s += s_part[w].s;
+      v.n += s_part[w].n;
+    }
     part_sum[seq * a.parts + blockIdx.y] = v.s;
     part_n[seq * a.parts + blockIdx.y] = v.n;
   }
@@ -85,21 +134,9 @@ __global__ __launch_bounds__(256) void preference_sum_kernel(const PrefArgs a, d
 
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
-// One wavefront, lane i = answer i: the list's loss (all lanes) and this lane's d loss / d sum_t lp_it.
-__device__ __forceinline__ void list_pairs(const PrefArgs& a, int b, const double* __restrict__ part_sum, const int* __restrict__ part_n,
-                                           double* loss_out, double* coef_out) {
-  const int lane = threadIdx.x & 63;
-  double sum = 0.0;
-  int n = 0;
-  float y = -1.f;
-  if (lane < a.L) {
-    const long seq = (long)b * a.L + lane;
-    y = a.labels[seq];
-    for (int p = 0; p < a.parts; ++p) {
-      sum += part_sum[seq * a.parts + p];
-      n += part_n[seq * a.parts + p];
-    }
-  }
+// One wavefront, lane i = answer i with its grade y (-1 behind the last), its sum and number of tokens: the list's loss (all
+// lanes) and this lane's d loss / d sum_t lp_it.
+__device__ __forceinline__ void list_pairs(const PrefArgs& a, int b, float y, double sum, int n, double* loss_out, double* coef_out) {
   const double f = (double)a.beta / (a.normalize ? (double)(n > 0 ? n : 1) : 1.0);
   const double s = f * sum;
   const double w = (a.weights ? (double)a.weights[b] : 1.0) * (double)a.scale;
@@ -140,52 +177,135 @@ __device__ __forceinline__ void list_pairs(const PrefArgs& a, int b, const doubl
 
 __global__ __launch_bounds__(64) void preference_pairs_kernel(const PrefArgs a, const double* __restrict__ part_sum, const int* __restrict__ part_n,
                                                               float* __restrict__ loss, float* __restrict__ coef) {
-  const int b = blockIdx.x;
-  double l, c;
-  list_pairs(a, b, part_sum, part_n, &l, &c);
-  if (threadIdx.x == 0) loss[b] = (float)l;
-  if (threadIdx.x < a.L) coef[(long)b * a.L + threadIdx.x] = (float)c;
+  const int b = blockIdx.x, lane = threadIdx.x;
+  double sum = 0.0, l, c;
+  int n = 0;
+  float y = -1.f;
+  if (lane < a.L) {
+    const long seq = (long)b * a.L + lane;
+    y = a.labels[seq];
+    for (int p = 0; p < a.parts; ++p) {
+      sum += part_sum[seq * a.parts + p];
+      n += part_n[seq * a.parts + p];
+    }
+  }
+  list_pairs(a, b, y, sum, n, &l, &c);
+  if (lane == 0) loss[b] = (float)l;
+  if (lane < a.L) coef[(long)b * a.L + lane] = (float)c;
 }
 
-// dlp[seq, t] = m * coef[seq] * upstream[list]
+// The lists' losses added in fp64, in an order that depends on their number alone.
+__device__ __forceinline__ void total_loss(const float* __restrict__ loss, int B, float* __restrict__ total) {
+  __shared__ double s_part[4];
+  double t = 0.0;
+  for (int b = threadIdx.x; b < B; b += 256) t += (double)loss[b];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) total[0] = (float)(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+}
+
+__global__ __launch_bounds__(256) void preference_total_kernel(const float* __restrict__ loss, int B, float* __restrict__ total) {
+  total_loss(loss, B, total);
+}
+
+// dlp[seq, t] = m * coef[seq] * upstream[list]; the last workgroup of the first part adds the lists' losses where a total is wanted.
 __global__ __launch_bounds__(256) void preference_grad_kernel(const float* __restrict__ coef, const float* __restrict__ upstream,
-                                                              const uint8_t* __restrict__ mask, int L, int T, float* __restrict__ out) {
+                                                              const uint8_t* __restrict__ mask, int L, int T, int part, bool wide,
+                                                              float* __restrict__ out, const float* __restrict__ loss, int B,
+                                                              float* __restrict__ total) {
   const long seq = blockIdx.x;
-  const int lo = blockIdx.y * PART, hi = lo + PART < T ? lo + PART : T;
+  if (seq == (long)B * L) {
+    if (blockIdx.y == 0) total_loss(loss, B, total);
+    return;
+  }
+  const int lo = blockIdx.y * part, hi = lo + part < T ? lo + part : T;
   float c = coef[seq];
   if (upstream) c *= upstream[seq / L];
-  const uint8_t* m = mask ? mask + seq * T : nullptr;
-  float* o = out + seq * T;
-  for (int t = lo + threadIdx.x; t < hi; t += 256) o[t] = (m ? m[t] != 0 : true) ? c : 0.f;
+  token_fill<256>(mask, wide, seq, T, lo, hi, threadIdx.x, c, out);
+}
+
+// A list from its sums to its gradient by one workgroup: an answer a wave and step.
+__global__ __launch_bounds__(256) void preference_list_kernel(const PrefArgs a, float* __restrict__ loss, float* __restrict__ out) {
+  __shared__ Sum s_sum[MAX_ANSWERS];
+  __shared__ float s_coef[MAX_ANSWERS];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = wave; i < a.L; i += 4) {
+    const long seq = (long)b * a.L + i;
+    Sum v = {0.0, 0};
+    if (a.labels[seq] >= 0.f) v = token_sum<64>(a, seq, 0, a.T, lane);
+    v = wave_sum_tokens(v);
+    if (lane == 0) s_sum[i] = v;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const bool here = lane < a.L;
+    double l, c;
+    list_pairs(a, b, here ? a.labels[(long)b * a.L + lane] : -1.f, here ? s_sum[lane].s : 0.0, here ? s_sum[lane].n : 0, &l, &c);
+    if (lane == 0) loss[b] = (float)l;
+    if (here) s_coef[lane] = (float)c;
+  }
+  __syncthreads();
+  for (int i = wave; i < a.L; i += 4) token_fill<64>(a.mask, a.wide, (long)b * a.L + i, a.T, 0, a.T, lane, s_coef[i], out);
 }
 
 constexpr long kMostTokens = 1 << 28;
-constexpr long kMostAnswers = (1l << 24) - 1;        // answers of all lists: a workgroup each, no grid gets 2^32 threads
+constexpr long kMostAnswers = (1l << 24) - 2;        // answers of all lists: a workgroup each and one more, no grid gets 2^32 threads
 
 bool bad_sizes(int B, int L, int T) { return B < 0 || L < 1 || L > MAX_ANSWERS || T < 0 || T > kMostTokens || (long)B * L > kMostAnswers; }
-int parts_of(int T) { return T > 0 ? (T + PART - 1) / PART : 1; }
+// Long parts where there are enough of them to fill the card, short ones else.
+int part_of(int B, int L, int T) { return (long)B * L * T >= (1l << 23) ? LONG_PART : SHORT_PART; }
+int parts_of(int B, int L, int T) { return T > 0 ? (T + part_of(B, L, T) - 1) / part_of(B, L, T) : 1; }
+bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }       // null too
+
+struct Workspace {                                   // sums [B * L * parts], numbers, coefficients [B * L], losses [B]
+  double* sum;
+  int* n;
+  float* coef;
+  float* loss;
+};
+long workspace_bytes_of(int B, int L, int T) { return (long)B * L * parts_of(B, L, T) * 12 + (long)B * L * 4 + (long)B * 4; }
+Workspace workspace_at(void* p, int B, int L, int T) {
+  const long n = (long)B * L * parts_of(B, L, T);
+  Workspace w;
+  w.sum = (double*)p;
+  w.n = (int*)(w.sum + n);
+  w.coef = (float*)(w.n + n);
+  w.loss = w.coef + (long)B * L;
+  return w;
+}
+
+int make_args(PrefArgs* a, const float* log_probs, const float* reference, const uint8_t* mask, const float* labels, const float* list_weights,
+              int B, int L, int T, int kind, float beta, float smoothing, int normalize, float scale) {
+  if (bad_sizes(B, L, T) || kind < TFR_PREFERENCE_LOGISTIC || kind > TFR_PREFERENCE_SQUARED) return TFR_EINVAL;
+  if (!(beta > 0.f) || beta == INFINITY || !(smoothing >= 0.f && smoothing < 0.5f)) return TFR_EINVAL;
+  if (B > 0 && (!labels || (T > 0 && !log_probs))) return TFR_EINVAL;
+  const bool wide = aligned(log_probs, 16) && aligned(reference, 16) && aligned(mask, 4);
+  *a = {log_probs, reference, mask, labels, list_weights, B, L, T, parts_of(B, L, T), part_of(B, L, T), kind, normalize != 0, wide, beta, smoothing, scale};
+  return TFR_OK;
+}
 
 }  // namespace
 
 extern "C" long tfr_preference_workspace_bytes(int B, int L, int T) {
   if (bad_sizes(B, L, T)) return TFR_EINVAL;
-  return (long)B * L * parts_of(T) * 12;
+  return workspace_bytes_of(B, L, T);
 }
 
 extern "C" int tfr_preference_loss_f32(const float* log_probs, const float* reference, const uint8_t* mask, const float* labels,
                                        const float* list_weights, int B, int L, int T, int kind, float beta, float smoothing,
-                                       int normalize, float scale, float* loss, float* coef, void* workspace, long workspace_bytes, void* stream) {
-  if (bad_sizes(B, L, T) || kind < TFR_PREFERENCE_LOGISTIC || kind > TFR_PREFERENCE_SQUARED) return TFR_EINVAL;
-  if (!(beta > 0.f) || beta == INFINITY || !(smoothing >= 0.f && smoothing < 0.5f)) return TFR_EINVAL;
+                                       int normalize, float scale, float* loss, float* coef, void* workspace, long workspace_bytes,
+                                       void* stream) {
+  PrefArgs a;
+  const int rc = make_args(&a, log_probs, reference, mask, labels, list_weights, B, L, T, kind, beta, smoothing, normalize, scale);
+  if (rc != TFR_OK) return rc;
   if (B == 0) return TFR_OK;
-  if (!labels || !loss || !coef || (T > 0 && !log_probs)) return TFR_EINVAL;
-  const PrefArgs a = {log_probs, reference, mask, labels, list_weights, B, L, T, parts_of(T), kind, normalize != 0, beta, smoothing, scale};
-  if (!workspace || workspace_bytes < (long)B * L * a.parts * 12 || ((uintptr_t)workspace & 7)) return TFR_EINVAL;
-  double* part_sum = (double*)workspace;
-  int* part_n = (int*)(part_sum + (long)B * L * a.parts);
+  if (!loss || !coef || !workspace || workspace_bytes < workspace_bytes_of(B, L, T) || !aligned(workspace, 8)) return TFR_EINVAL;
+  const Workspace w = workspace_at(workspace, B, L, T);
   hipStream_t st = (hipStream_t)stream;
-  preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, part_sum, part_n);
-  preference_pairs_kernel<<<B, 64, 0, st>>>(a, part_sum, part_n, loss, coef);
+  preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
+  preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, loss, coef);
   return (int)hipGetLastError();
 }
 
@@ -194,6 +314,30 @@ extern "C" int tfr_preference_grad_f32(const float* coef, const float* upstream,
   if (bad_sizes(B, L, T)) return TFR_EINVAL;
   if (B == 0 || T == 0) return TFR_OK;
   if (!coef || !dlog_probs) return TFR_EINVAL;
-  preference_grad_kernel<<<dim3((unsigned)(B * L), parts_of(T)), 256, 0, (hipStream_t)stream>>>(coef, upstream, mask, L, T, dlog_probs);
+  preference_grad_kernel<<<dim3((unsigned)(B * L), parts_of(B, L, T)), 256, 0, (hipStream_t)stream>>>(
+      coef, upstream, mask, L, T, part_of(B, L, T), aligned(dlog_probs, 16) && aligned(mask, 4), dlog_probs, nullptr, B, nullptr);
+  return (int)hipGetLastError();
+}
+
+extern "C" int tfr_preference_loss_and_grad_f32(const float* log_probs, const float* reference, const uint8_t* mask, const float* labels,
+                                                const float* list_weights, int B, int L, int T, int kind, float beta, float smoothing,
+                                                int normalize, float scale, float* total, float* dlog_probs, void* workspace,
+                                                long workspace_bytes, void* stream) {
+  PrefArgs a;
+  const int rc = make_args(&a, log_probs, reference, mask, labels, list_weights, B, L, T, kind, beta, smoothing, normalize, scale);
+  if (rc != TFR_OK) return rc;
+  if (!total || (B > 0 && T > 0 && !dlog_probs)) return TFR_EINVAL;
+  if (B > 0 && (!workspace || workspace_bytes < workspace_bytes_of(B, L, T) || !aligned(workspace, 8))) return TFR_EINVAL;
+  const Workspace w = workspace_at(workspace, B, L, T);
+  hipStream_t st = (hipStream_t)stream;
+  a.wide = a.wide && aligned(dlog_probs, 16);
+  if (B == 0 || (long)L * T <= SMALL_LIST) {
+    if (B > 0) preference_list_kernel<<<B, 256, 0, st>>>(a, w.loss, dlog_probs);
+    preference_total_kernel<<<1, 256, 0, st>>>(w.loss, B, total);
+  } else {
+    preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
+    preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, w.loss, w.coef);
+    preference_grad_kernel<<<dim3((unsigned)(B * L) + 1, a.parts), 256, 0, st>>>(w.coef, nullptr, mask, L, T, a.part, a.wide, dlog_probs, w.loss, B, total);
+  }
   return (int)hipGetLastError();
 }

@@ -18,8 +18,12 @@ constexpr int SMALL_VOCAB = 2048;          // up to here a wavefront takes a row
 constexpr int SPLIT_MIN = 16384;           // elements of a row that a workgroup gets at least when rows are split
 
 struct Rows {                              // logits[b, t, :] at b * stride_b + t * stride_t
-  long per, stride_b, stride_t;
-  __device__ __forceinline__ long offset(long n) const { return (n / per) * stride_b + (n % per) * stride_t; }
+  unsigned per;
+  long stride_b, stride_t;
+  __device__ __forceinline__ long offset(long n) const {       // n < 2^24
+    const unsigned b = (unsigned)n / per;
+    return b * stride_b + ((unsigned)n - b * per) * stride_t;
+  }
 };
 
 // Running softmax statistics: m = max x, s = sum exp2((x - m) c).
@@ -277,7 +281,7 @@ int splits_of(long n, int vocab) {
 
 bool bad_args(int dtype, long per, long stride_b, long stride_t, long n, int vocab, float temperature) {
   const float inv = 1.f / temperature;
-  return !elem_known(dtype) || n < 0 || n > kMostRows || vocab < 1 || vocab > kMostVocab || per < 1 || stride_b < 0 || stride_t < 0 ||
+  return !elem_known(dtype) || n < 0 || n > kMostRows || vocab < 1 || vocab > kMostVocab || per < 1 || per > UINT32_MAX || stride_b < 0 || stride_t < 0 ||
          !(temperature > 0.f) || !(inv > 0.f) || inv == INFINITY;
 }
 
@@ -326,7 +330,7 @@ extern "C" int tfr_token_logprob(const void* logits, int dtype, long per, long s
   if (!logits || !target || !logp) return TFR_EINVAL;
   const long need = tfr_token_logprob_workspace_bytes(n, vocab);
   if (need > 0 && (!workspace || workspace_bytes < need)) return TFR_EINVAL;
-  const Rows r = {per, stride_b, stride_t};
+  const Rows r = {(unsigned)per, stride_b, stride_t};
   hipStream_t st = (hipStream_t)stream;
   const float inv = 1.f / temperature;
   if (dtype == TFR_DTYPE_F32) return forward<float>((const float*)logits, r, target, n, vocab, inv, logp, stats, (float*)workspace, st);
@@ -340,7 +344,7 @@ extern "C" int tfr_token_logprob_grad(const void* logits, int dtype, long per, l
   if (bad_args(dtype, per, stride_b, stride_t, n, vocab, temperature)) return TFR_EINVAL;
   if (n == 0) return TFR_OK;
   if (!logits || !target || !stats || !upstream || !dlogits) return TFR_EINVAL;
-  const Rows r = {per, stride_b, stride_t};
+  const Rows r = {(unsigned)per, stride_b, stride_t};
   hipStream_t st = (hipStream_t)stream;
   const float inv = 1.f / temperature;
   if (dtype == TFR_DTYPE_F32) return backward<float>((const float*)logits, r, target, stats, upstream, n, vocab, inv, (float*)dlogits, st);

@@ -6,13 +6,14 @@ call, for loops that place gradients themselves (and for stream captures).
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
 
 from . import _lib
 from . import _ops
-from ._ops import _ptr, _stream, require_device
+from ._ops import _raw_stream, require_device
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # TFR_DTYPE_*
 _COMBINERS = {None: 0, 'sum': 1, 'mean': 2}                                # TFR_COMBINER_*
@@ -26,69 +27,88 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _same_device(a: torch.Tensor, b: torch.Tensor, na: str, nb: str) -> None:
-    if a.device != b.device:
-        raise ValueError('%s is on %s, %s on %s' % (na, a.device, nb, b.device))
+def _device_of(name: str, t: torch.Tensor, **others) -> int:
+    """Index of the HIP device that all these tensors are on."""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        require_device(t, name)
+    index = t.get_device()
+    for other, u in others.items():
+        if not torch.is_tensor(u) or not u.is_cuda:
+            require_device(u, other)
+        if u.get_device() != index:
+            raise ValueError('%s is on %s, %s on %s' % (name, t.device, other, u.device))
+    return index
 
 
 def _ids(ids: torch.Tensor, combiner: Optional[str]):
-    """(dense ids, id type, bags, tokens, shape of the lookup without its last axis)."""
-    require_device(ids, 'ids')
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise ValueError('ids must be int32 or int64, got %s' % ids.dtype)
-    if combiner not in _COMBINERS:
-        raise ValueError("combiner must be None, 'sum' or 'mean', got %r" % (combiner,))
-    if combiner is None:
-        bags, tokens, shape = ids.numel(), 1, tuple(ids.shape)
+    """(dense ids, id type, bags, tokens, combiner code, shape of the lookup without its last axis)."""
+    if ids.dtype is torch.int64:
+        id_type = 1
+    elif ids.dtype is torch.int32:
+        id_type = 0
     else:
-        if ids.dim() < 1:
+        raise ValueError('ids must be int32 or int64, got %s' % ids.dtype)
+    code = _COMBINERS.get(combiner)
+    if code is None:
+        raise ValueError("combiner must be None, 'sum' or 'mean', got %r" % (combiner,))
+    shape = tuple(ids.shape)
+    if code == 0:
+        bags, tokens = ids.numel(), 1
+    else:
+        if not shape:
             raise ValueError('a combiner needs ids of [..., tokens]')
-        tokens, shape = ids.shape[-1], tuple(ids.shape[:-1])
-        bags = 1
-        for n in shape:
-            bags *= n
-    if max(bags, bags * tokens) > _MOST:
+        tokens, shape = shape[-1], shape[:-1]
+        bags = ids.numel() // tokens if tokens else math.prod(shape)
+    if bags > _MOST or bags * tokens > _MOST:
         raise ValueError('at most %d lookups a call, got ids of shape %s' % (_MOST, tuple(ids.shape)))
-    return ids.contiguous(), (0 if ids.dtype == torch.int32 else 1), bags, tokens, shape
+    return ids.contiguous(), id_type, bags, tokens, code, shape
 
 
-@_ops.device_guarded
 def _lookup(table, ids, scale, combiner):
+    index = _device_of('table', table, ids=ids)
     code = _dtype_code(table, 'table')
-    ids, id_type, bags, tokens, shape = _ids(ids, combiner)
+    if table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError('table must be [rows, dim], got shape %s' % (tuple(table.shape),))
     rows, dim = table.shape
-    if table.stride(1) != 1 or table.stride(0) < dim:
+    if rows > _MOST:
+        raise ValueError('a table of at most %d rows, got %d' % (_MOST, rows))
+    ids, id_type, bags, tokens, how, shape = _ids(ids, combiner)
+    pitch, step = table.stride()
+    if step != 1 or pitch < dim:
         table = table.contiguous()
-    out = torch.empty(shape + (dim,), dtype=table.dtype, device=table.device)
-    rc = _lib.load().tfr_embedding_lookup(_ptr(table), max(table.stride(0), dim), rows, dim, code, _ptr(ids), id_type, bags, tokens,
-                                          _COMBINERS[combiner], float(scale), _ptr(out), _stream())
-    _lib.check(rc, 'tfr_embedding_lookup')
+        pitch = dim
+    with _ops.device_of(index):
+        out = torch.empty(shape + (dim,), dtype=table.dtype, device=table.device)
+        rc = _lib.load().tfr_embedding_lookup(table.data_ptr(), pitch, rows, dim, code, ids.data_ptr(), id_type, bags, tokens, how, scale,
+                                              out.data_ptr(), _raw_stream(index))
+    if rc:
+        _lib.check(rc, 'tfr_embedding_lookup')
     return out
 
 
-@_ops.device_guarded
 def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: int, scale: float = 1.0,
                    combiner: Optional[str] = None) -> torch.Tensor:
     """Gradient of ``embedding_lookup(table, ids, scale, combiner)`` with respect to the table:
     ``[num_embeddings, dim]`` in ``grad``'s type, sums in fp32, every row written.  The order of the sums depends on
     the ids alone: equal calls give equal bits."""
-    require_device(grad, 'grad')
+    index = _device_of('grad', grad, ids=ids)
     code = _dtype_code(grad, 'grad')
-    ids, id_type, bags, tokens, shape = _ids(ids, combiner)
-    _same_device(grad, ids, 'grad', 'ids')
-    if tuple(grad.shape[:-1]) != shape or grad.dim() < 1 or grad.shape[-1] < 1:
+    ids, id_type, bags, tokens, how, shape = _ids(ids, combiner)
+    if grad.dim() < 1 or tuple(grad.shape[:-1]) != shape or grad.shape[-1] < 1:
         raise ValueError('grad of shape %s does not fit ids of shape %s' % (tuple(grad.shape), tuple(ids.shape)))
     rows, dim = int(num_embeddings), grad.shape[-1]
     if not 0 <= rows <= _MOST:
         raise ValueError('num_embeddings must be in [0, %d], got %d' % (_MOST, rows))
     grad = grad.contiguous()
     lib = _lib.load()
-    out = torch.empty((rows, dim), dtype=grad.dtype, device=grad.device)
-    nbytes = lib.tfr_embedding_grad_workspace_bytes(rows, dim, bags, tokens, _COMBINERS[combiner])
-    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=grad.device) if nbytes > 0 else None
-    rc = lib.tfr_embedding_grad(_ptr(grad), code, _ptr(ids), id_type, bags, tokens, _COMBINERS[combiner], float(scale), rows, dim, _ptr(out),
-                                _ptr(workspace), nbytes, _stream())
-    _lib.check(rc, 'tfr_embedding_grad')
+    with _ops.device_of(index):
+        out = torch.empty((rows, dim), dtype=grad.dtype, device=grad.device)
+        nbytes = lib.tfr_embedding_grad_workspace_bytes(rows, dim, bags, tokens, how)
+        workspace = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=grad.device)
+        rc = lib.tfr_embedding_grad(grad.data_ptr(), code, ids.data_ptr(), id_type, bags, tokens, how, scale, rows, dim, out.data_ptr(),
+                                    workspace.data_ptr(), nbytes, _raw_stream(index))
+    if rc:
+        _lib.check(rc, 'tfr_embedding_grad')
     return out
 
 
@@ -113,13 +133,6 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
     are added (averaged over the ids that are not padding), in fp32, and rounded once: ``ids.shape[:-1] + (dim,)``.
     Ids below 0 are padding: zeros, no gradient.  An id beyond the table gives NaN and no gradient.  Differentiable with
     respect to ``table``; the gradient is a dense tensor of the table's type."""
-    require_device(table, 'table')
-    if table.dim() != 2 or table.shape[1] < 1:
-        raise ValueError('table must be [rows, dim], got shape %s' % (tuple(table.shape),))
-    if table.shape[0] > _MOST:
-        raise ValueError('a table of at most %d rows, got %d' % (_MOST, table.shape[0]))
-    require_device(ids, 'ids')
-    _same_device(table, ids, 'table', 'ids')
-    if torch.is_grad_enabled() and table.requires_grad:
+    if torch.is_grad_enabled() and torch.is_tensor(table) and table.requires_grad:
         return _EmbeddingFn.apply(table, ids, scale, combiner)
     return _lookup(table, ids, scale, combiner)

@@ -811,12 +811,13 @@ class PreferenceLoss(_RankingLoss):
     def _args(self, y_true, y_pred, sample_weight, reference, mask):
         """(y_pred [B, L, T] fp32, arguments of preference.preference_loss)."""
         _ops.require_device(y_pred, 'y_pred')
-        if y_pred.dim() not in (2, 3):
-            raise ValueError('y_pred must be [batch, answers] or [batch, answers, tokens], got shape %s' % (tuple(y_pred.shape),))
         shape = tuple(y_pred.shape)
-        flat = len(shape) == 2
+        if len(shape) not in (2, 3):
+            raise ValueError('y_pred must be [batch, answers] or [batch, answers, tokens], got shape %s' % (shape,))
         y_pred = y_pred.to(torch.float32).contiguous()
-        y_true = torch.as_tensor(y_true, dtype=torch.float32, device=y_pred.device).detach().contiguous()
+        if not torch.is_tensor(y_true) or y_true.device != y_pred.device:
+            y_true = torch.as_tensor(y_true, device=y_pred.device)
+        y_true = y_true.detach().to(torch.float32).contiguous()
         if tuple(y_true.shape) != shape[:2]:
             raise ValueError('y_true of shape %s does not fit y_pred of shape %s' % (tuple(y_true.shape), shape))
         if not 1 <= shape[1] <= _preference.MAX_ANSWERS:
@@ -826,9 +827,9 @@ class PreferenceLoss(_RankingLoss):
                 raise ValueError('%s of shape %s on %s does not fit y_pred of shape %s on %s'
                                  % (name, tuple(t.shape), t.device, shape, y_pred.device))
         if reference is not None:
-            reference = _ops._f32(reference.detach(), 'reference')
-        if mask is not None:
-            mask = _ops._u8(mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0, 'mask')
+            reference = reference.detach().to(torch.float32).contiguous()
+        if mask is not None:                                  # a byte a token: 0 or not
+            mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).contiguous()
         scale = 1.0 if self.reduction in (Reduction.SUM, Reduction.NONE) else 1.0 / max(1, shape[0])
         if sample_weight is not None:
             if not torch.is_tensor(sample_weight) and not hasattr(sample_weight, '__len__'):
@@ -842,7 +843,7 @@ class PreferenceLoss(_RankingLoss):
                 sample_weight = sample_weight.reshape(-1).contiguous()
         how = dict(kind=self._kind, beta=self._beta, label_smoothing=self._label_smoothing,
                    length_normalized=self._length_normalized, scale=scale)
-        return (y_pred.unsqueeze(2) if flat else y_pred), y_true, reference, mask, sample_weight, how
+        return (y_pred if len(shape) == 3 else y_pred.unsqueeze(2)), y_true, reference, mask, sample_weight, how
 
     def __call__(self, y_true, y_pred, sample_weight=None, reference=None, mask=None):
         y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred, sample_weight, reference, mask)
@@ -861,6 +862,5 @@ class PreferenceLoss(_RankingLoss):
         shape = tuple(y_pred.shape) if torch.is_tensor(y_pred) else None
         y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred.detach() if shape is not None else y_pred, sample_weight,
                                                                   reference, mask)
-        losses, coef = _preference.preference_loss(y_pred, y_true, reference, mask, weight, **how)
-        grad = _preference.preference_grad(coef, mask, y_pred.shape[2])
-        return (_ops.list_dot(losses) if losses.numel() else losses.sum()), grad.reshape(shape)
+        total, grad = _preference.preference_loss_and_grad(y_pred, y_true, reference, mask, weight, **how)
+        return total, grad if len(shape) == 3 else grad.reshape(shape)

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from . import _ops
-from ._ops import _ptr, _stream, require_device
+from ._ops import _ptr, _raw_stream, _stream, require_device
 
 QBLOCK = 128                          # TFR_ADAMW_QBLOCK: elements that share a scale
 _MAX_TENSORS, _MAX_TENSORS_8 = 88, 64  # TFR_ADAMW_MAX_TENSORS, TFR_ADAMW8_MAX_TENSORS: tensors of one launch
@@ -37,29 +37,14 @@ def _check_hyper(lr, betas, eps, weight_decay):
         raise ValueError('Invalid weight_decay value: {}'.format(weight_decay))
 
 
+def _refuse(t, like, numel, dtype, name):
+    raise ValueError('%s must be a dense %s tensor of %d elements on %s, got %s of shape %s on %s'
+                     % (name, dtype, numel, like.device, t.dtype, tuple(t.shape), t.device))
+
+
 def _check_dense(t, like, numel, dtype, name):
-    if t.dtype != dtype or t.numel() != numel or not t.is_contiguous() or t.device != like.device:
-        raise ValueError('%s must be a dense %s tensor of %d elements on %s, got %s of shape %s on %s'
-                         % (name, dtype, numel, like.device, t.dtype, tuple(t.shape), t.device))
-
-
-def _array(values):
-    return (ctypes.c_void_p * len(values))(*values)
-
-
-def _launch(items, bits, code, hyper, step, now):
-    """One launch: items = [(param, grad, exp_avg, exp_avg_sq)], their checks done."""
-    lr, (b1, b2), eps, decay = hyper
-    p, g, m, v = zip(*items)
-    addr = lambda ts: _array([t.data_ptr() for t in ts])                    # noqa: E731
-    sizes = (ctypes.c_int64 * len(p))(*[t.numel() for t in p])
-    lib = _lib.load()
-    tail = (sizes, float(lr), float(b1), float(b2), float(eps), float(decay), int(step), _ptr(now), _stream())
-    if bits == 32:
-        _lib.check(lib.tfr_adamw(code, len(p), addr(p), addr(g), addr(m), addr(v), *tail), 'tfr_adamw')
-    else:
-        _lib.check(lib.tfr_adamw8(code, len(p), addr(p), addr(g), addr([x[0] for x in m]), addr([x[1] for x in m]), addr([x[0] for x in v]),
-                                  addr([x[1] for x in v]), *tail), 'tfr_adamw8')
+    if t.dtype is not dtype or t.numel() != numel or t.get_device() != like.get_device() or not t.is_contiguous():
+        _refuse(t, like, numel, dtype, name)
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence, exp_avg_sqs: Sequence, *, step: int,
@@ -75,24 +60,27 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n):
         raise ValueError('lists of %d params, %d grads, %d exp_avgs and %d exp_avg_sqs' % (n, len(grads), len(exp_avgs), len(exp_avg_sqs)))
     _check_hyper(lr, betas, eps, weight_decay)
-    if torch.is_tensor(lr) and now is None:
-        raise ValueError('lr must be a number: a learning rate on the device needs a step that is counted there')
+    if torch.is_tensor(lr):
+        if now is None:
+            raise ValueError('lr must be a number: a learning rate on the device needs a step that is counted there')
+        lr = 0.0
     if now is None and step < 1:
         raise ValueError('step counts from 1, got %r' % (step,))
     if n == 0:
         return
-    if len({p.data_ptr() for p in params if p.numel()}) != sum(1 for p in params if p.numel()):
-        raise ValueError('the same parameter twice')
     eight = isinstance(exp_avgs[0], (tuple, list))
-    launches = {}
+    # Addresses of every tensor, by (device, type): param, grad, exp_avg, exp_avg_sq (8 bits: and their scales), elements.
+    groups, seen = {}, set()
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
-        require_device(p, 'params')
-        if p.dtype not in _DTYPES:
-            raise ValueError('params must be float32, bfloat16 or float16, got %s' % p.dtype)
-        numel = p.numel()
+        device, dtype, numel = p.get_device(), p.dtype, p.numel()
+        if device < 0:
+            require_device(p, 'params')
+        if dtype not in _DTYPES:
+            raise ValueError('params must be float32, bfloat16 or float16, got %s' % dtype)
         if not p.is_contiguous():
             raise ValueError('params must be dense, got strides %s' % (p.stride(),))
-        _check_dense(g, p, numel, p.dtype, 'grads')
+        if g.dtype is not dtype or g.numel() != numel or g.get_device() != device or not g.is_contiguous():
+            _refuse(g, p, numel, dtype, 'grads')
         if isinstance(m, (tuple, list)) != eight or isinstance(v, (tuple, list)) != eight:
             raise ValueError('moments of 8 and of 32 bits in one call')
         if eight:
@@ -101,27 +89,38 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             _check_dense(m[1], p, blocks, torch.float32, 'exp_avgs scales')
             _check_dense(v[0], p, codes, torch.uint8, 'exp_avg_sqs codes')
             _check_dense(v[1], p, blocks, torch.float32, 'exp_avg_sqs scales')
-            if (m[0].data_ptr() | v[0].data_ptr()) & 7:
+            row = (p.data_ptr(), g.data_ptr(), m[0].data_ptr(), m[1].data_ptr(), v[0].data_ptr(), v[1].data_ptr(), numel)
+            if (row[2] | row[4]) & 7:
                 raise ValueError('codes must be 8-byte aligned')
         else:
             _check_dense(m, p, numel, torch.float32, 'exp_avgs')
             _check_dense(v, p, numel, torch.float32, 'exp_avg_sqs')
+            row = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), numel)
         if numel >= _MAX_LAUNCH:
             raise ValueError('params of at most %d elements, got %d' % (_MAX_LAUNCH - 1, numel))
         if numel:
-            launches.setdefault((p.device, p.dtype), []).append((p, g, m, v))
+            if row[0] in seen:
+                raise ValueError('the same parameter twice')
+            seen.add(row[0])
+            groups.setdefault((device, dtype), []).append(row)
     cap = _MAX_TENSORS_8 if eight else _MAX_TENSORS
-    hyper = (0.0 if torch.is_tensor(lr) else lr, betas, eps, weight_decay)
-    for (device, dtype), items in launches.items():
-        with torch.cuda.device(device):
-            part, size = [], 0
-            for it in items:
-                if len(part) == cap or size + it[0].numel() >= _MAX_LAUNCH:
-                    _launch(part, 8 if eight else 32, _DTYPES[dtype], hyper, step, now)
-                    part, size = [], 0
-                part.append(it)
-                size += it[0].numel()
-            _launch(part, 8 if eight else 32, _DTYPES[dtype], hyper, step, now)
+    lib = _lib.load()
+    launch, name = (lib.tfr_adamw8, 'tfr_adamw8') if eight else (lib.tfr_adamw, 'tfr_adamw')
+    for (device, dtype), rows in groups.items():
+        with _ops.device_of(device):
+            tail = (lr, betas[0], betas[1], eps, weight_decay, step, None if now is None else now.data_ptr(), _raw_stream(device))
+            at = 0
+            while at < len(rows):
+                end, size = at, 0
+                while end < len(rows) and end - at < cap and size + rows[end][-1] < _MAX_LAUNCH:
+                    size += rows[end][-1]
+                    end += 1
+                columns = list(zip(*rows[at:end]))
+                addresses = ctypes.c_void_p * (end - at)
+                rc = launch(_DTYPES[dtype], end - at, *[addresses(*c) for c in columns[:-1]], (ctypes.c_int64 * (end - at))(*columns[-1]), *tail)
+                if rc:
+                    _lib.check(rc, name)
+                at = end
 
 
 def _dequantize(codes, scales, dtype, square):
