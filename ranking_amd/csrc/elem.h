@@ -21,8 +21,18 @@ template <typename T, int E> struct Pack { typedef T type __attribute__((ext_vec
 template <typename T> struct Pack<T, 1> { typedef T type; };
 
 template <typename T, int E>
-__device__ __forceinline__ void load_pack(const T* __restrict__ p, float (&v)[E]) {
-  const typename Pack<T, E>::type x = *reinterpret_cast<const typename Pack<T, E>::type*>(p);
+__device__ __forceinline__ typename Pack<T, E>::type load_raw(const T* __restrict__ p) {
+  return *reinterpret_cast<const typename Pack<T, E>::type*>(p);
+}
+
+// The same of what is read once and is larger than the caches.
+template <typename T, int E>
+__device__ __forceinline__ typename Pack<T, E>::type load_raw_stream(const T* __restrict__ p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const typename Pack<T, E>::type*>(p));
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void widen(const typename Pack<T, E>::type x, float (&v)[E]) {
   if constexpr (E == 1) {
     v[0] = (float)x;
   } else {
@@ -32,7 +42,12 @@ __device__ __forceinline__ void load_pack(const T* __restrict__ p, float (&v)[E]
 }
 
 template <typename T, int E>
-__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&v)[E]) {
+__device__ __forceinline__ void load_pack(const T* __restrict__ p, float (&v)[E]) {
+  widen<T, E>(load_raw<T, E>(p), v);
+}
+
+template <typename T, int E>
+__device__ __forceinline__ typename Pack<T, E>::type narrow(const float (&v)[E]) {
   typename Pack<T, E>::type x;
   if constexpr (E == 1) {
     x = (T)v[0];
@@ -40,7 +55,18 @@ __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&v)[E
 #pragma unroll
     for (int i = 0; i < E; ++i) x[i] = (T)v[i];
   }
-  *reinterpret_cast<typename Pack<T, E>::type*>(p) = x;
+  return x;
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&v)[E]) {
+  *reinterpret_cast<typename Pack<T, E>::type*>(p) = narrow<T, E>(v);
+}
+
+// The same past the caches, for results that are larger than them.
+template <typename T, int E>
+__device__ __forceinline__ void store_pack_stream(T* __restrict__ p, const float (&v)[E]) {
+  __builtin_nontemporal_store(narrow<T, E>(v), reinterpret_cast<typename Pack<T, E>::type*>(p));
 }
 
 }  // namespace tfr

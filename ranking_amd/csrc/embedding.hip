@@ -9,7 +9,7 @@
 // The gradient writes every row of dW exactly once and adds in an order that depends on the ids alone: no atomics on floating
 // point, no separate zero fill of rows that are written anyway.
 //   1. The occurrences are sorted by id (stable radix sort, least significant digit first, at most 10 bits a pass).
-//   2. A group of lanes walks a chunk of the sorted list (32 .. 128 occurrences) and adds the rows of each run of equal ids: a run
+//   2. A group of lanes walks a chunk of the sorted list (16 .. 128 occurrences) and adds the rows of each run of equal ids: a run
 //      that lies inside its chunk is a finished row of dW; the part of a run that crosses a chunk's border is left as a partial
 //      sum.  The work is cut by occurrences and not by rows, so a token that is 6 % of the batch costs what the others cost.
 //   3. Runs that cross borders are joined from their partial sums, and rows without an occurrence are filled with zeros.
@@ -22,7 +22,7 @@ namespace {
 
 constexpr int LONG_RUN = 16;            // partial sums from which the whole workgroup joins a run
 constexpr int SMALL_SORT = 4096;        // lookups that one workgroup sorts in LDS
-constexpr int ITEMS = 8;                // items a thread of the large sort holds
+constexpr int ITEMS = 4;                // items a thread of the large sort holds
 
 template <typename Id>
 __device__ __forceinline__ int id_key(const Id* __restrict__ ids, long i, int rows) {
@@ -31,42 +31,31 @@ __device__ __forceinline__ int id_key(const Id* __restrict__ ids, long i, int ro
 }
 
 // ------------------------------------------------------------------------------------------------ lookup
-// A row is handled by a group of `lanes` (a power of two) lanes, E elements a lane and step.
-template <typename T, int E, typename Id, int R>
+// A group of `lanes` (a power of two) lanes takes one step of a row, E elements a lane; the steps of a row are neighbours, so that a
+// workgroup moves whole rows.  One row a group: 8 rows of a group in flight together were slower (262 144 x 2048 bf16: 454 us for
+// 378).  STREAM: results beyond the L2 caches go past them (352 us for 378, and the gradient's kernels behind gain 10 us too).
+template <typename T, int E, typename Id, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_lookup_kernel(const T* __restrict__ table, long ld, int rows, int dim,
-                                                               const Id* __restrict__ ids, long n, int lanes_log2,
+                                                               const Id* __restrict__ ids, unsigned jobs, unsigned steps, int lanes_log2,
                                                                float scale, T* __restrict__ out) {
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const int groups = 256 >> lanes_log2;
-  const long first = (long)blockIdx.x * groups * R + (threadIdx.x >> lanes_log2);
-  const int packs = dim / E;
-  long id[R];
+  const unsigned job = blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (job >= jobs) return;
+  const unsigned row = job / steps;
+  const int c = (int)((job - row * steps) << lanes_log2) + (int)(threadIdx.x & ((1u << lanes_log2) - 1u));
+  if (c >= dim / E) return;
+  const long id = (long)ids[row];
+  float v[E];
+  if (id >= 0 && id < rows) {
+    load_pack<T, E>(table + id * ld + (long)c * E, v);
 #pragma unroll
-  for (int k = 0; k < R; ++k) {
-    const long row = first + (long)k * groups;
-    id[k] = row < n ? (long)ids[row] : -1;
+    for (int e = 0; e < E; ++e) v[e] *= scale;
+  } else {
+    const float fill = id < 0 ? 0.f : __builtin_nanf("");
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = fill;
   }
-  for (int c = lane + blockIdx.y * lanes; c < packs; c += lanes * gridDim.y) {
-    float v[R][E];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      if (id[k] >= 0 && id[k] < rows) {
-        load_pack<T, E>(table + id[k] * ld + (long)c * E, v[k]);
-      } else {
-        const float fill = id[k] < 0 ? 0.f : __builtin_nanf("");
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[k][e] = fill;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const long row = first + (long)k * groups;
-      if (row >= n) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[k][e] *= scale;
-      store_pack<T, E>(out + row * dim + (long)c * E, v[k]);
-    }
-  }
+  if (STREAM) store_pack_stream<T, E>(out + (long)row * dim + (long)c * E, v);
+  else store_pack<T, E>(out + (long)row * dim + (long)c * E, v);
 }
 
 // Pooled: `split` groups share a bag's tokens (1: a group a bag) and are joined through LDS in a fixed order.
@@ -136,26 +125,24 @@ __global__ __launch_bounds__(256) void embedding_bag_kernel(const T* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------------ sort
-// Lanes of the wave whose digit equals this lane's (`live` lanes only).
-__device__ __forceinline__ uint64_t same_digit(int digit, int bits, bool live) {
-  uint64_t m = __ballot(live);
-  for (int b = 0; b < bits; ++b) {
-    const uint64_t one = __ballot((digit >> b) & 1);
-    m &= ((digit >> b) & 1) ? one : ~one;
-  }
-  return m;
-}
-
 // Place of this lane's item among the items of the same digit that the wave has seen, in lane order; `counts` (one counter a
-// digit, this wave's own) is advanced.
+// digit, this wave's own) is advanced.  The lanes of the same digit are found bit by bit; every lane reads its counter and the
+// first of the lanes advances it: LDS serves a wave's accesses in order, so neither waits for the other.
 __device__ __forceinline__ int wave_place(int digit, int bits, bool live, int* counts) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t peers = same_digit(digit, bits, live);
-  const int leader = live ? __ffsll((unsigned long long)peers) - 1 : lane;
-  int before = 0;
-  if (live && lane == leader) before = atomicAdd(&counts[digit], __popcll(peers));
-  before = __shfl(before, leader, 64);
-  return before + __popcll(peers & ((1ull << lane) - 1ull));
+  const uint64_t alive = __ballot(live);
+  uint32_t lo = (uint32_t)alive, hi = (uint32_t)(alive >> 32);
+  for (int b = 0; b < bits; ++b) {
+    const uint32_t mine = (uint32_t)((digit << (31 - b)) >> 31);          // all ones where the bit is set
+    const uint64_t set = __ballot(mine != 0);
+    lo &= ~((uint32_t)set ^ mine);
+    hi &= ~((uint32_t)(set >> 32) ^ mine);
+  }
+  const int below = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+  const int before = counts[digit];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (live && below == 0) atomicAdd(&counts[digit], __popc(lo) + __popc(hi));
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return before + below;
 }
 
 // Exclusive prefix sum over one value a thread; `red` holds 16 ints.
@@ -200,7 +187,7 @@ __device__ __forceinline__ void prepare_rows(const Prepare& p, const Id* __restr
 
 // Workgroup 0 sorts up to SMALL_SORT (id, position) pairs, 8 bits a pass; the others prepare the rows.
 template <typename Id>
-__global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __restrict__ ids, int n, int rows, int bits, const Prepare prep,
+__global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __restrict__ ids, int n, int rows, int bits, int per_bag, const Prepare prep,
                                                                     int* __restrict__ keys_out, int* __restrict__ pos_out) {
   if (blockIdx.x > 0) {
     prepare_rows(prep, ids, blockIdx.x - 1, gridDim.x - 1);
@@ -252,17 +239,19 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __
     const int i = wave * 256 + k * 64 + lane;
     if (i < n) {
       keys_out[i] = (int)(item[k] >> 32);
-      pos_out[i] = (int)(uint32_t)item[k];
+      pos_out[i] = (int)((uint32_t)item[k] / (uint32_t)per_bag);
     }
   }
 }
 
 // The large sort.  One pass = the digit counts of every tile (a workgroup's `subs` * blockDim.x * ITEMS consecutive items), then
-// the scatter, in which a tile adds up the counts of the tiles before it by itself.  FIRST: the keys are the ids themselves, the
+// the scatter, in which a tile adds up the counts of the tiles before it by itself (counts[bin][tile], `pitch` apart) while
+// there are few tiles.  The last
+// pass turns positions into bags (per_bag > 1).  FIRST: the keys are the ids themselves, the
 // positions their indexes, and the workgroups behind the tiles prepare the rows.
 template <typename Id, bool FIRST>
-__global__ __launch_bounds__(1024) void embedding_digits_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, int n, int rows, int tiles,
-                                                                int subs, int shift, int bits, const Prepare prep, int* __restrict__ counts) {
+__global__ __launch_bounds__(256) void embedding_digits_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, int n, int rows, int tiles,
+                                                                int subs, int shift, int bits, int pitch, const Prepare prep, int* __restrict__ counts) {
   if (FIRST && (int)blockIdx.x >= tiles) {
     prepare_rows(prep, ids, blockIdx.x - tiles, gridDim.x - tiles);
     return;
@@ -280,35 +269,81 @@ __global__ __launch_bounds__(1024) void embedding_digits_kernel(const Id* __rest
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < bins; i += blockDim.x) counts[(long)blockIdx.x * bins + i] = s_bins[i];
+  for (int i = threadIdx.x; i < bins; i += blockDim.x) counts[(long)i * pitch + blockIdx.x] = s_bins[i];
+}
+
+// Where there are many tiles, between the two: a wave a bin replaces the tiles' counts by the counts before them.
+__global__ __launch_bounds__(64) void embedding_scan_kernel(int* __restrict__ counts, int tiles, int pitch, int* __restrict__ totals) {
+  const int lane = threadIdx.x;
+  int4* c = reinterpret_cast<int4*>(counts + (long)blockIdx.x * pitch);
+  int carry = 0;
+  for (int t0 = 0; t0 < tiles; t0 += 256) {
+    const int t = t0 + 4 * lane;
+    int4 v = t < tiles ? c[t / 4] : make_int4(0, 0, 0, 0);
+    v.y = t + 1 < tiles ? v.y : 0;
+    v.z = t + 2 < tiles ? v.z : 0;
+    v.w = t + 3 < tiles ? v.w : 0;
+    int x = v.x + v.y + v.z + v.w;
+    const int own = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o, 64);
+      if (lane >= o) x += y;
+    }
+    const int at = carry + x - own;
+    if (t < tiles) c[t / 4] = make_int4(at, at + v.x, at + v.x + v.y, at + v.x + v.y + v.z);
+    carry += __shfl(x, 63, 64);
+  }
+  if (lane == 0) totals[blockIdx.x] = carry;
 }
 
 template <typename Id, bool FIRST>
-__global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, const int* __restrict__ pos,
-                                                                 int n, int rows, int subs, int shift, int bits, const int* __restrict__ counts,
-                                                                 int* __restrict__ keys_out, int* __restrict__ pos_out) {
+__global__ __launch_bounds__(256) void embedding_scatter_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, const int* __restrict__ pos,
+                                                                 int n, int rows, int subs, int shift, int bits, int pitch, int per_bag,
+                                                                 const int* __restrict__ counts, const int* __restrict__ totals,
+                                                                 int* __restrict__ keys_out,
+                                                                 int* __restrict__ pos_out) {
   extern __shared__ int s_count[];                              // [waves][bins], the 16 ints of the prefix sum, the next place of each bin [bins]
   const int bins = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   int* red = s_count + waves * bins;
   int* next = red + 16;
   const int per = bins > (int)blockDim.x ? bins / blockDim.x : 1;        // bins of a thread: 1, 2 or 4, neighbours
+  const auto load_keys = [&](int sub, int (&key)[ITEMS]) {
+    const long base = ((long)blockIdx.x * subs + sub) * ((long)blockDim.x * ITEMS) + wave * (64 * ITEMS);
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const long i = base + k * 64 + lane;
+      key[k] = i < n ? (FIRST ? id_key(ids, i, rows) : keys[i]) : -1;
+    }
+  };
+  int key[ITEMS];
+  load_keys(0, key);                                            // under way while the counts are added up
   int before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0};
-  if (tid * per < bins) {
-    const int* c = counts + tid * per;
+  if (totals) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= per || tid * per >= bins) break;
+      before[j] = counts[(long)(tid * per + j) * pitch + blockIdx.x];
+      total[j] = totals[tid * per + j];
+    }
+  } else if (tid * per < bins) {
     const int tiles = gridDim.x, mine = blockIdx.x;
-    for (int t0 = 0; t0 < tiles; t0 += 8) {
-      int v[8][4];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+    for (int j = 0; j < 4; ++j) {
+      if (j >= per) break;
+      const int4* c = reinterpret_cast<const int4*>(counts + (long)(tid * per + j) * pitch);
+      for (int t0 = 0; t0 < tiles; t0 += 32) {                  // the counts of a bin lie side by side, padded to whole int4
+        int4 v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[u][j] = t0 + u < tiles && j < per ? c[(long)(t0 + u) * bins + j] : 0;
+        for (int u = 0; u < 8; ++u) v[u] = t0 + 4 * u < tiles ? c[t0 / 4 + u] : make_int4(0, 0, 0, 0);
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          before[j] += t0 + u < mine ? v[u][j] : 0;
-          total[j] += v[u][j];
+        for (int u = 0; u < 8; ++u) {
+          const int t = t0 + 4 * u;
+          const int x = t < tiles ? v[u].x : 0, y = t + 1 < tiles ? v[u].y : 0, z = t + 2 < tiles ? v[u].z : 0, w = t + 3 < tiles ? v[u].w : 0;
+          before[j] += (t < mine ? x : 0) + (t + 1 < mine ? y : 0) + (t + 2 < mine ? z : 0) + (t + 3 < mine ? w : 0);
+          total[j] += x + y + z + w;
         }
+      }
     }
   }
   int at = block_exclusive(total[0] + total[1] + total[2] + total[3], red);
@@ -323,11 +358,12 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Id* __res
     for (int i = tid; i < waves * bins; i += blockDim.x) s_count[i] = 0;
     __syncthreads();
     const long base = ((long)blockIdx.x * subs + sub) * ((long)blockDim.x * ITEMS) + wave * (64 * ITEMS);
-    int key[ITEMS], place[ITEMS];
+    int place[ITEMS], from[ITEMS];
+    if (sub > 0) load_keys(sub, key);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       const long i = base + k * 64 + lane;
-      key[k] = i < n ? (FIRST ? id_key(ids, i, rows) : keys[i]) : -1;
+      from[k] = FIRST || i >= n ? (int)i : pos[i];
     }
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) place[k] = wave_place((key[k] >> shift) & (bins - 1), bits, key[k] >= 0, s_count + wave * bins);
@@ -347,7 +383,7 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Id* __res
       if (key[k] < 0) continue;
       const int to = s_count[wave * bins + ((key[k] >> shift) & (bins - 1))] + place[k];
       keys_out[to] = key[k];
-      pos_out[to] = FIRST ? (int)(base + k * 64 + lane) : pos[base + k * 64 + lane];
+      pos_out[to] = per_bag > 1 ? (int)((unsigned)from[k] / (unsigned)per_bag) : from[k];
     }
     __syncthreads();
   }
@@ -356,26 +392,38 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Id* __res
 // ------------------------------------------------------------------------------------------------ gradient
 struct GradArgs {
   const int* keys;                      // [n] sorted ids; rows: no gradient
-  const int* pos;                       // [n] the lookup that each came from
+  const int* pos;                       // [n] the bag that each came from
   const float* factor;                  // [bags] or null: scale for all
   int* first;                           // [rows] where a row's run begins, -1: no occurrence
   int* last;                            // [rows] where it ends (rows with an occurrence)
   void* out;                            // [rows][dim]
   float* parts;                         // [2 * chunks][dim]: of chunk q the run that began before it (2 q) and the one that goes on (2 q + 1)
-  int n, rows, dim, tokens, chunk_log2, lanes_log2, wave_rows;
+  int n, rows, dim, chunk_log2, lanes_log2, wave_rows, steps;    // steps: column steps of a group over a row
   float scale;
 };
 
-// Step 2: a group of lanes a chunk, gridDim.y column steps of the group.
-template <typename T, int E>
+// STREAM: a gradient table beyond the Infinity Cache (256 MB) is written past the caches (131 072 x 2048 bf16: the step's kernels
+// 708 -> 657 us in all; 65 536 x 1024, 134 MB: 45 -> 49 us).
+template <typename T, int E, bool STREAM>
+__device__ __forceinline__ void put_row(T* __restrict__ p, const float (&v)[E]) {
+  if (STREAM) store_pack_stream<T, E>(p, v);
+  else store_pack<T, E>(p, v);
+}
+
+// Step 2: a group of lanes a chunk and column step; the column steps of a chunk are neighbours, so that a workgroup reads whole rows.
+// ONCE: every gradient row is read once (no bags), past the caches: 303 -> 262 us for 1 GB of them.  Rows of bags are read again for
+// every token (24 -> 36 us past the caches for 25 600 bags of 32).
+template <typename T, int E, bool ONCE, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, const T* __restrict__ grad) {
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
-  const long q = (long)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const long job = (long)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const long q = job / a.steps;
+  const int column = (int)(job - q * a.steps);
   const long begin = q << a.chunk_log2;
   if (begin >= a.n) return;
   const int lo = (int)begin, hi = a.n - lo < (1 << a.chunk_log2) ? a.n : lo + (1 << a.chunk_log2);
-  const int c = (blockIdx.y << a.lanes_log2) + lane;
-  const bool on = c < a.dim / E, scribe = lane == 0 && blockIdx.y == 0;
+  const int c = (column << a.lanes_log2) + lane;
+  const bool on = c < a.dim / E, scribe = lane == 0 && column == 0;
   int row = a.keys[lo], start = lo;
   bool began_before = lo > 0 && a.keys[lo - 1] == row;
   float acc[E];
@@ -395,26 +443,32 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, c
       float v[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = a.factor ? acc[e] : acc[e] * a.scale;
-      store_pack<T, E>(static_cast<T*>(a.out) + (long)row * a.dim + (long)c * E, v);
+      put_row<T, E, STREAM>(static_cast<T*>(a.out) + (long)row * a.dim + (long)c * E, v);
     }
   };
-  for (int i = lo; i < hi; i += 8) {
-    int key[8], b[8];
-    float v[8][E], f[8];
+  int next_key[8], next_bag[8];
+  const auto load_ids = [&](int i) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const bool in = i + k < hi;
-      key[k] = in ? a.keys[i + k] : a.rows;
-      b[k] = in ? a.pos[i + k] : 0;
+      next_key[k] = i + k < hi ? a.keys[i + k] : a.rows;
+      next_bag[k] = i + k < hi ? a.pos[i + k] : 0;
     }
+  };
+  load_ids(lo);
+  for (int i = lo; i < hi; i += 8) {
+    int key[8];
+    typename Pack<T, E>::type raw[8];
+    float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (a.tokens > 1) b[k] = (int)((unsigned)b[k] / (unsigned)a.tokens);
+      key[k] = next_key[k];
       if (key[k] < a.rows && on) {
-        load_pack<T, E>(grad + (long)b[k] * a.dim + (long)c * E, v[k]);
-        f[k] = a.factor ? a.factor[b[k]] : 1.f;
+        const T* at = grad + (long)next_bag[k] * a.dim + (long)c * E;
+        raw[k] = ONCE ? load_raw_stream<T, E>(at) : load_raw<T, E>(at);
+        f[k] = a.factor ? a.factor[next_bag[k]] : 1.f;
       }
     }
+    if (i + 8 < hi) load_ids(i + 8);                            // under way with the rows
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (i + k >= hi) break;
@@ -427,8 +481,10 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, c
         for (int e = 0; e < E; ++e) acc[e] = 0.f;
       }
       if (key[k] < a.rows && on) {
+        float v[E];
+        widen<T, E>(raw[k], v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(f[k], v[k][e], acc[e]);
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(f[k], v[e], acc[e]);
       }
     }
   }
@@ -470,7 +526,7 @@ __device__ __forceinline__ void write_row(const GradArgs& a, int row, int c, flo
 
 // Step 3: the first `joins` workgroups join the runs that cross the borders of their chunks (a group of lanes a border; long
 // runs the whole workgroup, through LDS in a fixed order), the others fill the rows that have no occurrence.
-template <typename T, int E>
+template <typename T, int E, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(const GradArgs a, int joins) {
   __shared__ float s_acc[256 * E];
   __shared__ int s_long[256], s_longs;
@@ -488,7 +544,7 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const GradArgs a, i
     for (int r = wlane >> a.lanes_log2; r < many; r += 64 >> a.lanes_log2) {
       if (!((empty >> r) & 1)) continue;
       T* o = static_cast<T*>(a.out) + (r0 + r) * a.dim;
-      for (int c = lane; c < packs; c += lanes) store_pack<T, E>(o + (long)c * E, zero);
+      for (int c = lane; c < packs; c += lanes) put_row<T, E, STREAM>(o + (long)c * E, zero);
     }
     return;
   }
@@ -557,7 +613,7 @@ int pack_elems(int dtype, int dim, long ld, const void* p, const void* q) {
 
 struct Sizes {
   long keys, pos, keys2, pos2, counts, factor, first, last, parts, total;   // byte offsets
-  int tiles, subs, threads, digit, passes, bits, chunk_log2;
+  int tiles, pitch, subs, digit, passes, bits, chunk_log2;
 };
 
 Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
@@ -566,14 +622,15 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   if (s.bits < 1) s.bits = 1;
   s.passes = (s.bits + 9) / 10;
   s.digit = (s.bits + s.passes - 1) / s.passes;
-  // Tiles of 2048 up to 64 of them, of 8192 up to 128, then longer ones: every tile reads the counts of all.
-  s.threads = n <= 64 * 256 * ITEMS ? 256 : 1024;
-  const long sub = (long)s.threads * ITEMS;
-  s.subs = (int)((n + 128 * sub - 1) / (128 * sub));
+  // Tiles of 1024, longer ones from 1 M lookups on; up to 32 of them a tile adds up the others' counts (128 bytes a bin, one
+  // round of loads), beyond a launch of its own does it for all.
+  const long tile = 256 * ITEMS;
+  s.subs = (int)((n + 1024 * tile - 1) / (1024 * tile));
   if (s.subs < 1) s.subs = 1;
-  s.tiles = (int)((n + s.subs * sub - 1) / (s.subs * sub));
+  s.tiles = (int)((n + s.subs * tile - 1) / (s.subs * tile));
+  s.pitch = (s.tiles + 3) / 4 * 4;
   // A chunk is walked by one group of lanes: short ones while there are few, long ones leave fewer partial sums.
-  s.chunk_log2 = n <= 65536 ? 5 : n <= (1 << 20) ? 6 : 7;
+  s.chunk_log2 = n <= 32768 ? 4 : n <= 65536 ? 5 : n <= (1 << 20) ? 6 : 7;
   long at = 0;
   auto take = [&at](long bytes) { const long p = at; at += (bytes + 255) / 256 * 256; return p; };
   s.keys = take(4 * n);
@@ -581,7 +638,7 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   const bool large = n > SMALL_SORT;
   s.keys2 = take(large ? 4 * n : 0);
   s.pos2 = take(large ? 4 * n : 0);
-  s.counts = take(large ? 4l * s.tiles << s.digit : 0);
+  s.counts = take(large ? 4l * (s.pitch + 1) << s.digit : 0);
   s.factor = take(mean ? 4 * bags : 0);
   s.first = take(n > 0 ? 4 * rows : 0);
   s.last = take(n > 0 ? 4 * rows : 0);
@@ -597,16 +654,11 @@ int launch_lookup(const T* table, long ld, int rows, int dim, const Id* ids, lon
   const int lg = log2_ceil(packs < 64 ? packs : 64);
   const int groups = 256 >> lg;
   if (combiner == TFR_COMBINER_NONE) {
-    // Few lookups: a row's columns are spread over workgroups too; many: four rows of a group are in flight together.
-    if (bags >= 4l * groups * 1024) {
-      embedding_lookup_kernel<T, E, Id, 4><<<dim3((unsigned)((bags + 4 * groups - 1) / (4 * groups))), 256, 0, stream>>>(
-          table, ld, rows, dim, ids, bags, lg, scale, out);
-    } else {
-      int y = (packs + (1 << lg) - 1) >> lg;
-      if (y > 16) y = 16;
-      embedding_lookup_kernel<T, E, Id, 1><<<dim3((unsigned)((bags + groups - 1) / groups), y), 256, 0, stream>>>(
-          table, ld, rows, dim, ids, bags, lg, scale, out);
-    }
+    const long steps = (packs + (1 << lg) - 1) >> lg, jobs = bags * steps;
+    if (jobs >= (1l << 26)) return TFR_EINVAL;                  // no grid of 2^32 threads
+    const bool stream_out = bags * dim * (long)sizeof(T) > (32l << 20);    // eight L2 caches of 4 MB
+    const auto kernel = stream_out ? embedding_lookup_kernel<T, E, Id, true> : embedding_lookup_kernel<T, E, Id, false>;
+    kernel<<<(unsigned)((jobs + groups - 1) / groups), 256, 0, stream>>>(table, ld, rows, dim, ids, (unsigned)jobs, (unsigned)steps, lg, scale, out);
   } else {
     int split = 0;                       // few bags: share a bag's tokens among groups, at least eight tokens each
     while ((2 << split) <= groups && (bags << split) * (packs >> lg > 0 ? packs >> lg : 1) < 8192 && (tokens >> (split + 1)) >= 8) ++split;
@@ -628,16 +680,15 @@ int launch_lookup_ids(const void* table, long ld, int rows, int dim, const void*
 }
 
 template <typename Id, bool FIRST>
-int launch_pass(const Id* ids, const int* keys, const int* pos, long n, int rows, const Sizes& s, int shift, const Prepare& prep, int extra,
-                int* counts, int* keys_out, int* pos_out, hipStream_t stream) {
-  const size_t lds = ((s.threads / 64 + 1) * (size_t)(1 << s.digit) + 16) * sizeof(int);
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)embedding_scatter_kernel<Id, FIRST>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return (int)e;
-  }
-  embedding_digits_kernel<Id, FIRST><<<s.tiles + extra, s.threads, sizeof(int) << s.digit, stream>>>(ids, keys, (int)n, rows, s.tiles, s.subs, shift,
-                                                                                                     s.digit, prep, counts);
-  embedding_scatter_kernel<Id, FIRST><<<s.tiles, s.threads, lds, stream>>>(ids, keys, pos, (int)n, rows, s.subs, shift, s.digit, counts, keys_out, pos_out);
+int launch_pass(const Id* ids, const int* keys, const int* pos, long n, int rows, const Sizes& s, int shift, int per_bag, const Prepare& prep,
+                int extra, int* counts, int* keys_out, int* pos_out, hipStream_t stream) {
+  const size_t lds = (5 * (size_t)(1 << s.digit) + 16) * sizeof(int);     // at most 10 bits: 20 KB
+  int* totals = s.tiles > 32 ? counts + ((long)s.pitch << s.digit) : nullptr;
+  embedding_digits_kernel<Id, FIRST><<<s.tiles + extra, 256, sizeof(int) << s.digit, stream>>>(ids, keys, (int)n, rows, s.tiles, s.subs, shift,
+                                                                                                     s.digit, s.pitch, prep, counts);
+  if (totals) embedding_scan_kernel<<<1 << s.digit, 64, 0, stream>>>(counts, s.tiles, s.pitch, totals);
+  embedding_scatter_kernel<Id, FIRST><<<s.tiles, 256, lds, stream>>>(ids, keys, pos, (int)n, rows, s.subs, shift, s.digit, s.pitch, per_bag,
+                                                                           counts, totals, keys_out, pos_out);
   return (int)hipGetLastError();
 }
 
@@ -645,26 +696,28 @@ template <typename Id>
 int launch_sort(const Id* ids, long n, int rows, const Sizes& s, char* ws, const Prepare& prep, int** keys, int** pos, hipStream_t stream) {
   int* k[2] = {(int*)(ws + s.keys), (int*)(ws + s.keys2)};
   int* p[2] = {(int*)(ws + s.pos), (int*)(ws + s.pos2)};
-  long extra = 1 + (prep.rows > prep.bags * (prep.factor ? 64 : 0) ? prep.rows : prep.bags * 64) / 16384;   // workgroups that prepare the rows
-  if (extra > 512) extra = 512;
+  long extra = 1 + prep.rows / 4096;                             // workgroups that prepare the rows
+  if (prep.factor && extra < prep.bags / 16) extra = prep.bags / 16;
+  if (extra > 2048) extra = 2048;
   if (n <= SMALL_SORT) {
-    embedding_sort_small_kernel<Id><<<1 + (unsigned)extra, 1024, 0, stream>>>(ids, (int)n, rows, s.bits, prep, k[0], p[0]);
+    embedding_sort_small_kernel<Id><<<1 + (unsigned)extra, 1024, 0, stream>>>(ids, (int)n, rows, s.bits, prep.tokens, prep, k[0], p[0]);
     *keys = k[0];
     *pos = p[0];
     return (int)hipGetLastError();
   }
   int* counts = (int*)(ws + s.counts);
-  int rc = launch_pass<Id, true>(ids, nullptr, nullptr, n, rows, s, 0, prep, (int)extra, counts, k[0], p[0], stream);
+  int rc = launch_pass<Id, true>(ids, nullptr, nullptr, n, rows, s, 0, s.passes == 1 ? prep.tokens : 1, prep, (int)extra, counts, k[0], p[0], stream);
   int from = 0;
   for (int pass = 1; pass < s.passes && rc == TFR_OK; ++pass, from ^= 1)
-    rc = launch_pass<Id, false>(ids, k[from], p[from], n, rows, s, pass * s.digit, prep, 0, counts, k[from ^ 1], p[from ^ 1], stream);
+    rc = launch_pass<Id, false>(ids, k[from], p[from], n, rows, s, pass * s.digit, pass + 1 == s.passes ? prep.tokens : 1, prep, 0, counts, k[from ^ 1],
+                                p[from ^ 1], stream);
   *keys = k[from];
   *pos = p[from];
   return rc;
 }
 
-template <typename T, int E>
-int launch_grad(GradArgs a, const void* grad, hipStream_t stream) {
+template <typename T, int E, bool STREAM>
+int launch_rows(GradArgs a, const void* grad, bool once, hipStream_t stream) {
   const int packs = a.dim / E;
   a.lanes_log2 = log2_ceil(packs < 64 ? packs : 64);
   const int groups = 256 >> a.lanes_log2;
@@ -675,13 +728,21 @@ int launch_grad(GradArgs a, const void* grad, hipStream_t stream) {
   a.wave_rows = wr;
   const long chunks = ((long)a.n + (1 << a.chunk_log2) - 1) >> a.chunk_log2;
   if (chunks > 0) {
-    const int y = (packs + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
-    if (y > 65535) return TFR_EINVAL;
-    embedding_runs_kernel<T, E><<<dim3((unsigned)((chunks + groups - 1) / groups), y), 256, 0, stream>>>(a, (const T*)grad);
+    a.steps = (packs + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
+    const long blocks = (chunks * a.steps + groups - 1) / groups;
+    if (blocks >= (1l << 24)) return TFR_EINVAL;                // no grid of 2^32 threads
+    if (once) embedding_runs_kernel<T, E, true, STREAM><<<(unsigned)blocks, 256, 0, stream>>>(a, (const T*)grad);
+    else embedding_runs_kernel<T, E, false, STREAM><<<(unsigned)blocks, 256, 0, stream>>>(a, (const T*)grad);
   }
   const unsigned joins = chunks > 1 ? (unsigned)((chunks - 1 + groups - 1) / groups) : 0;
-  embedding_rows_kernel<T, E><<<joins + (unsigned)((a.rows + 4l * wr - 1) / (4l * wr)), 256, 0, stream>>>(a, (int)joins);
+  embedding_rows_kernel<T, E, STREAM><<<joins + (unsigned)((a.rows + 4l * wr - 1) / (4l * wr)), 256, 0, stream>>>(a, (int)joins);
   return (int)hipGetLastError();
+}
+
+template <typename T, int E>
+int launch_grad(const GradArgs& a, const void* grad, bool once, hipStream_t stream) {
+  if ((long)a.rows * a.dim * (long)sizeof(T) > (256l << 20)) return launch_rows<T, E, true>(a, grad, once, stream);
+  return launch_rows<T, E, false>(a, grad, once, stream);
 }
 
 constexpr long kMost = 1l << 25;        // rows, bags and lookups: no grid gets 2^32 threads, and indexes stay in 32 bits
@@ -739,7 +800,6 @@ extern "C" int tfr_embedding_grad(const void* grad, int dtype, const void* ids, 
   a.n = (int)n;
   a.rows = (int)rows;
   a.dim = dim;
-  a.tokens = tokens;
   a.scale = scale;
   char* ws = (char*)workspace;
   if (n > 0) {
@@ -759,12 +819,12 @@ extern "C" int tfr_embedding_grad(const void* grad, int dtype, const void* ids, 
   }
   a.out = grad_table;
   const int e = pack_elems(dtype, dim, dim, n > 0 ? grad : grad_table, grad_table);
-  if (dtype == TFR_DTYPE_F32) return e == 4 ? launch_grad<float, 4>(a, grad, st) : launch_grad<float, 1>(a, grad, st);
+  if (dtype == TFR_DTYPE_F32) return e == 4 ? launch_grad<float, 4>(a, grad, tokens == 1, st) : launch_grad<float, 1>(a, grad, tokens == 1, st);
   if (dtype == TFR_DTYPE_BF16)
-    return e == 8   ? launch_grad<__bf16, 8>(a, grad, st)
-           : e == 2 ? launch_grad<__bf16, 2>(a, grad, st)
-                    : launch_grad<__bf16, 1>(a, grad, st);
-  return e == 8   ? launch_grad<_Float16, 8>(a, grad, st)
-         : e == 2 ? launch_grad<_Float16, 2>(a, grad, st)
-                  : launch_grad<_Float16, 1>(a, grad, st);
+    return e == 8   ? launch_grad<__bf16, 8>(a, grad, tokens == 1, st)
+           : e == 2 ? launch_grad<__bf16, 2>(a, grad, tokens == 1, st)
+                    : launch_grad<__bf16, 1>(a, grad, tokens == 1, st);
+  return e == 8   ? launch_grad<_Float16, 8>(a, grad, tokens == 1, st)
+         : e == 2 ? launch_grad<_Float16, 2>(a, grad, tokens == 1, st)
+                  : launch_grad<_Float16, 1>(a, grad, tokens == 1, st);
 }
