@@ -629,8 +629,11 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   if (s.subs < 1) s.subs = 1;
   s.tiles = (int)((n + s.subs * tile - 1) / (s.subs * tile));
   s.pitch = (s.tiles + 3) / 4 * 4;
-  // A chunk is walked by one group of lanes: short ones while there are few, long ones leave fewer partial sums.
-  s.chunk_log2 = n <= 32768 ? 4 : n <= 65536 ? 5 : n <= (1 << 20) ? 6 : 7;
+  // A chunk is walked by one group of lanes: as long as some thousand waves are left (long chunks leave fewer partial sums), at
+  // least 16 occurrences.
+  const long lanes = dim >= 256 ? 64 : 1l << log2_ceil((dim + 3) / 4);
+  s.chunk_log2 = 4;
+  while (s.chunk_log2 < (n <= (1 << 20) ? 6 : 7) && (2l << s.chunk_log2) * 65536 <= n * lanes) ++s.chunk_log2;
   long at = 0;
   auto take = [&at](long bytes) { const long p = at; at += (bytes + 255) / 256 * 256; return p; };
   s.keys = take(4 * n);

@@ -14,8 +14,8 @@ using namespace tfr;
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int SMALL_VOCAB = 2048;          // up to here a wavefront takes a row
-constexpr int SPLIT_MIN = 16384;           // elements of a row that a workgroup gets at least when rows are split
+constexpr int SMALL_VOCAB = 2048;          // up to here a wavefront or a part of it takes a row
+constexpr int SPLIT_MIN = 4096;           // elements of a row that a workgroup gets at least when rows are split
 
 struct Rows {                              // logits[b, t, :] at b * stride_b + t * stride_t
   unsigned per;
@@ -47,9 +47,11 @@ struct Stat {
   }
 };
 
+// The statistics of LANES neighbouring lanes, for all of them.
+template <int LANES = 64>
 __device__ __forceinline__ Stat wave_stat(Stat a, float c) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
+  for (int o = LANES / 2; o > 0; o >>= 1) {
     Stat b;
     b.m = __shfl_xor(a.m, o, 64);
     b.s = __shfl_xor(a.s, o, 64);
@@ -118,13 +120,14 @@ __device__ __forceinline__ void write_none(float* logp, float* stats) {
   if (stats) stats[0] = stats[1] = 0.f;
 }
 
-template <typename T>
+// Short rows: LANES lanes a row.
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void logprob_wave_kernel(const T* __restrict__ logits, const Rows rows, const int64_t* __restrict__ target,
                                                            long n, int vocab, float inv_t, float* __restrict__ logp,
                                                            float* __restrict__ stats) {
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long row = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   if (row >= n) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & (LANES - 1);
   const long y = target[row];
   float* st = stats ? stats + 2 * row : nullptr;
   if (y < 0) {
@@ -133,7 +136,7 @@ __global__ __launch_bounds__(256) void logprob_wave_kernel(const T* __restrict__
   }
   const T* x = logits + rows.offset(row);
   const float c = inv_t * kLog2e;
-  const Stat a = wave_stat(row_stat<T, 64>(x, 0, vocab, lane, c), c);
+  const Stat a = wave_stat<LANES>(row_stat<T, LANES>(x, 0, vocab, lane, c), c);
   if (lane == 0) write_logp(x, y, vocab, a, inv_t, logp + row, st);
 }
 
@@ -248,13 +251,13 @@ __device__ __forceinline__ void grad_part(const T* __restrict__ logits, const Ro
   }
 }
 
-template <typename T>
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void logprob_grad_wave_kernel(const T* __restrict__ logits, const Rows rows, const int64_t* __restrict__ target,
                                                                 const float* __restrict__ stats, const float* __restrict__ upstream, long n,
                                                                 int vocab, float inv_t, T* __restrict__ out) {
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long row = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   if (row >= n) return;
-  grad_part<T, 64>(logits, rows, target, stats, upstream, row, vocab, 0, vocab, threadIdx.x & 63, inv_t, out);
+  grad_part<T, LANES>(logits, rows, target, stats, upstream, row, vocab, 0, vocab, threadIdx.x & (LANES - 1), inv_t, out);
 }
 
 template <typename T>
@@ -285,11 +288,20 @@ bool bad_args(int dtype, long per, long stride_b, long stride_t, long n, int voc
          !(temperature > 0.f) || !(inv > 0.f) || inv == INFINITY;
 }
 
+// Lanes of a short row: a few 16-byte accesses each.
+template <typename T>
+int lanes_of(int vocab) {
+  const long bytes = (long)vocab * (long)sizeof(T);
+  return bytes <= 256 ? 8 : bytes <= 1024 ? 16 : 64;
+}
+
 template <typename T>
 int forward(const T* logits, Rows rows, const int64_t* target, long n, int vocab, float inv_t, float* logp, float* stats, float* parts,
             hipStream_t st) {
   if (vocab <= SMALL_VOCAB) {
-    logprob_wave_kernel<T><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(logits, rows, target, n, vocab, inv_t, logp, stats);
+    const int lanes = lanes_of<T>(vocab);
+    const auto kernel = lanes == 8 ? logprob_wave_kernel<T, 8> : lanes == 16 ? logprob_wave_kernel<T, 16> : logprob_wave_kernel<T, 64>;
+    kernel<<<(unsigned)((n * lanes + 255) / 256), 256, 0, st>>>(logits, rows, target, n, vocab, inv_t, logp, stats);
     return (int)hipGetLastError();
   }
   const int splits = splits_of(n, vocab);
@@ -304,7 +316,9 @@ template <typename T>
 int backward(const T* logits, Rows rows, const int64_t* target, const float* stats, const float* upstream, long n, int vocab, float inv_t,
              T* out, hipStream_t st) {
   if (vocab <= SMALL_VOCAB) {
-    logprob_grad_wave_kernel<T><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(logits, rows, target, stats, upstream, n, vocab, inv_t, out);
+    const int lanes = lanes_of<T>(vocab);
+    const auto kernel = lanes == 8 ? logprob_grad_wave_kernel<T, 8> : lanes == 16 ? logprob_grad_wave_kernel<T, 16> : logprob_grad_wave_kernel<T, 64>;
+    kernel<<<(unsigned)((n * lanes + 255) / 256), 256, 0, st>>>(logits, rows, target, stats, upstream, n, vocab, inv_t, out);
   } else {
     const int part = 256 * 8 * (16 / (int)sizeof(T));
     logprob_grad_block_kernel<T><<<dim3((unsigned)n, (vocab + part - 1) / part), 256, 0, st>>>(logits, rows, target, stats, upstream, vocab,

@@ -37,14 +37,83 @@ def _check_hyper(lr, betas, eps, weight_decay):
         raise ValueError('Invalid weight_decay value: {}'.format(weight_decay))
 
 
-def _refuse(t, like, numel, dtype, name):
-    raise ValueError('%s must be a dense %s tensor of %d elements on %s, got %s of shape %s on %s'
-                     % (name, dtype, numel, like.device, t.dtype, tuple(t.shape), t.device))
-
-
 def _check_dense(t, like, numel, dtype, name):
     if t.dtype is not dtype or t.numel() != numel or t.get_device() != like.get_device() or not t.is_contiguous():
-        _refuse(t, like, numel, dtype, name)
+        raise ValueError('%s must be a dense %s tensor of %d elements on %s, got %s of shape %s on %s'
+                         % (name, dtype, numel, like.device, t.dtype, tuple(t.shape), t.device))
+
+
+def _uniform(params, grads, exp_avgs, exp_avg_sqs, eight):
+    """The addresses of tensors of one device and type, all of them as they have to be; None where a closer look is needed
+    (``_grouped``: several devices or types, nothing in a tensor, or something to refuse).  Whole lists at a time: a tower's
+    14 tensors go in 25 us with the launch, 31 one by one."""
+    T = torch.Tensor
+    lists = [params, grads]
+    for moments in (exp_avgs, exp_avg_sqs):
+        if not eight:
+            lists.append(moments)
+        elif all(isinstance(x, (tuple, list)) and len(x) == 2 for x in moments):
+            lists += zip(*moments)
+        else:
+            return None
+    try:
+        device, dtype = params[0].get_device(), params[0].dtype
+        wanted = [dtype, dtype] + ([torch.int8, torch.float32, torch.uint8, torch.float32] if eight else [torch.float32] * 2)
+        sizes = list(map(T.numel, params))
+        fit = [sizes] * 4
+        if eight:
+            scales = [-(-n // QBLOCK) for n in sizes]
+            codes = [n * QBLOCK for n in scales]
+            fit = [sizes, sizes, codes, scales, codes, scales]
+        for ts, d, n in zip(lists, wanted, fit):
+            if ({t.dtype for t in ts} != {d} or set(map(T.get_device, ts)) != {device} or not all(map(T.is_contiguous, ts))
+                    or list(map(T.numel, ts)) != n):
+                return None
+        columns = [list(map(T.data_ptr, ts)) for ts in lists]
+    except (TypeError, AttributeError):
+        return None
+    if (device < 0 or dtype not in _DTYPES or min(sizes) == 0 or max(sizes) >= _MAX_LAUNCH or len(set(columns[0])) != len(columns[0])
+            or (eight and any((a | b) & 7 for a, b in zip(columns[2], columns[4])))):
+        return None
+    return {(device, dtype): list(zip(*columns, sizes))}
+
+
+def _grouped(params, grads, exp_avgs, exp_avg_sqs, eight):
+    """By (device, type), the addresses of every tensor that holds something: param, grad, exp_avg, exp_avg_sq (8 bits: codes
+    and scales of both), and its number of elements."""
+    groups, seen = {}, set()
+    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+        device, dtype, numel = p.get_device(), p.dtype, p.numel()
+        if device < 0:
+            require_device(p, 'params')
+        if dtype not in _DTYPES:
+            raise ValueError('params must be float32, bfloat16 or float16, got %s' % dtype)
+        if not p.is_contiguous():
+            raise ValueError('params must be dense, got strides %s' % (p.stride(),))
+        _check_dense(g, p, numel, dtype, 'grads')
+        if isinstance(m, (tuple, list)) != eight or isinstance(v, (tuple, list)) != eight:
+            raise ValueError('moments of 8 and of 32 bits in one call')
+        if eight:
+            codes, blocks = quantized_size(numel)
+            _check_dense(m[0], p, codes, torch.int8, 'exp_avgs codes')
+            _check_dense(m[1], p, blocks, torch.float32, 'exp_avgs scales')
+            _check_dense(v[0], p, codes, torch.uint8, 'exp_avg_sqs codes')
+            _check_dense(v[1], p, blocks, torch.float32, 'exp_avg_sqs scales')
+            row = (p.data_ptr(), g.data_ptr(), m[0].data_ptr(), m[1].data_ptr(), v[0].data_ptr(), v[1].data_ptr(), numel)
+            if (row[2] | row[4]) & 7:
+                raise ValueError('codes must be 8-byte aligned')
+        else:
+            _check_dense(m, p, numel, torch.float32, 'exp_avgs')
+            _check_dense(v, p, numel, torch.float32, 'exp_avg_sqs')
+            row = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), numel)
+        if numel >= _MAX_LAUNCH:
+            raise ValueError('params of at most %d elements, got %d' % (_MAX_LAUNCH - 1, numel))
+        if numel:
+            if row[0] in seen:
+                raise ValueError('the same parameter twice')
+            seen.add(row[0])
+            groups.setdefault((device, dtype), []).append(row)
+    return groups
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence, exp_avg_sqs: Sequence, *, step: int,
@@ -69,52 +138,19 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if n == 0:
         return
     eight = isinstance(exp_avgs[0], (tuple, list))
-    # Addresses of every tensor, by (device, type): param, grad, exp_avg, exp_avg_sq (8 bits: and their scales), elements.
-    groups, seen = {}, set()
-    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
-        device, dtype, numel = p.get_device(), p.dtype, p.numel()
-        if device < 0:
-            require_device(p, 'params')
-        if dtype not in _DTYPES:
-            raise ValueError('params must be float32, bfloat16 or float16, got %s' % dtype)
-        if not p.is_contiguous():
-            raise ValueError('params must be dense, got strides %s' % (p.stride(),))
-        if g.dtype is not dtype or g.numel() != numel or g.get_device() != device or not g.is_contiguous():
-            _refuse(g, p, numel, dtype, 'grads')
-        if isinstance(m, (tuple, list)) != eight or isinstance(v, (tuple, list)) != eight:
-            raise ValueError('moments of 8 and of 32 bits in one call')
-        if eight:
-            codes, blocks = quantized_size(numel)
-            _check_dense(m[0], p, codes, torch.int8, 'exp_avgs codes')
-            _check_dense(m[1], p, blocks, torch.float32, 'exp_avgs scales')
-            _check_dense(v[0], p, codes, torch.uint8, 'exp_avg_sqs codes')
-            _check_dense(v[1], p, blocks, torch.float32, 'exp_avg_sqs scales')
-            row = (p.data_ptr(), g.data_ptr(), m[0].data_ptr(), m[1].data_ptr(), v[0].data_ptr(), v[1].data_ptr(), numel)
-            if (row[2] | row[4]) & 7:
-                raise ValueError('codes must be 8-byte aligned')
-        else:
-            _check_dense(m, p, numel, torch.float32, 'exp_avgs')
-            _check_dense(v, p, numel, torch.float32, 'exp_avg_sqs')
-            row = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), numel)
-        if numel >= _MAX_LAUNCH:
-            raise ValueError('params of at most %d elements, got %d' % (_MAX_LAUNCH - 1, numel))
-        if numel:
-            if row[0] in seen:
-                raise ValueError('the same parameter twice')
-            seen.add(row[0])
-            groups.setdefault((device, dtype), []).append(row)
+    groups = _uniform(params, grads, exp_avgs, exp_avg_sqs, eight) or _grouped(params, grads, exp_avgs, exp_avg_sqs, eight)
     cap = _MAX_TENSORS_8 if eight else _MAX_TENSORS
     lib = _lib.load()
     launch, name = (lib.tfr_adamw8, 'tfr_adamw8') if eight else (lib.tfr_adamw, 'tfr_adamw')
     for (device, dtype), rows in groups.items():
+        size_of = [row[-1] for row in rows]
         with _ops.device_of(device):
             tail = (lr, betas[0], betas[1], eps, weight_decay, step, None if now is None else now.data_ptr(), _raw_stream(device))
             at = 0
             while at < len(rows):
-                end, size = at, 0
-                while end < len(rows) and end - at < cap and size + rows[end][-1] < _MAX_LAUNCH:
-                    size += rows[end][-1]
-                    end += 1
+                end = min(at + cap, len(rows))
+                while sum(size_of[at:end]) >= _MAX_LAUNCH:
+                    end -= 1
                 columns = list(zip(*rows[at:end]))
                 addresses = ctypes.c_void_p * (end - at)
                 rc = launch(_DTYPES[dtype], end - at, *[addresses(*c) for c in columns[:-1]], (ctypes.c_int64 * (end - at))(*columns[-1]), *tail)
