@@ -633,7 +633,7 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   // least 16 occurrences.
   const long lanes = dim >= 256 ? 64 : 1l << log2_ceil((dim + 3) / 4);
   s.chunk_log2 = 4;
-  while (s.chunk_log2 < (n <= (1 << 20) ? 6 : 7) && (2l << s.chunk_log2) * 65536 <= n * lanes) ++s.chunk_log2;
+  while (s.chunk_log2 < (n <= (1 << 20) ? 6 : 7) && (2l << s.chunk_log2) * 131072 <= n * lanes) ++s.chunk_log2;
   long at = 0;
   auto take = [&at](long bytes) { const long p = at; at += (bytes + 255) / 256 * 256; return p; };
   s.keys = take(4 * n);

@@ -19,6 +19,7 @@ namespace {
 constexpr int MAX_ANSWERS = 64;                      // one lane an answer
 constexpr int LONG_PART = 8192, SHORT_PART = 2048;   // tokens of an answer that a workgroup sums
 constexpr int SMALL_LIST = 8192;                     // tokens of a list that one workgroup takes from its sums to its gradient
+constexpr int SHORT_LIST = 1024;                     // and a wavefront: 1087 lists of 672 tokens 20 us (39 by workgroups), 2000 of 1800 30 us (20)
 
 struct PrefArgs {
   const float* lp;
@@ -194,20 +195,31 @@ __global__ __launch_bounds__(64) void preference_pairs_kernel(const PrefArgs a, 
   if (lane < a.L) coef[(long)b * a.L + lane] = (float)c;
 }
 
-// The lists' losses added in fp64, in an order that depends on their number alone.
+// The lists' losses added in fp64, in an order that depends on their number alone; eight loads of a thread in flight (39 747 lists
+// took 37 us one by one).
+template <int THREADS>
 __device__ __forceinline__ void total_loss(const float* __restrict__ loss, int B, float* __restrict__ total) {
-  __shared__ double s_part[4];
+  __shared__ double s_part[THREADS / 64];
   double t = 0.0;
-  for (int b = threadIdx.x; b < B; b += 256) t += (double)loss[b];
+  for (int b0 = threadIdx.x; b0 < B; b0 += 8 * THREADS) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = b0 + k * THREADS < B ? loss[b0 + k * THREADS] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += (double)v[k];
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = t;
   __syncthreads();
-  if (threadIdx.x == 0) total[0] = (float)(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < THREADS / 64; ++w) t += s_part[w];
+    total[0] = (float)t;
+  }
 }
 
-__global__ __launch_bounds__(256) void preference_total_kernel(const float* __restrict__ loss, int B, float* __restrict__ total) {
-  total_loss(loss, B, total);
+__global__ __launch_bounds__(1024) void preference_total_kernel(const float* __restrict__ loss, int B, float* __restrict__ total) {
+  total_loss<1024>(loss, B, total);
 }
 
 // dlp[seq, t] = m * coef[seq] * upstream[list]; the last workgroup of the first part adds the lists' losses where a total is wanted.
@@ -217,7 +229,7 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const float* __res
                                                               float* __restrict__ total) {
   const long seq = blockIdx.x;
   if (seq == (long)B * L) {
-    if (blockIdx.y == 0) total_loss(loss, B, total);
+    if (blockIdx.y == 0) total_loss<256>(loss, B, total);
     return;
   }
   const int lo = blockIdx.y * part, hi = lo + part < T ? lo + part : T;
@@ -227,7 +239,7 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const float* __res
 }
 
 // Short lists, a wavefront each: an answer has 64 / `slots` lanes (slots: the power of two that holds the answers).  A workgroup a
-// list took 200 us for 39 747 lists of 4 answers of 3 tokens.
+// list took 160 us for 39 747 lists of 4 answers of 3 tokens, this 31.
 __global__ __launch_bounds__(256) void preference_wave_kernel(const PrefArgs a, int slots_log2, float* __restrict__ loss, float* __restrict__ out) {
   const long b = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (b >= a.B) return;
@@ -363,11 +375,11 @@ extern "C" int tfr_preference_loss_and_grad_f32(const float* log_probs, const fl
   if (B == 0 || (long)L * T <= SMALL_LIST) {
     int slots = 0;
     while ((1 << slots) < L) ++slots;
-    if (B > 0 && ((long)L * T <= 512 || (B >= 1024 && (long)L * T <= 2048)))
+    if (B > 0 && (long)L * T <= SHORT_LIST)
       preference_wave_kernel<<<(B + 3) / 4, 256, 0, st>>>(a, slots, w.loss, dlog_probs);
     else if (B > 0)
       preference_list_kernel<<<B, 256, 0, st>>>(a, w.loss, dlog_probs);
-    preference_total_kernel<<<1, 256, 0, st>>>(w.loss, B, total);
+    preference_total_kernel<<<1, 1024, 0, st>>>(w.loss, B, total);
   } else {
     preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
     preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, w.loss, w.coef);
