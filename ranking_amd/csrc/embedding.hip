@@ -658,7 +658,7 @@ int launch_lookup(const T* table, long ld, int rows, int dim, const Id* ids, lon
   const int groups = 256 >> lg;
   if (combiner == TFR_COMBINER_NONE) {
     const long steps = (packs + (1 << lg) - 1) >> lg, jobs = bags * steps;
-    if (jobs >= (1l << 26)) return TFR_EINVAL;                  // no grid of 2^32 threads
+    if ((jobs + groups - 1) / groups >= (1l << 24)) return TFR_EINVAL;    // no grid of 2^32 threads
     const bool stream_out = bags * dim * (long)sizeof(T) > (32l << 20);    // eight L2 caches of 4 MB
     const auto kernel = stream_out ? embedding_lookup_kernel<T, E, Id, true> : embedding_lookup_kernel<T, E, Id, false>;
     kernel<<<(unsigned)((jobs + groups - 1) / groups), 256, 0, stream>>>(table, ld, rows, dim, ids, (unsigned)jobs, (unsigned)steps, lg, scale, out);

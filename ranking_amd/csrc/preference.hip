@@ -151,7 +151,7 @@ __device__ __forceinline__ void list_pairs(const PrefArgs& a, int b, float y, do
     if (a.kind == TFR_PREFERENCE_LOGISTIC) {
       // softplus(+-h) = max(+-h, 0) + log(1 + e) and sigma(h) from one e = exp(-|h|): no overflow at any margin
       const double e = exp(-fabs(h)), q = 1.0 / (1.0 + e);
-      l = log1p(e) + (h < 0.0 ? -(1.0 - a.smoothing) * h : a.smoothing * h);
+      l = log1p(e) + (h < 0.0 ? -(1.0 - a.smoothing) * h : a.smoothing > 0.f ? a.smoothing * h : 0.0);   // h may be infinite
       d = (h < 0.0 ? e * q : q) - (1.0 - a.smoothing);
     } else if (a.kind == TFR_PREFERENCE_HINGE) {
       l = fmax(0.0, 1.0 - h);

@@ -79,8 +79,8 @@ def _lookup(table, ids, scale, combiner):
         pitch = dim
     with _ops.device_of(index):
         out = torch.empty(shape + (dim,), dtype=table.dtype, device=table.device)
-        rc = _lib.load().tfr_embedding_lookup(table.data_ptr(), pitch, rows, dim, code, ids.data_ptr(), id_type, bags, tokens, how, scale,
-                                              out.data_ptr(), _raw_stream(index))
+        rc = _lib.load().tfr_embedding_lookup(table.data_ptr(), pitch, rows, dim, code, ids.data_ptr(), id_type, bags, tokens, how,
+                                              float(scale), out.data_ptr(), _raw_stream(index))
     if rc:
         _lib.check(rc, 'tfr_embedding_lookup')
     return out
@@ -105,7 +105,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: int, s
         out = torch.empty((rows, dim), dtype=grad.dtype, device=grad.device)
         nbytes = lib.tfr_embedding_grad_workspace_bytes(rows, dim, bags, tokens, how)
         workspace = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=grad.device)
-        rc = lib.tfr_embedding_grad(grad.data_ptr(), code, ids.data_ptr(), id_type, bags, tokens, how, scale, rows, dim, out.data_ptr(),
+        rc = lib.tfr_embedding_grad(grad.data_ptr(), code, ids.data_ptr(), id_type, bags, tokens, how, float(scale), rows, dim, out.data_ptr(),
                                     workspace.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         _lib.check(rc, 'tfr_embedding_grad')

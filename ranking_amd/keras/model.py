@@ -38,7 +38,9 @@ class DNNScorer(UnivariateScorer):
 
     def __init__(self, input_dim: int, embeddings: Optional[Dict[str, nn.Module]] = None, **dnn_kwargs):
         super().__init__()
-        self._embeddings = nn.ModuleDict(embeddings or {})
+        # (names of features are no names of modules: a ModuleDict takes neither 'a.b' nor 'keys')
+        self._embeddings = dict(embeddings or {})
+        self._embedding_tables = nn.ModuleList(self._embeddings[k] for k in sorted(self._embeddings))
         self._dnn_kwargs = dict(dnn_kwargs)
         self._dnn_kwargs.setdefault('output_units', 1)
         self._tower = layers.create_tower(input_dim=input_dim, **self._dnn_kwargs)

@@ -137,6 +137,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError('step counts from 1, got %r' % (step,))
     if n == 0:
         return
+    if now is not None:
+        _check_dense(now, params[0], 3, torch.float32, 'now')
+        if any(p.get_device() != now.get_device() for p in params):
+            raise ValueError('now is on %s: a step that is counted on a device takes the parameters of that device' % (now.device,))
     eight = isinstance(exp_avgs[0], (tuple, list))
     groups = _uniform(params, grads, exp_avgs, exp_avg_sqs, eight) or _grouped(params, grads, exp_avgs, exp_avg_sqs, eight)
     cap = _MAX_TENSORS_8 if eight else _MAX_TENSORS
@@ -194,13 +198,21 @@ class AdamW(torch.optim.Optimizer):
     ``init_state()``); a capture needs it to be there."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
-        _check_hyper(lr, betas, eps, weight_decay)
-        if state_bits not in (8, 32):
-            raise ValueError('state_bits must be 8 or 32, got {}'.format(state_bits))
-        if torch.is_tensor(lr) and not capturable:
-            raise ValueError('lr as a tensor needs capturable=True')
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       capturable=capturable))
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            _check_hyper(g['lr'], g['betas'], g['eps'], g['weight_decay'])
+            if g['state_bits'] not in (8, 32):
+                raise ValueError('state_bits must be 8 or 32, got {}'.format(g['state_bits']))
+            if torch.is_tensor(g['lr']) and not g['capturable']:
+                raise ValueError('lr as a tensor needs capturable=True')
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     def _state_of(self, p, group):
         s = self.state[p]

@@ -348,6 +348,10 @@ def test_refusals():
                 lambda: step(p, z(), (z(4, torch.int8), z(1)), eight[1]), lambda: step(p, z(), z(), z(), lr=torch.tensor(1.0, device=DEV)),
                 lambda: step(p, z(), (z(136, torch.int8)[4:132], z(1)), eight[1]),
                 lambda: O().adamw_step([p, p], [z(), z()], [z(), z()], [z(), z()], step=1, lr=1e-3),
+                lambda: step(p, z(), z(), z(), now=z(2)), lambda: step(p, z(), z(), z(), now=z(3, torch.float64)),
+                lambda: step(p, z(), z(), z(), now=torch.zeros(3)),
+                lambda: O().AdamW([dict(params=[torch.nn.Parameter(z())], state_bits=16)]),
+                lambda: O().AdamW([torch.nn.Parameter(z())]).add_param_group(dict(params=[torch.nn.Parameter(z())], lr=-1.0)),
                 lambda: O().dequantize_exp_avg(z(130, torch.int8), z(2)), lambda: O().dequantize_exp_avg(z(128, torch.uint8), z(1)),
                 lambda: O().dequantize_exp_avg_sq(z(128, torch.uint8), z(2))):
         with pytest.raises(ValueError):

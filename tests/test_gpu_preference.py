@@ -123,6 +123,35 @@ def test_large_margins_and_infinities():
     assert total == float('inf') and grad[1, 0, 0] == -0.5
 
 
+def test_an_answer_of_probability_zero():
+    """-inf on either side of a pair: the loss is infinite where the better answer is impossible, and 0 where the worse one is."""
+    y = torch.tensor([[1.0, 0.0], [1.0, 0.0], [1.0, 0.0]])
+    lp = torch.tensor([[[-1.0], [-float('inf')]], [[-float('inf')], [-1.0]], [[-float('inf')], [-float('inf')]]])
+    loss = K().PreferenceLoss(reduction='none', beta=1.0)(y.to(DEV), lp.to(DEV))
+    assert loss[0] == 0 and loss[1] == float('inf') and loss[2].isnan()
+    _, grad = K().PreferenceLoss(reduction='sum', beta=1.0).loss_and_grad(y.to(DEV), lp.to(DEV))
+    assert not grad[0].any() and grad[1].flatten().tolist() == [-1.0, 1.0]
+
+
+@pytest.mark.parametrize('B,L,tokens', [(3, 2, 33), (2, 4, 700), (2, 2, 9001)])
+def test_shifted_tensors(B, L, tokens):
+    """Dense tensors that start anywhere: single tokens an access instead of four, the same sums and gradients."""
+    y, lp, ref, mask, w = make(B, L, tokens)
+    y[:, 0], y[:, 1] = 2.0, 1.0
+    want = K().PreferenceLoss().loss_and_grad(y.to(DEV), lp.to(DEV), w.to(DEV), reference=ref.to(DEV), mask=mask.to(DEV))
+
+    def shifted(t):
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device=DEV)
+        flat[1:] = t.flatten().to(DEV)
+        return flat[1:].view(t.shape)
+    for move in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1)):
+        a, b, c = (shifted(t) if m else t.to(DEV) for t, m in zip((lp, ref, mask), move))
+        got = K().PreferenceLoss().loss_and_grad(y.to(DEV), a, w.to(DEV), reference=b, mask=c)
+        # fp64 sums in another order: the same after rounding but for the last bit
+        T.assert_within(got[0], want[0].double(), 2 * T.U * want[0].double().abs() + 1e-12)
+        T.assert_within(got[1], want[1].double(), 2 * T.U * want[1].double().abs() + 1e-12)
+
+
 def test_strides_types_and_empty_batch():
     y, lp, ref, mask, w = make(6, 4, 30)
     want = K().PreferenceLoss().loss_and_grad(y[::2, :3].contiguous().to(DEV), lp[::2, :3, 5:].contiguous().to(DEV),

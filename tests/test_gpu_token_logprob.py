@@ -37,7 +37,7 @@ def check(logits, targets, temperature=1.0, upstream=None):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('n,vocab', [(1, 1), (3, 2), (5, 7), (4, 64), (9, 200), (2, 2048), (3, 2049), (2, 5003), (1, 40000), (2, 100003), (700, 2100)])
+@pytest.mark.parametrize('n,vocab', [(1, 1), (3, 2), (5, 7), (4, 64), (9, 200), (2, 2048), (3, 2049), (2, 5003), (1, 40000), (2, 100003), (700, 2100), (1000, 6), (333, 70), (77, 300)])
 def test_sizes(dtype, n, vocab):
     g = torch.Generator().manual_seed(vocab)
     logits = (torch.randn(n, vocab, generator=g) * 4).to(dtype).to(DEV)
