@@ -78,7 +78,7 @@ def _lookup(table, ids, scale, combiner):
         table = table.contiguous()
         pitch = dim
     with _ops.device_of(index):
-        out = torch.empty(shape + (dim,), dtype=table.dtype, device=table.device)
+        out = table.new_empty(shape + (dim,))
         rc = _lib.load().tfr_embedding_lookup(table.data_ptr(), pitch, rows, dim, code, ids.data_ptr(), id_type, bags, tokens, how,
                                               float(scale), out.data_ptr(), _raw_stream(index))
     if rc:
@@ -102,9 +102,9 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: int, s
     grad = grad.contiguous()
     lib = _lib.load()
     with _ops.device_of(index):
-        out = torch.empty((rows, dim), dtype=grad.dtype, device=grad.device)
+        out = grad.new_empty((rows, dim))
         nbytes = lib.tfr_embedding_grad_workspace_bytes(rows, dim, bags, tokens, how)
-        workspace = torch.empty((max(nbytes, 0),), dtype=torch.uint8, device=grad.device)
+        workspace = grad.new_empty((max(nbytes, 0),), dtype=torch.uint8)
         rc = lib.tfr_embedding_grad(grad.data_ptr(), code, ids.data_ptr(), id_type, bags, tokens, how, float(scale), rows, dim, out.data_ptr(),
                                     workspace.data_ptr(), nbytes, _raw_stream(index))
     if rc:

@@ -814,10 +814,14 @@ class PreferenceLoss(_RankingLoss):
         shape = tuple(y_pred.shape)
         if len(shape) not in (2, 3):
             raise ValueError('y_pred must be [batch, answers] or [batch, answers, tokens], got shape %s' % (shape,))
-        y_pred = y_pred.to(torch.float32).contiguous()
+
+        def dense(t):                                         # float32, no part of a graph
+            t = t.detach() if t.requires_grad else t
+            return (t if t.dtype is torch.float32 else t.to(torch.float32)).contiguous()
+        y_pred = (y_pred if y_pred.dtype is torch.float32 else y_pred.to(torch.float32)).contiguous()
         if not torch.is_tensor(y_true) or y_true.device != y_pred.device:
             y_true = torch.as_tensor(y_true, device=y_pred.device)
-        y_true = y_true.detach().to(torch.float32).contiguous()
+        y_true = dense(y_true)
         if tuple(y_true.shape) != shape[:2]:
             raise ValueError('y_true of shape %s does not fit y_pred of shape %s' % (tuple(y_true.shape), shape))
         if not 1 <= shape[1] <= _preference.MAX_ANSWERS:
@@ -827,7 +831,7 @@ class PreferenceLoss(_RankingLoss):
                 raise ValueError('%s of shape %s on %s does not fit y_pred of shape %s on %s'
                                  % (name, tuple(t.shape), t.device, shape, y_pred.device))
         if reference is not None:
-            reference = reference.detach().to(torch.float32).contiguous()
+            reference = dense(reference)
         if mask is not None:                                  # a byte a token: 0 or not
             mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).contiguous()
         scale = 1.0 if self.reduction in (Reduction.SUM, Reduction.NONE) else 1.0 / max(1, shape[0])
@@ -835,7 +839,9 @@ class PreferenceLoss(_RankingLoss):
             if not torch.is_tensor(sample_weight) and not hasattr(sample_weight, '__len__'):
                 scale, sample_weight = scale * float(sample_weight), None
             else:
-                sample_weight = torch.as_tensor(sample_weight, dtype=torch.float32, device=y_pred.device).detach()
+                if not torch.is_tensor(sample_weight) or sample_weight.device != y_pred.device:
+                    sample_weight = torch.as_tensor(sample_weight, device=y_pred.device)
+                sample_weight = dense(sample_weight)
                 if sample_weight.dim() == 0:
                     sample_weight = sample_weight.expand(shape[0])
                 if tuple(sample_weight.shape) not in ((shape[0],), (shape[0], 1)):

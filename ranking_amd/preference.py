@@ -40,7 +40,9 @@ def _rows(logits: torch.Tensor, targets: torch.Tensor):
         per, stride_b, stride_t = 1, 0, 0
     else:
         per, stride_b, stride_t = max(1, shape[1]), logits.stride(0), logits.stride(1)
-    return logits, n, vocab, per, stride_b, stride_t, targets.to(torch.int64).contiguous()
+    if targets.dtype is not torch.int64:
+        targets = targets.to(torch.int64)
+    return logits, n, vocab, per, stride_b, stride_t, targets.contiguous()
 
 
 def _temperature(t) -> float:
@@ -55,10 +57,10 @@ def _log_probs(logits, targets, temperature, want_stats):
     logits, n, vocab, per, stride_b, stride_t, targets = _rows(logits, targets)
     lib = _lib.load()
     with _ops.device_of(index):
-        logp = torch.empty(targets.shape, dtype=torch.float32, device=logits.device)
-        stats = torch.empty(targets.shape + (2,), dtype=torch.float32, device=logits.device) if want_stats else None
+        logp = torch.empty_like(targets, dtype=torch.float32)
+        stats = targets.new_empty(targets.shape + (2,), dtype=torch.float32) if want_stats else None
         nbytes = lib.tfr_token_logprob_workspace_bytes(n, vocab)
-        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=logits.device) if nbytes > 0 else None
+        workspace = targets.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
         rc = lib.tfr_token_logprob(logits.data_ptr(), code, per, stride_b, stride_t, targets.data_ptr(), n, vocab, _temperature(temperature),
                                    logp.data_ptr(), stats.data_ptr() if want_stats else None, workspace.data_ptr() if nbytes > 0 else None, nbytes,
                                    _raw_stream(index))
@@ -69,7 +71,7 @@ def _log_probs(logits, targets, temperature, want_stats):
 
 def token_log_probs_with_stats(logits: torch.Tensor, targets: torch.Tensor, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """``token_log_probs`` without autograd, and the row statistics ``[..., 2]`` that ``token_log_probs_grad`` takes."""
-    return _log_probs(logits.detach(), targets, temperature, True)
+    return _log_probs(logits.detach() if torch.is_tensor(logits) else logits, targets, temperature, True)
 
 
 def token_log_probs_grad(grad: torch.Tensor, logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor,
@@ -82,9 +84,11 @@ def token_log_probs_grad(grad: torch.Tensor, logits: torch.Tensor, targets: torc
     if grad.shape != shape[:-1] or stats.shape != shape[:-1] + (2,) or stats.dtype is not torch.float32:
         raise ValueError('grad of shape %s and stats of shape %s do not fit logits of shape %s'
                          % (tuple(grad.shape), tuple(stats.shape), tuple(shape)))
-    grad, stats = grad.to(torch.float32).contiguous(), stats.contiguous()
+    if grad.dtype is not torch.float32:
+        grad = grad.to(torch.float32)
+    grad, stats = grad.contiguous(), stats.contiguous()
     with _ops.device_of(index):
-        out = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(shape)
         rc = _lib.load().tfr_token_logprob_grad(logits.data_ptr(), code, per, stride_b, stride_t, targets.data_ptr(), stats.data_ptr(),
                                                 grad.data_ptr(), n, vocab, _temperature(temperature), out.data_ptr(), _raw_stream(index))
     if rc:
@@ -127,7 +131,7 @@ def _loss_args(log_probs, labels, reference, mask, list_weights, kind, beta, lab
     if nbytes < 0:
         raise ValueError('log_probs of shape %s: at most %d answers a list, 2^24 - 2 answers and 2^28 tokens an answer'
                          % (tuple(log_probs.shape), MAX_ANSWERS))
-    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=log_probs.device)
+    workspace = log_probs.new_empty((nbytes,), dtype=torch.uint8)
     return B, L, T, workspace, nbytes, (log_probs.data_ptr(), _address(reference), _address(mask), labels.data_ptr(), _address(list_weights),
                                         B, L, T, KINDS[kind], beta, label_smoothing, int(length_normalized), scale)
 
@@ -160,8 +164,8 @@ def preference_loss_and_grad(log_probs: torch.Tensor, labels: torch.Tensor, refe
     with _ops.device_of(index):
         B, L, T, workspace, nbytes, args = _loss_args(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing,
                                                       length_normalized, scale)
-        total = torch.empty((), dtype=torch.float32, device=log_probs.device)
-        grad = torch.empty((B, L, T), dtype=torch.float32, device=log_probs.device)
+        total = log_probs.new_empty(())
+        grad = torch.empty_like(log_probs)
         rc = _lib.load().tfr_preference_loss_and_grad_f32(*args, total.data_ptr(), grad.data_ptr(), workspace.data_ptr(), nbytes,
                                                           _raw_stream(index))
     if rc:
