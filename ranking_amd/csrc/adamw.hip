@@ -3,7 +3,8 @@
 //   m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2
 //   p <- p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// HBM-bound: with fp32 parameters and moments 16 bytes are read and 12 written an element.  The addresses and lengths of up to
+// HBM-bound: with fp32 parameters and moments 16 bytes are read and 12 written an element (152 M elements in 98 tensors: 830 us =
+// 5.1 TB/s; the 14 tensors of a 136-512-512-512-1 tower: 7 us).  The addresses and lengths of up to
 // TFR_ADAMW_MAX_TENSORS (TFR_ADAMW8_MAX_TENSORS) tensors travel in the kernel's arguments: no table in device memory that a
 // step would have to copy first (the gradients' addresses change from step to step), and a captured launch holds its own.
 //

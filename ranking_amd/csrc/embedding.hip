@@ -13,6 +13,8 @@
 //      that lies inside its chunk is a finished row of dW; the part of a run that crosses a chunk's border is left as a partial
 //      sum.  The work is cut by occurrences and not by rows, so a token that is 6 % of the batch costs what the others cost.
 //   3. Runs that cross borders are joined from their partial sums, and rows without an occurrence are filled with zeros.
+// Steps 2 and 3 are bound by HBM: 262 144 x 2048 bf16 into 131 072 rows 259 + 74 us (1.07 GB read, 0.54 GB written: 4.8 TB/s),
+// 16 384 x 1024 into 65 536 rows 15 + 18 us; the lookups before them 328 and 11 us.
 #include "common.h"
 #include "elem.h"
 
@@ -246,9 +248,10 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __
 
 // The large sort.  One pass = the digit counts of every tile (a workgroup's `subs` * blockDim.x * ITEMS consecutive items), then
 // the scatter, in which a tile adds up the counts of the tiles before it by itself (counts[bin][tile], `pitch` apart) while
-// there are few tiles.  The last
-// pass turns positions into bags (per_bag > 1).  FIRST: the keys are the ids themselves, the
+// there are few tiles.  The last pass turns positions into bags (per_bag > 1).  FIRST: the keys are the ids themselves, the
 // positions their indexes, and the workgroups behind the tiles prepare the rows.
+// Bound by latency (a pass is two or three launches of a few dependent round trips): two passes take 24 us at 16 384 lookups, 37 at
+// 262 144, 45 at 819 200.
 template <typename Id, bool FIRST>
 __global__ __launch_bounds__(256) void embedding_digits_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, int n, int rows, int tiles,
                                                                 int subs, int shift, int bits, int pitch, const Prepare prep, int* __restrict__ counts) {

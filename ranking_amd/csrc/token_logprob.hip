@@ -6,6 +6,10 @@
 // (max x, sum exp((x - max) / T)) of every row kept for the backward, which is one read and one write of the row:
 // p = exp((x - max) / T) / sum.  A row with target < 0 is no target: log probability 0, gradient 0, its logits are not read.
 // A target beyond the row: NaN in both.
+// Bound by HBM (8192 x 50 021 bf16, a tenth without a target: 177 us forward = 4.2 TB/s, 312 us backward = 5.0 TB/s; a copy
+// reaches 4.9).  A row is read by 16-byte accesses between its first and last 16-byte boundary: rows of an odd length start
+// anywhere.  Few long rows are split over workgroups and joined by a second launch (2 x 131 072: 5 us), short ones share a
+// wavefront (16 384 x 200 fp32: 11 us with the gradient, 17 with a wavefront a row).
 #include "common.h"
 #include "elem.h"
 

@@ -80,6 +80,15 @@ def test_gradient_sort_sizes(n, rows):
     assert torch.equal(first, E().embedding_grad(up, ids, rows))            # the same bits again
 
 
+@pytest.mark.parametrize('n,rows', [(32768, 700), (32769, 700), (40001, 70001), (1300001, 5003)])
+def test_gradient_of_many_tiles(n, rows):
+    """As many tiles as add each other's counts up, one more, and tiles of several parts; bags of three."""
+    ids = make_ids((n,), rows, n, torch.int32, common=0.05).to(DEV)
+    up = torch.randn(n, 4, generator=torch.Generator().manual_seed(n)).to(DEV)
+    check_grad(up, ids, rows, 1.0, None)
+    check_grad(up[:n // 3], ids[:n // 3 * 3].view(-1, 3), rows, 0.5, 'mean')
+
+
 def test_gradient_table_with_three_digit_ids():
     rows, n = (1 << 20) + 5, 20000
     ids = make_ids((n,), rows, 3, common=0.1).to(DEV)
