@@ -23,7 +23,7 @@ using namespace tfr;
 namespace {
 
 constexpr int LONG_RUN = 16;            // partial sums from which the whole workgroup joins a run
-constexpr int SMALL_SORT = 4096;        // lookups that one workgroup sorts in LDS
+constexpr int SMALL_SORT = 4096;        // lookups that one workgroup sorts in LDS (9 us; 16 384 of them: 33 us, by the large sort 25)
 constexpr int ITEMS = 4;                // items a thread of the large sort holds
 
 template <typename Id>
