@@ -650,7 +650,7 @@ int tfr_token_logprob_grad(const void* logits, int dtype, long per, long stride_
  *   TFR_PREFERENCE_SQUARED  (s_i - s_j - 1/2)^2
  * times scale and the list's weight.  Sums are fp64.  reference, mask (uint8 [B, L, T]), list_weights ([B]) are nullable.
  *   loss [B];  coef [B, L] = d loss[b] / d (any unmasked log prob of the answer); the gradient spreads it over the tokens,
- *   times upstream[b] (nullable).  B * L below 2^24 - 1, T at most 2^28; workspace: 8-byte aligned. */
+ *   times upstream[b] (nullable).  B * L below 2^24 - 1, T at most 2^28; workspace: 16-byte aligned. */
 #define TFR_PREFERENCE_LOGISTIC 0
 #define TFR_PREFERENCE_HINGE 1
 #define TFR_PREFERENCE_SQUARED 2

@@ -20,7 +20,7 @@ namespace {
 constexpr int MAX_ANSWERS = 64;                      // one lane an answer
 constexpr int LONG_PART = 8192, SHORT_PART = 2048;   // tokens of an answer that a workgroup sums
 constexpr int SMALL_LIST = 8192;                     // tokens of a list that one workgroup takes from its sums to its gradient
-constexpr int SHORT_LIST = 1024;                     // and a wavefront: 1087 lists of 672 tokens 20 us (39 by workgroups), 2000 of 1800 30 us (20)
+constexpr int SHORT_LIST = 1024;                     // and a wavefront or a part of one: 1087 lists of 672 tokens 20 us (39 by workgroups), 2000 of 1800 30 us (20)
 
 struct PrefArgs {
   const float* lp;
@@ -134,17 +134,18 @@ __global__ __launch_bounds__(256) void preference_sum_kernel(const PrefArgs a, d
   }
 }
 
-// One wavefront, lane i = answer i with its grade y (-1 behind the last), its sum and number of tokens: the list's loss (all
-// lanes) and this lane's d loss / d sum_t lp_it.
-__device__ __forceinline__ void list_pairs(const PrefArgs& a, int b, float y, double sum, int n, double* loss_out, double* coef_out) {
+// `lanes` neighbouring lanes (a power of two, at least L), lane i of them = answer i with its grade y (-1 behind the last), its sum and
+// number of tokens: the list's loss (all lanes) and this lane's d loss / d sum_t lp_it.
+__device__ __forceinline__ void list_pairs(const PrefArgs& a, long b, float y, double sum, int n, int lanes, double* loss_out, double* coef_out) {
+  const int base = (threadIdx.x & 63) & ~(lanes - 1);
   const double f = (double)a.beta / (a.normalize ? (double)(n > 0 ? n : 1) : 1.0);
   const double s = f * sum;
   const double w = (a.weights ? (double)a.weights[b] : 1.0) * (double)a.scale;
   double loss = 0.0, slope = 0.0;
   int pairs = 0;
   for (int j = 0; j < a.L; ++j) {
-    const double sj = __shfl(s, j, 64);
-    const float yj = __shfl(y, j, 64);
+    const double sj = __shfl(s, base + j, 64);
+    const float yj = __shfl(y, base + j, 64);
     const bool win = y > yj && yj >= 0.f, lose = yj > y && y >= 0.f;
     if (!win && !lose) continue;
     const double h = win ? s - sj : sj - s;
@@ -167,8 +168,7 @@ __device__ __forceinline__ void list_pairs(const PrefArgs& a, int b, float y, do
     }
     slope += win ? d : -d;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
     loss += __shfl_xor(loss, o, 64);
     pairs += __shfl_xor(pairs, o, 64);
   }
@@ -191,24 +191,26 @@ __global__ __launch_bounds__(64) void preference_pairs_kernel(const PrefArgs a, 
       n += part_n[seq * a.parts + p];
     }
   }
-  list_pairs(a, b, y, sum, n, &l, &c);
+  list_pairs(a, b, y, sum, n, 64, &l, &c);
   if (lane == 0) loss[b] = (float)l;
   if (lane < a.L) coef[(long)b * a.L + lane] = (float)c;
 }
 
-// The lists' losses added in fp64, in an order that depends on their number alone; eight loads of a thread in flight (39 747 lists
-// took 37 us one by one).
+// The lists' losses (16-byte aligned) added in fp64, in an order that depends on their number alone; 32 values of a thread in flight
+// (39 747 lists took 37 us one by one).
 template <int THREADS>
 __device__ __forceinline__ void total_loss(const float* __restrict__ loss, int B, float* __restrict__ total) {
   __shared__ double s_part[THREADS / 64];
   double t = 0.0;
-  for (int b0 = threadIdx.x; b0 < B; b0 += 8 * THREADS) {
-    float v[8];
+  const float4* packs = reinterpret_cast<const float4*>(loss);
+  for (int p0 = threadIdx.x; p0 < B / 4; p0 += 8 * THREADS) {
+    float4 v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = b0 + k * THREADS < B ? loss[b0 + k * THREADS] : 0.f;
+    for (int k = 0; k < 8; ++k) v[k] = p0 + k * THREADS < B / 4 ? packs[p0 + k * THREADS] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += (double)v[k];
+    for (int k = 0; k < 8; ++k) t += ((double)v[k].x + (double)v[k].y) + ((double)v[k].z + (double)v[k].w);
   }
+  if ((int)threadIdx.x < (B & 3)) t += (double)loss[(B & ~3) + threadIdx.x];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
   if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = t;
@@ -239,16 +241,19 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const float* __res
   token_fill<256>(mask, wide, seq, T, lo, hi, threadIdx.x, c, out);
 }
 
-// Short lists, a wavefront each: an answer has 64 / `slots` lanes (slots: the power of two that holds the answers).  A workgroup a
-// list took 160 us for 39 747 lists of 4 answers of 3 tokens, this 31.
-__global__ __launch_bounds__(256) void preference_wave_kernel(const PrefArgs a, int slots_log2, float* __restrict__ loss, float* __restrict__ out) {
-  const long b = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (b >= a.B) return;
-  const int lane = threadIdx.x & 63, width_log2 = 6 - slots_log2, width = 1 << width_log2;
-  const int answer = lane >> width_log2, first = lane & (width - 1);
+// Short lists, `lanes` (a power of two) lanes each, of which an answer has lanes / slots (slots: the power of two that holds the
+// answers).  Either the gradient is written (out) or the answers' coefficients (coef).  39 747 lists of 4 answers of 3 tokens: 160 us by
+// a workgroup a list, 31 by a wavefront, 6 by 8 lanes.
+__global__ __launch_bounds__(256) void preference_wave_kernel(const PrefArgs a, int lanes_log2, int slots_log2, float* __restrict__ loss,
+                                                              float* __restrict__ out, float* __restrict__ coef) {
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & 63, base = lane & ~(lanes - 1), li = lane & (lanes - 1);
+  const long b = ((long)blockIdx.x * 256 + threadIdx.x) >> lanes_log2;
+  const int width_log2 = lanes_log2 - slots_log2, width = 1 << width_log2;
+  const int answer = li >> width_log2, first = li & (width - 1);
+  const bool list = b < a.B, mine = list && answer < a.L;      // the lanes behind the last list stay: others read them
   const long seq = b * a.L + answer;
   Sum v = {0.0, 0};
-  if (answer < a.L && a.labels[seq] >= 0.f) {
+  if (mine && a.labels[seq] >= 0.f) {
     for (long t = seq * a.T + first; t < (seq + 1) * a.T; t += width)
       add_token(v, a.lp[t], a.ref ? a.ref[t] : 0.f, a.mask ? a.mask[t] != 0 : true);
   }
@@ -256,16 +261,32 @@ __global__ __launch_bounds__(256) void preference_wave_kernel(const PrefArgs a, 
     v.s += __shfl_xor(v.s, o, 64);
     v.n += __shfl_xor(v.n, o, 64);
   }
-  const int from = (lane << width_log2) & 63;                  // lane i takes answer i's sum
+  const int from = base + ((li << width_log2) & (lanes - 1));  // lane i of the list takes answer i's sum
   const double sum = __shfl(v.s, from, 64);
   const int n = __shfl(v.n, from, 64);
   double l, c;
-  list_pairs(a, (int)b, lane < a.L ? a.labels[b * a.L + lane] : -1.f, sum, n, &l, &c);
-  if (lane == 0) loss[b] = (float)l;
-  const float mine = __shfl((float)c, answer, 64);
-  if (answer < a.L) {
-    for (long t = seq * a.T + first; t < (seq + 1) * a.T; t += width) out[t] = (a.mask ? a.mask[t] != 0 : true) ? mine : 0.f;
+  list_pairs(a, list ? b : 0, list && li < a.L ? a.labels[b * a.L + li] : -1.f, sum, n, lanes, &l, &c);
+  if (list && li == 0) loss[b] = (float)l;
+  if (coef) {
+    if (list && li < a.L) coef[b * a.L + li] = (float)c;
+    return;
   }
+  const float by = __shfl((float)c, base + answer, 64);
+  if (mine) {
+    for (long t = seq * a.T + first; t < (seq + 1) * a.T; t += width) out[t] = (a.mask ? a.mask[t] != 0 : true) ? by : 0.f;
+  }
+}
+
+// The gradient of short answers from their coefficients: a thread a token.
+__global__ __launch_bounds__(256) void preference_grad_short_kernel(const float* __restrict__ coef, const float* __restrict__ upstream,
+                                                                    const uint8_t* __restrict__ mask, unsigned L, unsigned T, unsigned n,
+                                                                    float* __restrict__ out) {
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= n) return;
+  const unsigned seq = i / T;
+  float c = coef[seq];
+  if (upstream) c *= upstream[seq / L];
+  out[i] = (mask ? mask[i] != 0 : true) ? c : 0.f;
 }
 
 // A list from its sums to its gradient by one workgroup: an answer a wave and step.
@@ -284,7 +305,7 @@ __global__ __launch_bounds__(256) void preference_list_kernel(const PrefArgs a, 
   if (wave == 0) {
     const bool here = lane < a.L;
     double l, c;
-    list_pairs(a, b, here ? a.labels[(long)b * a.L + lane] : -1.f, here ? s_sum[lane].s : 0.0, here ? s_sum[lane].n : 0, &l, &c);
+    list_pairs(a, b, here ? a.labels[(long)b * a.L + lane] : -1.f, here ? s_sum[lane].s : 0.0, here ? s_sum[lane].n : 0, 64, &l, &c);
     if (lane == 0) loss[b] = (float)l;
     if (here) s_coef[lane] = (float)c;
   }
@@ -301,21 +322,31 @@ int part_of(int B, int L, int T) { return (long)B * L * T >= (1l << 23) ? LONG_P
 int parts_of(int B, int L, int T) { return T > 0 ? (T + part_of(B, L, T) - 1) / part_of(B, L, T) : 1; }
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }       // null too
 
-struct Workspace {                                   // sums [B * L * parts], numbers, coefficients [B * L], losses [B]
+struct Workspace {                                   // losses [B, padded to 4], coefficients [B * L, padded], sums [B * L * parts], numbers
+  float* loss;
+  float* coef;
   double* sum;
   int* n;
-  float* coef;
-  float* loss;
 };
-long workspace_bytes_of(int B, int L, int T) { return (long)B * L * parts_of(B, L, T) * 12 + (long)B * L * 4 + (long)B * 4; }
+long padded(long n) { return (n + 3) & ~3l; }
+long workspace_bytes_of(int B, int L, int T) {
+  return padded(B) * 4 + padded((long)B * L) * 4 + (long)B * L * parts_of(B, L, T) * 12;
+}
 Workspace workspace_at(void* p, int B, int L, int T) {
-  const long n = (long)B * L * parts_of(B, L, T);
   Workspace w;
-  w.sum = (double*)p;
-  w.n = (int*)(w.sum + n);
-  w.coef = (float*)(w.n + n);
-  w.loss = w.coef + (long)B * L;
+  w.loss = (float*)p;
+  w.coef = w.loss + padded(B);
+  w.sum = (double*)(w.coef + padded((long)B * L));
+  w.n = (int*)(w.sum + (long)B * L * parts_of(B, L, T));
   return w;
+}
+
+// Short lists (L * T <= SHORT_LIST): a wavefront a list, fewer lanes where there are lists enough to fill the card so.
+void launch_short(const PrefArgs& a, float* loss, float* out, float* coef, hipStream_t st) {
+  int slots = 0, lanes = 6;
+  while ((1 << slots) < a.L) ++slots;
+  while (lanes > slots && (4l << lanes) >= (long)a.L * a.T && ((long)a.B << lanes) > 64 * 4096) --lanes;
+  preference_wave_kernel<<<(unsigned)((((long)a.B << lanes) + 255) / 256), 256, 0, st>>>(a, lanes, slots, loss, out, coef);
 }
 
 int make_args(PrefArgs* a, const float* log_probs, const float* reference, const uint8_t* mask, const float* labels, const float* list_weights,
@@ -343,11 +374,15 @@ extern "C" int tfr_preference_loss_f32(const float* log_probs, const float* refe
   const int rc = make_args(&a, log_probs, reference, mask, labels, list_weights, B, L, T, kind, beta, smoothing, normalize, scale);
   if (rc != TFR_OK) return rc;
   if (B == 0) return TFR_OK;
-  if (!loss || !coef || !workspace || workspace_bytes < workspace_bytes_of(B, L, T) || !aligned(workspace, 8)) return TFR_EINVAL;
+  if (!loss || !coef || !workspace || workspace_bytes < workspace_bytes_of(B, L, T) || !aligned(workspace, 16)) return TFR_EINVAL;
   const Workspace w = workspace_at(workspace, B, L, T);
   hipStream_t st = (hipStream_t)stream;
-  preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
-  preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, loss, coef);
+  if ((long)L * T <= SHORT_LIST) {
+    launch_short(a, loss, nullptr, coef, st);
+  } else {
+    preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
+    preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, loss, coef);
+  }
   return (int)hipGetLastError();
 }
 
@@ -356,6 +391,11 @@ extern "C" int tfr_preference_grad_f32(const float* coef, const float* upstream,
   if (bad_sizes(B, L, T)) return TFR_EINVAL;
   if (B == 0 || T == 0) return TFR_OK;
   if (!coef || !dlog_probs) return TFR_EINVAL;
+  const long n = (long)B * L * T;
+  if (T <= 128 && n < (1l << 31)) {                  // a workgroup an answer would leave most of its threads without a token
+    preference_grad_short_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (hipStream_t)stream>>>(coef, upstream, mask, L, T, (unsigned)n, dlog_probs);
+    return (int)hipGetLastError();
+  }
   preference_grad_kernel<<<dim3((unsigned)(B * L), parts_of(B, L, T)), 256, 0, (hipStream_t)stream>>>(
       coef, upstream, mask, L, T, part_of(B, L, T), aligned(dlog_probs, 16) && aligned(mask, 4), dlog_probs, nullptr, B, nullptr);
   return (int)hipGetLastError();
@@ -369,17 +409,13 @@ extern "C" int tfr_preference_loss_and_grad_f32(const float* log_probs, const fl
   const int rc = make_args(&a, log_probs, reference, mask, labels, list_weights, B, L, T, kind, beta, smoothing, normalize, scale);
   if (rc != TFR_OK) return rc;
   if (!total || (B > 0 && T > 0 && !dlog_probs)) return TFR_EINVAL;
-  if (B > 0 && (!workspace || workspace_bytes < workspace_bytes_of(B, L, T) || !aligned(workspace, 8))) return TFR_EINVAL;
+  if (B > 0 && (!workspace || workspace_bytes < workspace_bytes_of(B, L, T) || !aligned(workspace, 16))) return TFR_EINVAL;
   const Workspace w = workspace_at(workspace, B, L, T);
   hipStream_t st = (hipStream_t)stream;
   a.wide = a.wide && aligned(dlog_probs, 16);
   if (B == 0 || (long)L * T <= SMALL_LIST) {
-    int slots = 0;
-    while ((1 << slots) < L) ++slots;
-    if (B > 0 && (long)L * T <= SHORT_LIST)
-      preference_wave_kernel<<<(B + 3) / 4, 256, 0, st>>>(a, slots, w.loss, dlog_probs);
-    else if (B > 0)
-      preference_list_kernel<<<B, 256, 0, st>>>(a, w.loss, dlog_probs);
+    if (B > 0 && (long)L * T <= SHORT_LIST) launch_short(a, w.loss, dlog_probs, nullptr, st);
+    else if (B > 0) preference_list_kernel<<<B, 256, 0, st>>>(a, w.loss, dlog_probs);
     preference_total_kernel<<<1, 1024, 0, st>>>(w.loss, B, total);
   } else {
     preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);

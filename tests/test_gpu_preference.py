@@ -58,6 +58,12 @@ def test_sizes(B, L, tokens):
     check(*make(B, L, tokens))
 
 
+@pytest.mark.parametrize('B,L,tokens', [(4500, 3, 5), (5001, 2, 1), (4099, 5, 30), (8191, 1, 3)])
+def test_many_short_lists(B, L, tokens):
+    """So many that a list has a part of a wavefront, the last wavefront some lists too few."""
+    check(*make(B, L, tokens), kind='squared', normalize=True)
+
+
 def test_optional_arguments():
     y, lp, ref, mask, w = make(4, 3, 50)
     check(y, lp, None, None, None)
