@@ -3,8 +3,8 @@
 //   m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2
 //   p <- p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// HBM-bound: with fp32 parameters and moments 16 bytes are read and 12 written an element (152 M elements in 98 tensors: 830 us =
-// 5.1 TB/s; the 14 tensors of a 136-512-512-512-1 tower: 7 us).  The addresses and lengths of up to
+// HBM-bound: with fp32 parameters and moments 16 bytes are read and 12 written an element (152 M elements in 98 tensors: 801 us =
+// 5.3 TB/s; the 14 tensors of a 136-512-512-512-1 tower: 7 us).  The addresses and lengths of up to
 // TFR_ADAMW_MAX_TENSORS (TFR_ADAMW8_MAX_TENSORS) tensors travel in the kernel's arguments: no table in device memory that a
 // step would have to copy first (the gradients' addresses change from step to step), and a captured launch holds its own.
 //
@@ -67,10 +67,22 @@ __device__ __forceinline__ float updated(float p, float m, float v, const Now& w
   return p * w.decay - m * w.step / (sqrtf(v) * w.root + eps);
 }
 
+// STREAM: a launch over more than the Infinity Cache (256 MB) goes past the caches (152 M fp32 elements 833 -> 801 us, 246 M bf16 with
+// 8-bit moments 536 -> 524; the tower's 14 tensors, 10 MB: 7.1 -> 7.7).
+template <typename T, int E, bool STREAM>
+__device__ __forceinline__ void get(const T* __restrict__ p, float (&v)[E]) {
+  widen<T, E>(STREAM ? load_raw_stream<T, E>(p) : load_raw<T, E>(p), v);
+}
+template <typename T, int E, bool STREAM>
+__device__ __forceinline__ void put(T* __restrict__ p, const float (&v)[E]) {
+  if (STREAM) store_pack_stream<T, E>(p, v);
+  else store_pack<T, E>(p, v);
+}
+
 constexpr int BLOCK32 = 4096;          // elements of a workgroup
 constexpr int BLOCK8 = 4096;
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void adamw_kernel(const Table32 t) {
   const int i = tensor_of(t, blockIdx.x);
   const long n = t.n[i], base = (long)(blockIdx.x - t.first[i]) * BLOCK32;
@@ -87,19 +99,19 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table32 t) {
     for (int k = 0; k < BLOCK32 / 1024; ++k) {
       const int at = k * 1024 + threadIdx.x * 4;
       float pe[4], ge[4], me[4], ve[4];
-      load_pack<T, 4>(p + at, pe);
-      load_pack<T, 4>(g + at, ge);
-      load_pack<float, 4>(m + at, me);
-      load_pack<float, 4>(v + at, ve);
+      get<T, 4, STREAM>(p + at, pe);
+      get<T, 4, STREAM>(g + at, ge);
+      get<float, 4, STREAM>(m + at, me);
+      get<float, 4, STREAM>(v + at, ve);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         me[e] = b1 * me[e] + c1 * ge[e];
         ve[e] = b2 * ve[e] + c2 * (ge[e] * ge[e]);
         pe[e] = updated(pe[e], me[e], ve[e], w, eps);
       }
-      store_pack<float, 4>(m + at, me);
-      store_pack<float, 4>(v + at, ve);
-      store_pack<T, 4>(p + at, pe);
+      put<float, 4, STREAM>(m + at, me);
+      put<float, 4, STREAM>(v + at, ve);
+      put<T, 4, STREAM>(p + at, pe);
     }
     return;
   }
@@ -136,8 +148,8 @@ __device__ __forceinline__ float row_max(float x) {
 //
 // Codes are chosen in fp32 (the value over the scale is off by at most 255 * 5.5 * 2^-24 = 8.4e-5 of a step) and again in fp64 by the
 // few threads that hold a value within 1e-4 of a border: the same codes as fp64 throughout, at half the instructions (246 M
-// bf16 elements: 787 us with all of it in fp64, bound by instruction issue; 535 us so, 4.6 TB/s, near what a copy reaches).
-template <typename T>
+// bf16 elements: 787 us with all of it in fp64, bound by instruction issue; 524 us so, 4.7 TB/s, near what a copy reaches).
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
   const int i = tensor_of(t, blockIdx.x);
   const long n = t.n[i], base = (long)(blockIdx.x - t.first[i]) * BLOCK8;
@@ -163,8 +175,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
     if (whole) {
 #pragma unroll
       for (int q = 0; q < 8; q += W) {
-        load_pack<T, W>(p + at + q, *reinterpret_cast<float(*)[W]>(pe + q));
-        load_pack<T, W>(g + at + q, *reinterpret_cast<float(*)[W]>(ge + q));
+        get<T, W, STREAM>(p + at + q, *reinterpret_cast<float(*)[W]>(pe + q));
+        get<T, W, STREAM>(g + at + q, *reinterpret_cast<float(*)[W]>(ge + q));
       }
     } else {
 #pragma unroll
@@ -272,7 +284,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
     }
     if (whole) {
 #pragma unroll
-      for (int q = 0; q < 8; q += W) store_pack<T, W>(p + at + q, *reinterpret_cast<float(*)[W]>(pe + q));
+      for (int q = 0; q < 8; q += W) put<T, W, STREAM>(p + at + q, *reinterpret_cast<float(*)[W]>(pe + q));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -313,6 +325,19 @@ __global__ void adamw_advance_kernel(long* __restrict__ count, const float* __re
   now[0] = (float)(1.0 - lr * decay);
   now[1] = (float)(lr / (1.0 - pow(b1, (double)t)));
   now[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+}
+
+constexpr long kCache = 256l << 20;
+
+template <typename T>
+void launch32(const Table32& t, int blocks, hipStream_t st) {
+  const auto kernel = (long)blocks * BLOCK32 * (2 * (long)sizeof(T) + 8) > kCache ? adamw_kernel<T, true> : adamw_kernel<T, false>;
+  kernel<<<blocks, 256, 0, st>>>(t);
+}
+template <typename T>
+void launch8(const Table8& t, int blocks, hipStream_t st) {
+  const auto kernel = (long)blocks * BLOCK8 * (2 * (long)sizeof(T) + 2) > kCache ? adamw8_kernel<T, true> : adamw8_kernel<T, false>;
+  kernel<<<blocks, 256, 0, st>>>(t);
 }
 
 bool bad_betas(double b1, double b2) { return !(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0); }
@@ -361,9 +386,9 @@ extern "C" int tfr_adamw(int dtype, int count, void* const* params_host, const v
   const int blocks = t.first[count];
   if (blocks == 0) return TFR_OK;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == TFR_DTYPE_F32) adamw_kernel<float><<<blocks, 256, 0, st>>>(t);
-  else if (dtype == TFR_DTYPE_BF16) adamw_kernel<__bf16><<<blocks, 256, 0, st>>>(t);
-  else adamw_kernel<_Float16><<<blocks, 256, 0, st>>>(t);
+  if (dtype == TFR_DTYPE_F32) launch32<float>(t, blocks, st);
+  else if (dtype == TFR_DTYPE_BF16) launch32<__bf16>(t, blocks, st);
+  else launch32<_Float16>(t, blocks, st);
   return (int)hipGetLastError();
 }
 
@@ -384,9 +409,9 @@ extern "C" int tfr_adamw8(int dtype, int count, void* const* params_host, const 
   const int blocks = t.first[count];
   if (blocks == 0) return TFR_OK;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == TFR_DTYPE_F32) adamw8_kernel<float><<<blocks, 256, 0, st>>>(t);
-  else if (dtype == TFR_DTYPE_BF16) adamw8_kernel<__bf16><<<blocks, 256, 0, st>>>(t);
-  else adamw8_kernel<_Float16><<<blocks, 256, 0, st>>>(t);
+  if (dtype == TFR_DTYPE_F32) launch8<float>(t, blocks, st);
+  else if (dtype == TFR_DTYPE_BF16) launch8<__bf16>(t, blocks, st);
+  else launch8<_Float16>(t, blocks, st);
   return (int)hipGetLastError();
 }
 

@@ -7,11 +7,11 @@
 //   l(h)  = (1 - a) softplus(-h) + a softplus(h)   |   max(0, 1 - h)   |   (h - 1/2)^2
 //   dloss/dlp_it = m_it f_i sum over the pairs of i of +-l'(h) w / P,   f_i = beta (/ length)
 // 9 bytes a token are read (4 + 4 + the mask's 1) and, with the mask once more, 4 written: HBM-bound for long answers (512 lists x 6
-// x 8192 tokens: 48 us for the sums = 4.7 TB/s, 28 for the gradient, 7 for the pairs), launch-bound for short ones.
+// x 8192 tokens: 31 us for the sums = 7.2 TB/s, 19 for the gradient = 6.6, 6 for the pairs), launch-bound for short ones.
 // Sums over tokens are fp64: a margin is the difference of two sums of thousands of tokens.  What stands in masked places or
 // in answers with y < 0 is never used (NaN there does no harm).
 #include "common.h"
-#include "../../include/tfr_hip.h"
+#include "elem.h"
 
 using namespace tfr;
 
@@ -43,8 +43,14 @@ __device__ __forceinline__ void add_token(Sum& r, float lp, float ref, bool on) 
   r.n += on ? 1 : 0;
 }
 
+// STREAM: arrays beyond the L2 caches (32 MB each) go past the caches (100 MB each: sums 48 -> 31 us, gradient 28 -> 19).
+template <bool STREAM>
+__device__ __forceinline__ void load4(const float* __restrict__ p, float (&v)[4]) {
+  widen<float, 4>(STREAM ? load_raw_stream<float, 4>(p) : load_raw<float, 4>(p), v);
+}
+
 // Tokens lo .. hi of answer `seq`, by THREADS threads; 4 tokens an access between the first and the last multiple of 4 in memory.
-template <int THREADS>
+template <int THREADS, bool STREAM>
 __device__ __forceinline__ Sum token_sum(const PrefArgs& a, long seq, int lo, int hi, int tid) {
   Sum r = {0.0, 0};
   const long at = seq * a.T + lo, end = seq * a.T + hi;
@@ -59,33 +65,29 @@ __device__ __forceinline__ Sum token_sum(const PrefArgs& a, long seq, int lo, in
   if (tid < head - at) one(at + tid);
   if (tid < end - tail) one(tail + tid);
   for (long t = head + 4 * tid; t < tail; t += 16 * THREADS) {
-    float4 x[4], y[4];
+    float x[4][4], y[4][4];
     uint32_t m[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const long u = t + 4l * THREADS * k;
       if (u < tail) {
-        x[k] = *reinterpret_cast<const float4*>(a.lp + u);
-        y[k] = a.ref ? *reinterpret_cast<const float4*>(a.ref + u) : make_float4(0.f, 0.f, 0.f, 0.f);
+        load4<STREAM>(a.lp + u, x[k]);
+        if (a.ref) load4<STREAM>(a.ref + u, y[k]);
         m[k] = a.mask ? *reinterpret_cast<const uint32_t*>(a.mask + u) : 0x01010101u;
       } else {
-        x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        m[k] = 0u;
+        m[k] = 0u;                                              // what is not loaded is not used
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      add_token(r, x[k].x, y[k].x, (m[k] & 0xffu) != 0);
-      add_token(r, x[k].y, y[k].y, (m[k] & 0xff00u) != 0);
-      add_token(r, x[k].z, y[k].z, (m[k] & 0xff0000u) != 0);
-      add_token(r, x[k].w, y[k].w, (m[k] & 0xff000000u) != 0);
-    }
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add_token(r, x[k][e], a.ref ? y[k][e] : 0.f, ((m[k] >> (8 * e)) & 0xffu) != 0);
   }
   return r;
 }
 
 // out = m c on tokens lo .. hi of answer `seq`.
-template <int THREADS>
+template <int THREADS, bool STREAM>
 __device__ __forceinline__ void token_fill(const uint8_t* __restrict__ mask, bool wide, long seq, int T, int lo, int hi, int tid, float c,
                                            float* __restrict__ out) {
   const long at = seq * T + lo, end = seq * T + hi;
@@ -102,7 +104,9 @@ __device__ __forceinline__ void token_fill(const uint8_t* __restrict__ mask, boo
 #pragma unroll 4
   for (long t = head + 4 * tid; t < tail; t += 4 * THREADS) {
     const uint32_t m = mask ? *reinterpret_cast<const uint32_t*>(mask + t) : 0x01010101u;
-    *reinterpret_cast<float4*>(out + t) = make_float4(m & 0xffu ? c : 0.f, m & 0xff00u ? c : 0.f, m & 0xff0000u ? c : 0.f, m & 0xff000000u ? c : 0.f);
+    const float v[4] = {m & 0xffu ? c : 0.f, m & 0xff00u ? c : 0.f, m & 0xff0000u ? c : 0.f, m & 0xff000000u ? c : 0.f};
+    if (STREAM) store_pack_stream<float, 4>(out + t, v);
+    else store_pack<float, 4>(out + t, v);
   }
 }
 
@@ -115,12 +119,13 @@ __device__ __forceinline__ Sum wave_sum_tokens(Sum v) {
   return v;
 }
 
+template <bool STREAM>
 __global__ __launch_bounds__(256) void preference_sum_kernel(const PrefArgs a, double* __restrict__ part_sum, int* __restrict__ part_n) {
   __shared__ Sum s_part[4];
   const long seq = blockIdx.x;
   const int lo = blockIdx.y * a.part, hi = lo + a.part < a.T ? lo + a.part : a.T;
   Sum v = {0.0, 0};
-  if (a.labels[seq] >= 0.f) v = token_sum<256>(a, seq, lo, hi, threadIdx.x);
+  if (a.labels[seq] >= 0.f) v = token_sum<256, STREAM>(a, seq, lo, hi, threadIdx.x);
   v = wave_sum_tokens(v);
   if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -226,6 +231,7 @@ __global__ __launch_bounds__(1024) void preference_total_kernel(const float* __r
 }
 
 // dlp[seq, t] = m * coef[seq] * upstream[list]; the last workgroup of the first part adds the lists' losses where a total is wanted.
+template <bool STREAM>
 __global__ __launch_bounds__(256) void preference_grad_kernel(const float* __restrict__ coef, const float* __restrict__ upstream,
                                                               const uint8_t* __restrict__ mask, int L, int T, int part, bool wide,
                                                               float* __restrict__ out, const float* __restrict__ loss, int B,
@@ -238,7 +244,7 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const float* __res
   const int lo = blockIdx.y * part, hi = lo + part < T ? lo + part : T;
   float c = coef[seq];
   if (upstream) c *= upstream[seq / L];
-  token_fill<256>(mask, wide, seq, T, lo, hi, threadIdx.x, c, out);
+  token_fill<256, STREAM>(mask, wide, seq, T, lo, hi, threadIdx.x, c, out);
 }
 
 // Short lists, `lanes` (a power of two) lanes each, of which an answer has lanes / slots (slots: the power of two that holds the
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(256) void preference_list_kernel(const PrefArgs a, 
   for (int i = wave; i < a.L; i += 4) {
     const long seq = (long)b * a.L + i;
     Sum v = {0.0, 0};
-    if (a.labels[seq] >= 0.f) v = token_sum<64>(a, seq, 0, a.T, lane);
+    if (a.labels[seq] >= 0.f) v = token_sum<64, false>(a, seq, 0, a.T, lane);
     v = wave_sum_tokens(v);
     if (lane == 0) s_sum[i] = v;
   }
@@ -310,7 +316,7 @@ __global__ __launch_bounds__(256) void preference_list_kernel(const PrefArgs a, 
     if (here) s_coef[lane] = (float)c;
   }
   __syncthreads();
-  for (int i = wave; i < a.L; i += 4) token_fill<64>(a.mask, a.wide, (long)b * a.L + i, a.T, 0, a.T, lane, s_coef[i], out);
+  for (int i = wave; i < a.L; i += 4) token_fill<64, false>(a.mask, a.wide, (long)b * a.L + i, a.T, 0, a.T, lane, s_coef[i], out);
 }
 
 constexpr long kMostTokens = 1 << 28;
@@ -318,7 +324,8 @@ constexpr long kMostAnswers = (1l << 24) - 2;        // answers of all lists: a 
 
 bool bad_sizes(int B, int L, int T) { return B < 0 || L < 1 || L > MAX_ANSWERS || T < 0 || T > kMostTokens || (long)B * L > kMostAnswers; }
 // Long parts where there are enough of them to fill the card, short ones else.
-int part_of(int B, int L, int T) { return (long)B * L * T >= (1l << 23) ? LONG_PART : SHORT_PART; }
+bool many_tokens(int B, int L, int T) { return (long)B * L * T >= (1l << 23); }
+int part_of(int B, int L, int T) { return many_tokens(B, L, T) ? LONG_PART : SHORT_PART; }
 int parts_of(int B, int L, int T) { return T > 0 ? (T + part_of(B, L, T) - 1) / part_of(B, L, T) : 1; }
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }       // null too
 
@@ -347,6 +354,11 @@ void launch_short(const PrefArgs& a, float* loss, float* out, float* coef, hipSt
   while ((1 << slots) < a.L) ++slots;
   while (lanes > slots && (4l << lanes) >= (long)a.L * a.T && ((long)a.B << lanes) > 64 * 4096) --lanes;
   preference_wave_kernel<<<(unsigned)((((long)a.B << lanes) + 255) / 256), 256, 0, st>>>(a, lanes, slots, loss, out, coef);
+}
+
+void launch_sums(const PrefArgs& a, const Workspace& w, hipStream_t st) {
+  const auto kernel = many_tokens(a.B, a.L, a.T) ? preference_sum_kernel<true> : preference_sum_kernel<false>;
+  kernel<<<dim3((unsigned)(a.B * a.L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
 }
 
 int make_args(PrefArgs* a, const float* log_probs, const float* reference, const uint8_t* mask, const float* labels, const float* list_weights,
@@ -380,7 +392,7 @@ extern "C" int tfr_preference_loss_f32(const float* log_probs, const float* refe
   if ((long)L * T <= SHORT_LIST) {
     launch_short(a, loss, nullptr, coef, st);
   } else {
-    preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
+    launch_sums(a, w, st);
     preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, loss, coef);
   }
   return (int)hipGetLastError();
@@ -396,7 +408,8 @@ extern "C" int tfr_preference_grad_f32(const float* coef, const float* upstream,
     preference_grad_short_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (hipStream_t)stream>>>(coef, upstream, mask, L, T, (unsigned)n, dlog_probs);
     return (int)hipGetLastError();
   }
-  preference_grad_kernel<<<dim3((unsigned)(B * L), parts_of(B, L, T)), 256, 0, (hipStream_t)stream>>>(
+  const auto kernel = many_tokens(B, L, T) ? preference_grad_kernel<true> : preference_grad_kernel<false>;
+  kernel<<<dim3((unsigned)(B * L), parts_of(B, L, T)), 256, 0, (hipStream_t)stream>>>(
       coef, upstream, mask, L, T, part_of(B, L, T), aligned(dlog_probs, 16) && aligned(mask, 4), dlog_probs, nullptr, B, nullptr);
   return (int)hipGetLastError();
 }
@@ -418,9 +431,10 @@ extern "C" int tfr_preference_loss_and_grad_f32(const float* log_probs, const fl
     else if (B > 0) preference_list_kernel<<<B, 256, 0, st>>>(a, w.loss, dlog_probs);
     preference_total_kernel<<<1, 1024, 0, st>>>(w.loss, B, total);
   } else {
-    preference_sum_kernel<<<dim3((unsigned)(B * L), a.parts), 256, 0, st>>>(a, w.sum, w.n);
+    launch_sums(a, w, st);
     preference_pairs_kernel<<<B, 64, 0, st>>>(a, w.sum, w.n, w.loss, w.coef);
-    preference_grad_kernel<<<dim3((unsigned)(B * L) + 1, a.parts), 256, 0, st>>>(w.coef, nullptr, mask, L, T, a.part, a.wide, dlog_probs, w.loss, B, total);
+    const auto kernel = many_tokens(B, L, T) ? preference_grad_kernel<true> : preference_grad_kernel<false>;
+    kernel<<<dim3((unsigned)(B * L) + 1, a.parts), 256, 0, st>>>(w.coef, nullptr, mask, L, T, a.part, a.wide, dlog_probs, w.loss, B, total);
   }
   return (int)hipGetLastError();
 }

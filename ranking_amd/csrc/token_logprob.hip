@@ -6,10 +6,10 @@
 // (max x, sum exp((x - max) / T)) of every row kept for the backward, which is one read and one write of the row:
 // p = exp((x - max) / T) / sum.  A row with target < 0 is no target: log probability 0, gradient 0, its logits are not read.
 // A target beyond the row: NaN in both.
-// Bound by HBM (8192 x 50 021 bf16, a tenth without a target: 177 us forward = 4.2 TB/s, 312 us backward = 5.0 TB/s; a copy
+// Bound by HBM (8192 x 50 021 bf16, a tenth without a target: 123 us forward = 6.0 TB/s, 330 us backward = 4.7 TB/s; a copy
 // reaches 4.9).  A row is read by 16-byte accesses between its first and last 16-byte boundary: rows of an odd length start
 // anywhere.  Few long rows are split over workgroups and joined by a second launch (2 x 131 072: 5 us), short ones share a
-// wavefront (16 384 x 200 fp32: 11 us with the gradient, 17 with a wavefront a row).
+// wavefront (16 384 x 200 fp32: 12 us with the gradient, 17 with a wavefront a row).
 #include "common.h"
 #include "elem.h"
 
@@ -75,8 +75,15 @@ __device__ __forceinline__ Stat block_stat(Stat a, float c) {
   return a;
 }
 
-// Statistics of x[lo, hi) by `threads` threads: single elements up to the first 16-byte boundary and behind the last.
-template <typename T, int THREADS>
+// STREAM: logits beyond the Infinity Cache (256 MB) are read, and their gradient written, past the caches (8192 x 50 021 bf16: 175 +
+// 311 us through them, 123 + 330 so; 16 384 x 200 fp32, 13 MB: 12.5 us for 13.5).
+template <typename T, int E, bool STREAM>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, float (&v)[E]) {
+  widen<T, E>(STREAM ? load_raw_stream<T, E>(p) : load_raw<T, E>(p), v);
+}
+
+// Statistics of x[lo, hi) by THREADS threads: single elements up to the first 16-byte boundary and behind the last.
+template <typename T, int THREADS, bool STREAM>
 __device__ __forceinline__ Stat row_stat(const T* __restrict__ x, int lo, int hi, int tid, float c) {
   constexpr int E = 16 / sizeof(T);
   Stat a = {-INFINITY, 0.f};
@@ -93,13 +100,13 @@ __device__ __forceinline__ Stat row_stat(const T* __restrict__ x, int lo, int hi
   for (; i + 3 * THREADS < packs; i += 4 * THREADS) {
     float v[4][E];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) load_pack<T, E>(p + (long)(i + k * THREADS) * E, v[k]);
+    for (int k = 0; k < 4; ++k) load_row<T, E, STREAM>(p + (long)(i + k * THREADS) * E, v[k]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) a.take<E>(v[k], c);
   }
   for (; i < packs; i += THREADS) {
     float v[E];
-    load_pack<T, E>(p + (long)i * E, v);
+    load_row<T, E, STREAM>(p + (long)i * E, v);
     a.take<E>(v, c);
   }
   const int tail = head + packs * E;
@@ -110,9 +117,14 @@ __device__ __forceinline__ Stat row_stat(const T* __restrict__ x, int lo, int hi
   return a;
 }
 
+// The chosen token's logit, read while the row is summed; NaN where there is no such token.
 template <typename T>
-__device__ __forceinline__ void write_logp(const T* x, long target, int vocab, Stat a, float inv_t, float* logp, float* stats) {
-  *logp = target < vocab ? ((float)x[target] - a.m) * inv_t - logf(a.s) : __builtin_nanf("");
+__device__ __forceinline__ float chosen(const T* __restrict__ x, long target, int vocab) {
+  return target < vocab ? (float)x[target] : __builtin_nanf("");
+}
+
+__device__ __forceinline__ void write_logp(float xy, Stat a, float inv_t, float* logp, float* stats) {
+  *logp = (xy - a.m) * inv_t - logf(a.s);
   if (stats) {
     stats[0] = a.m;
     stats[1] = a.s;
@@ -140,12 +152,13 @@ __global__ __launch_bounds__(256) void logprob_wave_kernel(const T* __restrict__
   }
   const T* x = logits + rows.offset(row);
   const float c = inv_t * kLog2e;
-  const Stat a = wave_stat<LANES>(row_stat<T, LANES>(x, 0, vocab, lane, c), c);
-  if (lane == 0) write_logp(x, y, vocab, a, inv_t, logp + row, st);
+  const float xy = chosen(x, y, vocab);
+  const Stat a = wave_stat<LANES>(row_stat<T, LANES, false>(x, 0, vocab, lane, c), c);
+  if (lane == 0) write_logp(xy, a, inv_t, logp + row, st);
 }
 
 // One workgroup a row (gridDim.y == 1), or a part of a row whose statistics go to parts[row][blockIdx.y].
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void logprob_block_kernel(const T* __restrict__ logits, const Rows rows, const int64_t* __restrict__ target,
                                                             int vocab, int part, float inv_t, float* __restrict__ logp,
                                                             float* __restrict__ stats, float* __restrict__ parts) {
@@ -160,10 +173,11 @@ __global__ __launch_bounds__(256) void logprob_block_kernel(const T* __restrict_
   const float c = inv_t * kLog2e;
   const long lo = (long)blockIdx.y * part;
   const int hi = (int)(lo + part < vocab ? lo + part : vocab);
-  const Stat a = block_stat(row_stat<T, 256>(x, (int)lo, hi, threadIdx.x, c), c);
+  const float xy = gridDim.y == 1 && threadIdx.x == 0 ? chosen(x, y, vocab) : 0.f;
+  const Stat a = block_stat(row_stat<T, 256, STREAM>(x, (int)lo, hi, threadIdx.x, c), c);
   if (threadIdx.x != 0) return;
   if (gridDim.y == 1) {
-    write_logp(x, y, vocab, a, inv_t, logp + row, st);
+    write_logp(xy, a, inv_t, logp + row, st);
   } else {
     float* p = parts + 2 * (row * gridDim.y + blockIdx.y);
     p[0] = a.m;
@@ -181,18 +195,19 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(const T* __restrict__
   const long y = target[row];
   if (y < 0) return;                                           // written by the first launch
   const float c = inv_t * kLog2e;
+  const float xy = chosen(logits + rows.offset(row), y, vocab);
   Stat a = {-INFINITY, 0.f};
   for (int i = lane; i < splits; i += 64) {
     const Stat b = {parts[2 * (row * splits + i)], parts[2 * (row * splits + i) + 1]};
     a.add(b, c);
   }
   a = wave_stat(a, c);
-  if (lane == 0) write_logp(logits + rows.offset(row), y, vocab, a, inv_t, logp + row, stats ? stats + 2 * row : nullptr);
+  if (lane == 0) write_logp(xy, a, inv_t, logp + row, stats ? stats + 2 * row : nullptr);
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
 // out[lo, hi) of one row by THREADS threads; aligned stores, the loads wide as well where x lies on the same offset.
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool STREAM>
 __device__ __forceinline__ void grad_row(const T* __restrict__ x, T* __restrict__ out, int lo, int hi, int tid, long y, float g, float m,
                                          float over_s, float c) {
   constexpr int E = 16 / sizeof(T);
@@ -211,13 +226,14 @@ __device__ __forceinline__ void grad_row(const T* __restrict__ x, T* __restrict_
     for (int i = tid; i < packs; i += THREADS) {
       const int at = head + i * E;
       float v[E];
-      load_pack<T, E>(x + at, v);
+      load_row<T, E, STREAM>(x + at, v);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float p = scale * __builtin_amdgcn_exp2f((v[e] - m) * c);
         v[e] = at + e == y ? g + p : p;
       }
-      store_pack<T, E>(out + at, v);
+      if (STREAM) store_pack_stream<T, E>(out + at, v);
+      else store_pack<T, E>(out + at, v);
     }
   } else {
     for (int i = head + tid; i < tail; i += THREADS) one(i);
@@ -239,7 +255,7 @@ __device__ __forceinline__ void fill_row(T* __restrict__ out, int lo, int hi, in
   for (int i = tid; i < packs; i += THREADS) store_pack<T, E>(out + head + (long)i * E, v);
 }
 
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool STREAM>
 __device__ __forceinline__ void grad_part(const T* __restrict__ logits, const Rows& rows, const int64_t* __restrict__ target,
                                           const float* __restrict__ stats, const float* __restrict__ upstream, long row, int vocab,
                                           int lo, int hi, int tid, float inv_t, T* __restrict__ out) {
@@ -251,7 +267,7 @@ __device__ __forceinline__ void grad_part(const T* __restrict__ logits, const Ro
   } else if (y >= vocab) {
     fill_row<T, THREADS>(o, lo, hi, tid, __builtin_nanf(""));
   } else {
-    grad_row<T, THREADS>(logits + rows.offset(row), o, lo, hi, tid, y, upstream[row] * inv_t, m, 1.f / s, inv_t * kLog2e);
+    grad_row<T, THREADS, STREAM>(logits + rows.offset(row), o, lo, hi, tid, y, upstream[row] * inv_t, m, 1.f / s, inv_t * kLog2e);
   }
 }
 
@@ -261,16 +277,16 @@ __global__ __launch_bounds__(256) void logprob_grad_wave_kernel(const T* __restr
                                                                 int vocab, float inv_t, T* __restrict__ out) {
   const long row = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   if (row >= n) return;
-  grad_part<T, LANES>(logits, rows, target, stats, upstream, row, vocab, 0, vocab, threadIdx.x & (LANES - 1), inv_t, out);
+  grad_part<T, LANES, false>(logits, rows, target, stats, upstream, row, vocab, 0, vocab, threadIdx.x & (LANES - 1), inv_t, out);
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void logprob_grad_block_kernel(const T* __restrict__ logits, const Rows rows, const int64_t* __restrict__ target,
                                                                  const float* __restrict__ stats, const float* __restrict__ upstream,
                                                                  int vocab, int part, float inv_t, T* __restrict__ out) {
   const long lo = (long)blockIdx.y * part;
   const int hi = (int)(lo + part < vocab ? lo + part : vocab);
-  grad_part<T, 256>(logits, rows, target, stats, upstream, blockIdx.x, vocab, (int)lo, hi, threadIdx.x, inv_t, out);
+  grad_part<T, 256, STREAM>(logits, rows, target, stats, upstream, blockIdx.x, vocab, (int)lo, hi, threadIdx.x, inv_t, out);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -292,6 +308,9 @@ bool bad_args(int dtype, long per, long stride_b, long stride_t, long n, int voc
          !(temperature > 0.f) || !(inv > 0.f) || inv == INFINITY;
 }
 
+template <typename T>
+bool beyond_cache(long n, int vocab) { return n * vocab * (long)sizeof(T) > (256l << 20); }
+
 // Lanes of a short row: a few 16-byte accesses each.
 template <typename T>
 int lanes_of(int vocab) {
@@ -310,7 +329,8 @@ int forward(const T* logits, Rows rows, const int64_t* target, long n, int vocab
   }
   const int splits = splits_of(n, vocab);
   const int part = ((vocab + splits - 1) / splits + 7) / 8 * 8;
-  logprob_block_kernel<T><<<dim3((unsigned)n, splits), 256, 0, st>>>(logits, rows, target, vocab, part, inv_t, logp, stats, parts);
+  const auto kernel = beyond_cache<T>(n, vocab) ? logprob_block_kernel<T, true> : logprob_block_kernel<T, false>;
+  kernel<<<dim3((unsigned)n, splits), 256, 0, st>>>(logits, rows, target, vocab, part, inv_t, logp, stats, parts);
   if (splits > 1)
     logprob_join_kernel<T><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(logits, rows, target, n, vocab, splits, inv_t, parts, logp, stats);
   return (int)hipGetLastError();
@@ -325,8 +345,8 @@ int backward(const T* logits, Rows rows, const int64_t* target, const float* sta
     kernel<<<(unsigned)((n * lanes + 255) / 256), 256, 0, st>>>(logits, rows, target, stats, upstream, n, vocab, inv_t, out);
   } else {
     const int part = 256 * 8 * (16 / (int)sizeof(T));
-    logprob_grad_block_kernel<T><<<dim3((unsigned)n, (vocab + part - 1) / part), 256, 0, st>>>(logits, rows, target, stats, upstream, vocab,
-                                                                                                part, inv_t, out);
+    const auto kernel = beyond_cache<T>(n, vocab) ? logprob_grad_block_kernel<T, true> : logprob_grad_block_kernel<T, false>;
+    kernel<<<dim3((unsigned)n, (vocab + part - 1) / part), 256, 0, st>>>(logits, rows, target, stats, upstream, vocab, part, inv_t, out);
   }
   return (int)hipGetLastError();
 }

@@ -170,6 +170,32 @@ def test_shifted_and_shaped_tensors(dtype):
     assert torch.equal(P[1:], Q[0]) and P[0] == p[0][0].to(DEV) and all(torch.equal(a, b) for a, b in zip(S[0], R[0]))
 
 
+@pytest.mark.parametrize('bits,dtype', [(32, torch.float32), (32, torch.bfloat16), (8, torch.float32), (8, torch.bfloat16)])
+def test_launches_beyond_the_caches(bits, dtype):
+    """48 M elements, a launch that goes past the caches: the same bits as in parts that do not."""
+    n = 48 * 1024 * 1024 + 77
+    p, g = (torch.randn(n, device=DEV) * s for s in (1.0, 0.1))
+    whole, parts = [p.to(dtype), g.to(dtype)], [p.to(dtype), g.to(dtype)]
+    codes, blocks = O().quantized_size(n)
+    for t in (whole, parts):
+        t += ([torch.zeros(codes, dtype=torch.int8, device=DEV), torch.zeros(blocks, device=DEV), torch.zeros(codes, dtype=torch.uint8, device=DEV),
+               torch.zeros(blocks, device=DEV)] if bits == 8 else [torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)])
+
+    def step(t, a, b, k):
+        q = (a // 128, (b + 127) // 128)
+        if bits == 8:
+            moments = [(t[i][q[0] * 128:q[1] * 128], t[i + 1][q[0]:q[1]]) for i in (2, 4)]
+        else:
+            moments = [t[i][a:b] for i in (2, 3)]
+        O().adamw_step([t[0][a:b]], [t[1][a:b]], [moments[0]], [moments[1]], step=k, **HYPER)
+    cut = 4 * 1024 * 1024
+    for k in (1, 2):
+        step(whole, 0, n, k)
+        for a in range(0, n, cut):
+            step(parts, a, min(n, a + cut), k)
+    assert all(torch.equal(x, y) for x, y in zip(whole, parts))
+
+
 def test_mixed_types_in_one_call():
     a, b = make([100, 50], torch.float32), make([200], torch.bfloat16)
     mixed = [x + y for x, y in zip(a, b)]

@@ -64,6 +64,25 @@ def test_many_short_lists(B, L, tokens):
     check(*make(B, L, tokens), kind='squared', normalize=True)
 
 
+def test_tokens_beyond_the_caches():
+    """8.7 M tokens go past the caches, each list as it is alone; odd rows."""
+    B, L, tokens = 11, 3, 264001
+    g = torch.Generator(device=DEV).manual_seed(4)
+    lp, ref = (torch.randn(B, L, tokens, device=DEV, generator=g) for _ in range(2))
+    mask = torch.rand(B, L, tokens, device=DEV, generator=g) < 0.5
+    y = torch.tensor([2.0, 0.0, 1.0], device=DEV).expand(B, L)
+    loss = K().PreferenceLoss(reduction='sum', length_normalized=True, beta=1.0)
+    total, grad = loss.loss_and_grad(y, lp, reference=ref, mask=mask)
+    parts = [loss.loss_and_grad(y[k:k + 1], lp[k:k + 1].clone(), reference=ref[k:k + 1].clone(), mask=mask[k:k + 1].clone()) for k in range(B)]
+    # fp64 sums in another order, then the same roundings
+    want = torch.cat([p[1] for p in parts]).double()
+    T.assert_within(grad, want, 2 * T.U * want.abs())
+    T.assert_within(total, sum(p[0].double() for p in parts), (B + 1) * T.U * total.double().abs())
+    p = lp.requires_grad_()
+    loss(y, p, reference=ref, mask=mask).backward()
+    assert torch.equal(p.grad, grad)
+
+
 def test_optional_arguments():
     y, lp, ref, mask, w = make(4, 3, 50)
     check(y, lp, None, None, None)

@@ -145,6 +145,20 @@ def test_offsets_beyond_32_bits():
     assert grad[n - 1, vocab - 1] > 0.99 and not grad[n - 2].any() and grad[n - 1, 0] < 0
 
 
+def test_logits_beyond_the_caches():
+    """300 MB of logits go past the caches: the same bits as the same rows alone."""
+    x = torch.randn(1500, 100003, dtype=torch.bfloat16, device=DEV)
+    t = torch.randint(-1, 100003, (1500,), generator=torch.Generator().manual_seed(8)).to(DEV)
+    up = torch.randn(1500, device=DEV)
+    logp, stats = P().token_log_probs_with_stats(x, t)
+    grad = P().token_log_probs_grad(up, x, t, stats)
+    for rows in (slice(0, 600), slice(900, 1500)):
+        part, part_stats = P().token_log_probs_with_stats(x[rows], t[rows])
+        assert torch.equal(part, logp[rows]) and torch.equal(part_stats, stats[rows])
+        assert torch.equal(P().token_log_probs_grad(up[rows], x[rows], t[rows], part_stats), grad[rows])
+    check(x[3:6, 1:], t[3:6].clamp(max=100001), upstream=up[3:6])
+
+
 def test_other_stream_and_graphs():
     x, t = torch.randn(6, 50000, device=DEV), torch.tensor([1, -1, 3, 4, 5, 6], device=DEV)
     up = torch.randn(6, device=DEV)
