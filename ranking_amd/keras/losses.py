@@ -868,5 +868,5 @@ class PreferenceLoss(_RankingLoss):
         shape = tuple(y_pred.shape) if torch.is_tensor(y_pred) else None
         y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred.detach() if shape is not None else y_pred, sample_weight,
                                                                   reference, mask)
-        total, grad = _preference.preference_loss_and_grad(y_pred, y_true, reference, mask, weight, **how)
+        total, grad = _preference._loss_and_grad(y_pred, y_true, reference, mask, weight, **how)
         return total, grad if len(shape) == 3 else grad.reshape(shape)

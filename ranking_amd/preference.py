@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from . import _ops
-from ._ops import _raw_stream
+from ._ops import _raw_stream, require_device
 from .embedding import _device_of, _dtype_code
 
 KINDS = {'logistic': 0, 'hinge': 1, 'squared': 2}                          # TFR_PREFERENCE_*
@@ -124,6 +124,31 @@ def _address(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _check_dense(index, t, name, shape, dtypes=(torch.float32,)):
+    require_device(t, name)
+    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.get_device() != index or not t.is_contiguous():
+        raise ValueError('%s must be a dense %s tensor of shape %s on device %d, got %s of shape %s on %s'
+                         % (name, ' or '.join(map(str, dtypes)), tuple(shape), index, t.dtype, tuple(t.shape), t.device))
+
+
+def _check_loss(log_probs, labels, reference, mask, list_weights, kind):
+    """Refuses what the loss kernels would not read as it is meant (``keras.losses.PreferenceLoss`` makes its tensors fit)."""
+    if kind not in KINDS:
+        raise ValueError('Invalid kind: {}. Expected "{}"'.format(kind, tuple(KINDS)))
+    require_device(log_probs, 'log_probs')
+    if log_probs.dim() != 3:
+        raise ValueError('log_probs must be [batch, answers, tokens], got shape %s' % (tuple(log_probs.shape),))
+    index, shape = log_probs.get_device(), log_probs.shape
+    _check_dense(index, log_probs, 'log_probs', shape)
+    _check_dense(index, labels, 'labels', shape[:2])
+    if reference is not None:
+        _check_dense(index, reference, 'reference', shape)
+    if mask is not None:
+        _check_dense(index, mask, 'mask', shape, (torch.uint8, torch.bool))
+    if list_weights is not None:
+        _check_dense(index, list_weights, 'list_weights', shape[:1])
+
+
 def _loss_args(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing, length_normalized, scale):
     """(B, L, T, workspace, its bytes, the arguments that both forms of the loss share)."""
     B, L, T = log_probs.shape
@@ -143,6 +168,11 @@ def preference_loss(log_probs: torch.Tensor, labels: torch.Tensor, reference: Op
     """(loss ``[B]``, coefficients ``[B, L]`` of ``preference_grad``).  Dense device tensors: ``log_probs`` and ``reference``
     ``[B, L, T]``, ``labels`` ``[B, L]``, ``list_weights`` ``[B]`` in float32, ``mask`` ``[B, L, T]`` uint8 or bool (what
     ``keras.losses.PreferenceLoss`` makes of its arguments)."""
+    _check_loss(log_probs, labels, reference, mask, list_weights, kind)
+    return _loss(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing, length_normalized, scale)
+
+
+def _loss(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing, length_normalized, scale):
     index = log_probs.get_device()
     with _ops.device_of(index):
         B, L, T, workspace, nbytes, args = _loss_args(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing,
@@ -160,6 +190,11 @@ def preference_loss_and_grad(log_probs: torch.Tensor, labels: torch.Tensor, refe
                              beta: float = 0.1, label_smoothing: float = 0.0, length_normalized: bool = False,
                              scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """(sum of the lists' losses, its gradient ``[B, L, T]``) of the same arguments as ``preference_loss``."""
+    _check_loss(log_probs, labels, reference, mask, list_weights, kind)
+    return _loss_and_grad(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing, length_normalized, scale)
+
+
+def _loss_and_grad(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing, length_normalized, scale):
     index = log_probs.get_device()
     with _ops.device_of(index):
         B, L, T, workspace, nbytes, args = _loss_args(log_probs, labels, reference, mask, list_weights, kind, beta, label_smoothing,
@@ -174,7 +209,21 @@ def preference_loss_and_grad(log_probs: torch.Tensor, labels: torch.Tensor, refe
 
 
 def preference_grad(coef: torch.Tensor, mask: Optional[torch.Tensor], tokens: int, upstream: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``[B, L, tokens]``: the coefficients on the unmasked tokens, times ``upstream`` ``[B]`` (dense float32)."""
+    """``[B, L, tokens]``: the coefficients ``[B, L]`` on the unmasked tokens, times ``upstream`` ``[B]`` (dense float32)."""
+    require_device(coef, 'coef')
+    if coef.dim() != 2 or not 1 <= coef.shape[1] <= MAX_ANSWERS or tokens < 0:
+        raise ValueError('coef must be [batch, answers] with at most %d answers and tokens a length, got shape %s and %r'
+                         % (MAX_ANSWERS, tuple(coef.shape), tokens))
+    index = coef.get_device()
+    _check_dense(index, coef, 'coef', coef.shape)
+    if mask is not None:
+        _check_dense(index, mask, 'mask', tuple(coef.shape) + (tokens,), (torch.uint8, torch.bool))
+    if upstream is not None:
+        _check_dense(index, upstream, 'upstream', coef.shape[:1])
+    return _grad(coef, mask, tokens, upstream)
+
+
+def _grad(coef, mask, tokens, upstream):
     B, L = coef.shape
     index = coef.get_device()
     with _ops.device_of(index):
@@ -189,7 +238,7 @@ def preference_grad(coef: torch.Tensor, mask: Optional[torch.Tensor], tokens: in
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, log_probs, labels, reference, mask, list_weights, how):
-        loss, coef = preference_loss(log_probs, labels, reference, mask, list_weights, **how)
+        loss, coef = _loss(log_probs, labels, reference, mask, list_weights, **how)
         ctx.save_for_backward(coef, *([] if mask is None else [mask]))
         ctx.tokens = log_probs.shape[2]
         return loss
@@ -198,4 +247,4 @@ class _PreferenceFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         coef, *mask = ctx.saved_tensors
-        return preference_grad(coef, mask[0] if mask else None, ctx.tokens, g.contiguous()), None, None, None, None, None
+        return _grad(coef, mask[0] if mask else None, ctx.tokens, g.contiguous()), None, None, None, None, None

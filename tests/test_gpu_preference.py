@@ -229,3 +229,30 @@ def test_refusals():
                 lambda: loss(y.new_zeros(1, 0), lp.new_zeros(1, 0, 2)), lambda: K().PreferenceLoss(reduction='none').loss_and_grad(y, lp)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_raw_calls():
+    """preference_loss, preference_loss_and_grad and preference_grad by themselves, and what they refuse: every tensor has to be
+    dense, of the type and shape that the kernels read."""
+    from ranking_amd import preference as P
+    y, lp, ref, mask, w = (t.to(DEV) for t in make(4, 3, 50))
+    total, grad = P.preference_loss_and_grad(lp, y, ref, mask, w, beta=0.3)
+    want = K().PreferenceLoss('sum', beta=0.3).loss_and_grad(y, lp, w, reference=ref, mask=mask)
+    assert torch.equal(total, want[0]) and torch.equal(grad, want[1])
+    loss, coef = P.preference_loss(lp, y, ref, mask.to(torch.uint8), w, beta=0.3)
+    assert loss.shape == (4,) and coef.shape == (4, 3)
+    assert torch.equal(P.preference_grad(coef, mask, 50), grad)
+    up = torch.tensor([1.0, 2.0, 0.0, -1.0], device=DEV)
+    assert torch.equal(P.preference_grad(coef, mask, 50, up), grad * up.view(4, 1, 1))       # the kernel rounds this product too
+    wide = torch.cat([lp, lp], 2)
+    for bad in (dict(log_probs=lp.double()), dict(log_probs=lp.bfloat16()), dict(log_probs=wide[:, :, :50]), dict(log_probs=lp[0]),
+                dict(labels=y[:3]), dict(labels=y.long()), dict(labels=y.t().contiguous().t()), dict(reference=ref[:, :, :49].contiguous()),
+                dict(reference=ref.half()), dict(mask=mask.float()), dict(mask=mask[:, :2].contiguous()), dict(list_weights=w[:2]),
+                dict(list_weights=w.double()), dict(kind='other')):
+        for call in (P.preference_loss, P.preference_loss_and_grad):
+            with pytest.raises(ValueError):
+                call(**dict(dict(log_probs=lp, labels=y, reference=ref, mask=mask, list_weights=w), **bad))
+    for bad in ((coef.double(), mask, 50), (coef[0], mask, 50), (coef, mask, 49), (coef, mask.float(), 50), (coef, mask, 50, up[:3]),
+                (coef, mask, 50, up.double()), (coef, None, -1), (coef.repeat(1, 22), None, 50)):
+        with pytest.raises(ValueError):
+            P.preference_grad(*bad)

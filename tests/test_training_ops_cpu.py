@@ -108,6 +108,17 @@ def test_cpu_tensors_are_refused():
         optim.dequantize_exp_avg(torch.zeros(128, dtype=torch.int8), torch.zeros(1))
 
 
+def test_raw_preference_calls_refuse_cpu_tensors():
+    from ranking_amd import _lib, preference
+    lp, y = torch.zeros(2, 3, 4), torch.zeros(2, 3)
+    for bad in (lambda: preference.preference_loss(lp, y), lambda: preference.preference_loss_and_grad(lp, y), lambda: preference.preference_grad(y, None, 4)):
+        with pytest.raises(_lib.TfrHipError):
+            bad()
+    for bad in (lambda: preference.preference_loss(lp, y, kind='other'), lambda: preference.preference_loss_and_grad(lp, y, kind=None)):
+        with pytest.raises(ValueError):
+            bad()
+
+
 @pytest.mark.parametrize('kw', [dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1.0), dict(weight_decay=-1.0),
                                 dict(state_bits=16), dict(lr=torch.tensor(0.1))])
 def test_adamw_hyperparameters(kw):
