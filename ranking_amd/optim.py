@@ -161,6 +161,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                 if rc:
                     _lib.check(rc, name)
                 at = end
+    try:                                                       # a graph that saved a parameter must not go backward any more
+        torch.autograd.graph.increment_version(params)
+    except RuntimeError:                                       # inference tensors have no version
+        for p in params:
+            if not p.is_inference():
+                torch.autograd.graph.increment_version(p)
 
 
 def _dequantize(codes, scales, dtype, square):

@@ -387,3 +387,19 @@ def test_refusals():
     with pytest.raises(ValueError):
         O().AdamW([sparse]).step()
     assert math.isfinite(p.sum().item())
+
+
+def test_stale_graphs_are_refused():
+    """A step changes the parameters that an earlier graph saved: its backward raises instead of mixing old and new values."""
+    w = torch.nn.Parameter(torch.ones(4, 4, device=DEV))
+    x = torch.ones(2, 4, device=DEV, requires_grad=True)
+    opt = O().AdamW([w], lr=0.1)
+    loss = (x @ w).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    with torch.inference_mode():                                           # tensors without a version are stepped all the same
+        a, b = torch.ones(3, device=DEV), torch.zeros(3, device=DEV)
+        O().adamw_step([a], [torch.ones_like(a)], [b], [torch.zeros_like(a)], step=1, lr=0.1, weight_decay=0.0)
+        assert torch.allclose(a, torch.full_like(a, 0.9), atol=1e-6)
