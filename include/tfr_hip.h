@@ -658,6 +658,8 @@ long tfr_preference_workspace_bytes(int B, int L, int T);
 int tfr_preference_loss_f32(const float* log_probs, const float* reference, const uint8_t* mask, const float* labels,
                             const float* list_weights, int B, int L, int T, int kind, float beta, float smoothing,
                             int normalize, float scale, float* loss, float* coef, void* workspace, long workspace_bytes, void* stream);
+/* total[0] = sum of loss [B] (16-byte aligned) in fp64, rounded once. */
+int tfr_preference_total_f32(const float* loss, int B, float* total, void* stream);
 int tfr_preference_grad_f32(const float* coef, const float* upstream, const uint8_t* mask, int B, int L, int T,
                             float* dlog_probs, void* stream);
 /* Both at once: total[0] = sum of the lists' losses, dlog_probs its gradient; lists of up to 8192 tokens in all go from their

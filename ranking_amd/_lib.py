@@ -183,6 +183,7 @@ _SIGNATURES = {
                                 + [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p] + _WS),
     'tfr_preference_loss_and_grad_f32': (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int] * 4 + [ctypes.c_float] * 2
                                          + [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p] + _WS),
+    'tfr_preference_total_f32': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
     'tfr_preference_grad_f32': (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2),
     # optimizer (adamw.hip): pointer tables live in host memory
     'tfr_adamw': (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_void_p] * 5 + [ctypes.c_double] * 5

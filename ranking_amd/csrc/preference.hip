@@ -398,6 +398,12 @@ extern "C" int tfr_preference_loss_f32(const float* log_probs, const float* refe
   return (int)hipGetLastError();
 }
 
+extern "C" int tfr_preference_total_f32(const float* loss, int B, float* total, void* stream) {
+  if (B < 0 || B > kMostAnswers || !total || (B > 0 && !loss) || !aligned(loss, 16)) return TFR_EINVAL;
+  preference_total_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(loss, B, total);
+  return (int)hipGetLastError();
+}
+
 extern "C" int tfr_preference_grad_f32(const float* coef, const float* upstream, const uint8_t* mask, int B, int L, int T, float* dlog_probs,
                                        void* stream) {
   if (bad_sizes(B, L, T)) return TFR_EINVAL;

@@ -853,13 +853,12 @@ class PreferenceLoss(_RankingLoss):
 
     def __call__(self, y_true, y_pred, sample_weight=None, reference=None, mask=None):
         y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred, sample_weight, reference, mask)
-        losses = _preference._PreferenceFn.apply(y_pred, y_true, reference, mask, weight, how)
-        return losses if self.reduction == Reduction.NONE else losses.sum()
+        return _preference._PreferenceFn.apply(y_pred, y_true, reference, mask, weight, how, self.reduction != Reduction.NONE)
 
     def call(self, y_true, y_pred):
         """The unreduced losses, one a list."""
         y_pred, y_true, reference, mask, weight, how = self._args(y_true, y_pred, None, None, None)
-        return _preference._PreferenceFn.apply(y_pred, y_true, reference, mask, weight, dict(how, scale=1.0))
+        return _preference._PreferenceFn.apply(y_pred, y_true, reference, mask, weight, dict(how, scale=1.0), False)
 
     def loss_and_grad(self, y_true, y_pred, sample_weight=None, reference=None, mask=None):
         """(scalar loss, d loss / d y_pred in y_pred's shape, float32) without an autograd graph."""

@@ -235,16 +235,28 @@ def _grad(coef, mask, tokens, upstream):
     return out
 
 
+def _total(loss):
+    index = loss.get_device()
+    with _ops.device_of(index):
+        total = loss.new_empty(())
+        rc = _lib.load().tfr_preference_total_f32(loss.data_ptr(), loss.shape[0], total.data_ptr(), _raw_stream(index))
+    if rc:
+        _lib.check(rc, 'tfr_preference_total_f32')
+    return total
+
+
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, log_probs, labels, reference, mask, list_weights, how):
+    def forward(ctx, log_probs, labels, reference, mask, list_weights, how, total):
         loss, coef = _loss(log_probs, labels, reference, mask, list_weights, **how)
         ctx.save_for_backward(coef, *([] if mask is None else [mask]))
-        ctx.tokens = log_probs.shape[2]
-        return loss
+        ctx.tokens, ctx.total = log_probs.shape[2], total
+        return _total(loss) if total else loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         coef, *mask = ctx.saved_tensors
-        return _grad(coef, mask[0] if mask else None, ctx.tokens, g.contiguous()), None, None, None, None, None
+        if ctx.total:
+            g = g.expand(coef.shape[0])
+        return (_grad(coef, mask[0] if mask else None, ctx.tokens, g.contiguous()),) + (None,) * 6

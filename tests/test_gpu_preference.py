@@ -256,3 +256,25 @@ def test_raw_calls():
                 (coef, mask, 50, up.double()), (coef, None, -1), (coef.repeat(1, 22), None, 50)):
         with pytest.raises(ValueError):
             P.preference_grad(*bad)
+
+
+@pytest.mark.parametrize('B,tokens', [(1, 3), (40001, 2), (2, 9000)])
+def test_the_scalar_of_both_paths_and_in_a_graph(B, tokens):
+    """At sizes where __call__ and loss_and_grad take the same sums the scalars are the same bits, eager and on every replay."""
+    y, lp, ref, mask, w = (t.to(DEV) for t in make(B, 2, tokens, graded=False))
+    loss = K().PreferenceLoss(label_smoothing=0.1)
+    p = lp.clone().requires_grad_()
+    out = loss(y, p, w, reference=ref, mask=mask)
+    out.backward()
+    total, grad = loss.loss_and_grad(y, lp, w, reference=ref, mask=mask)
+    assert out.shape == () and torch.equal(out, total) and torch.equal(p.grad, grad)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(g):
+        held = loss(y, lp, w, reference=ref, mask=mask)
+    for _ in range(4):
+        lp.uniform_(-4, 0)
+        g.replay()
+        total, _ = loss.loss_and_grad(y, lp, w, reference=ref, mask=mask)
+        torch.cuda.synchronize()
+        assert torch.equal(held, total)

@@ -138,6 +138,70 @@ def test_training_step_in_a_graph():
     assert torch.equal(results[0][1], results[1][1]) and torch.equal(results[0][2], results[1][2])
 
 
+def work_of(seed, dtype):
+    """One of two programs that run at the same time: its inputs, and a call that gives the outputs of every operator on them."""
+    from ranking_amd import optim, preference
+    from ranking_amd.embedding import embedding_grad, embedding_lookup
+    from ranking_amd.keras.losses import PreferenceLoss
+    g = torch.Generator().manual_seed(seed)
+    vocab, dim, n = 5000 + seed, 40, 9000
+    table = torch.randn(vocab, dim, generator=g).to(dtype).to(DEV)
+    ids = torch.randint(-1, vocab, (n,), generator=g).to(DEV)
+    bags = torch.randint(-1, vocab, (600, 7), generator=g).to(DEV)
+    logits = torch.randn(6, 40000, generator=g).to(dtype).to(DEV)
+    targets = torch.randint(-1, 40000, (6,), generator=g).to(DEV)
+    up, loss = torch.randn(6, generator=g).to(DEV), PreferenceLoss(beta=0.5)
+    lp = (-torch.rand(3, 2, 6000, generator=g)).to(DEV)
+    y = torch.tensor([[1.0, 0.0]] * 3, device=DEV)
+
+    def run():
+        rows = embedding_lookup(table, ids, 2.0)
+        means = embedding_lookup(table, bags, combiner='mean')
+        logp, stats = preference.token_log_probs_with_stats(logits, targets)
+        param, m, v = table.clone(), torch.zeros(table.shape, device=DEV), torch.zeros(table.shape, device=DEV)
+        grad = embedding_grad(rows, ids, vocab, 2.0)
+        optim.adamw_step([param], [grad], [m], [v], step=1, lr=0.1)
+        codes, blocks = optim.quantized_size(param.numel())
+        m8 = torch.zeros(codes, dtype=torch.int8, device=DEV), torch.zeros(blocks, device=DEV)
+        v8 = torch.zeros(codes, dtype=torch.uint8, device=DEV), torch.zeros(blocks, device=DEV)
+        optim.adamw_step([param], [grad], [m8], [v8], step=1, lr=0.1)
+        return [rows, means, grad, embedding_grad(means, bags, vocab, combiner='mean'), logp,
+                preference.token_log_probs_grad(up, logits, targets, stats), *loss.loss_and_grad(y, lp), param, m, v, *m8, *v8]
+    return run
+
+
+@pytest.mark.parametrize('threads', [False, True])
+def test_two_programs_at_once(threads):
+    """Two streams, driven by one thread or by one each, run every operator on inputs of their own: the same bits as alone."""
+    import threading
+    work = [work_of(1, torch.float32), work_of(2, torch.bfloat16)]
+    want = [run() for run in work]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in work], [[], []]
+
+    def drive(k):
+        with torch.cuda.stream(streams[k]):
+            got[k].append(work[k]())
+    if threads:
+        def many(k):
+            for _ in range(5):
+                drive(k)
+        both = [threading.Thread(target=many, args=(k,)) for k in range(2)]
+        for t in both:
+            t.start()
+        for t in both:
+            t.join()
+    else:
+        for _ in range(5):
+            drive(0)
+            drive(1)
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert len(got[k]) == 5
+        for outs in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[k]))
+
+
 @pytest.mark.parametrize('optimizer', ['adamw', 'adamw_8bit'])
 @pytest.mark.parametrize('loss', ['softmax_loss', 'preference_loss'])
 def test_pipeline_with_embedded_features(tmp_path, optimizer, loss):

@@ -71,6 +71,9 @@ def test_preference_arguments_are_checked_before_any_launch():
     assert call(B=0) == 0
     assert g(None, None, None, 2, 3, 5, one, None) == -1 and g(one, None, None, 2, 3, 0, None, None) == 0
     assert _lib.load().tfr_preference_workspace_bytes(1 << 24, 2, 1) < 0
+    h = _lib.load().tfr_preference_total_f32
+    assert h(None, 2, one, None) == -1 and h(one, 2, None, None) == -1 and h(one, -1, one, None) == -1 and h(one, 1 << 24, one, None) == -1
+    assert h(ctypes.c_void_p(260), 2, one, None) == -1
 
 
 def test_adamw_arguments_are_checked_before_any_launch():
