@@ -190,7 +190,7 @@ __device__ __forceinline__ void prepare_rows(const Prepare& p, const Id* __restr
 // Workgroup 0 sorts up to SMALL_SORT (id, position) pairs, 8 bits a pass; the others prepare the rows.
 template <typename Id>
 __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __restrict__ ids, int n, int rows, int bits, int per_bag, const Prepare prep,
-                                                                    int* __restrict__ keys_out, int* __restrict__ pos_out) {
+                                                                    int2* __restrict__ out) {
   if (blockIdx.x > 0) {
     prepare_rows(prep, ids, blockIdx.x - 1, gridDim.x - 1);
     return;
@@ -239,10 +239,7 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int i = wave * 256 + k * 64 + lane;
-    if (i < n) {
-      keys_out[i] = (int)(item[k] >> 32);
-      pos_out[i] = (int)((uint32_t)item[k] / (uint32_t)per_bag);
-    }
+    if (i < n) out[i] = make_int2((int)(item[k] >> 32), (int)((uint32_t)item[k] / (uint32_t)per_bag));
   }
 }
 
@@ -250,10 +247,12 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const Id* __
 // the scatter, in which a tile adds up the counts of the tiles before it by itself (counts[bin][tile], `pitch` apart) while
 // there are few tiles.  The last pass turns positions into bags (per_bag > 1).  FIRST: the keys are the ids themselves, the
 // positions their indexes, and the workgroups behind the tiles prepare the rows.
-// Bound by latency (a pass is two or three launches of a few dependent round trips): two passes take 24 us at 16 384 lookups, 37 at
-// 262 144, 45 at 819 200.
+// An id and its position move as one 8-byte item: a tile's items scatter one by one, and it is the number of accesses that counts
+// (819 200 lookups: 11 + 9 us the two scatters, 15 + 11 with an array each).
+// Bound by latency (a pass is two or three launches of a few dependent round trips): two passes take 24 us at 16 384 lookups, 36 at
+// 262 144, 41 at 819 200.
 template <typename Id, bool FIRST>
-__global__ __launch_bounds__(256) void embedding_digits_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, int n, int rows, int tiles,
+__global__ __launch_bounds__(256) void embedding_digits_kernel(const Id* __restrict__ ids, const int2* __restrict__ items, int n, int rows, int tiles,
                                                                 int subs, int shift, int bits, int pitch, const Prepare prep, int* __restrict__ counts) {
   if (FIRST && (int)blockIdx.x >= tiles) {
     prepare_rows(prep, ids, blockIdx.x - tiles, gridDim.x - tiles);
@@ -268,7 +267,7 @@ __global__ __launch_bounds__(256) void embedding_digits_kernel(const Id* __restr
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       const long i = base + k * blockDim.x + threadIdx.x;
-      if (i < n) atomicAdd(&s_bins[((FIRST ? id_key(ids, i, rows) : keys[i]) >> shift) & (bins - 1)], 1);
+      if (i < n) atomicAdd(&s_bins[((FIRST ? id_key(ids, i, rows) : items[i].x) >> shift) & (bins - 1)], 1);
     }
   }
   __syncthreads();
@@ -301,26 +300,25 @@ __global__ __launch_bounds__(64) void embedding_scan_kernel(int* __restrict__ co
 }
 
 template <typename Id, bool FIRST>
-__global__ __launch_bounds__(256) void embedding_scatter_kernel(const Id* __restrict__ ids, const int* __restrict__ keys, const int* __restrict__ pos,
-                                                                 int n, int rows, int subs, int shift, int bits, int pitch, int per_bag,
+__global__ __launch_bounds__(256) void embedding_scatter_kernel(const Id* __restrict__ ids, const int2* __restrict__ items, int n,
+                                                                 int rows, int subs, int shift, int bits, int pitch, int per_bag,
                                                                  const int* __restrict__ counts, const int* __restrict__ totals,
-                                                                 int* __restrict__ keys_out,
-                                                                 int* __restrict__ pos_out) {
+                                                                 int2* __restrict__ out) {
   extern __shared__ int s_count[];                              // [waves][bins], the 16 ints of the prefix sum, the next place of each bin [bins]
   const int bins = 1 << bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   int* red = s_count + waves * bins;
   int* next = red + 16;
   const int per = bins > (int)blockDim.x ? bins / blockDim.x : 1;        // bins of a thread: 1, 2 or 4, neighbours
-  const auto load_keys = [&](int sub, int (&key)[ITEMS]) {
+  const auto load_items = [&](int sub, int2 (&item)[ITEMS]) {
     const long base = ((long)blockIdx.x * subs + sub) * ((long)blockDim.x * ITEMS) + wave * (64 * ITEMS);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       const long i = base + k * 64 + lane;
-      key[k] = i < n ? (FIRST ? id_key(ids, i, rows) : keys[i]) : -1;
+      item[k] = i >= n ? make_int2(-1, 0) : FIRST ? make_int2(id_key(ids, i, rows), (int)i) : items[i];
     }
   };
-  int key[ITEMS];
-  load_keys(0, key);                                            // under way while the counts are added up
+  int2 item[ITEMS];
+  load_items(0, item);                                            // under way while the counts are added up
   int before[4] = {0, 0, 0, 0}, total[4] = {0, 0, 0, 0};
   if (totals) {
 #pragma unroll
@@ -360,16 +358,10 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(const Id* __rest
   for (int sub = 0; sub < subs; ++sub) {
     for (int i = tid; i < waves * bins; i += blockDim.x) s_count[i] = 0;
     __syncthreads();
-    const long base = ((long)blockIdx.x * subs + sub) * ((long)blockDim.x * ITEMS) + wave * (64 * ITEMS);
-    int place[ITEMS], from[ITEMS];
-    if (sub > 0) load_keys(sub, key);
+    int place[ITEMS];
+    if (sub > 0) load_items(sub, item);
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const long i = base + k * 64 + lane;
-      from[k] = FIRST || i >= n ? (int)i : pos[i];
-    }
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) place[k] = wave_place((key[k] >> shift) & (bins - 1), bits, key[k] >= 0, s_count + wave * bins);
+    for (int k = 0; k < ITEMS; ++k) place[k] = wave_place((item[k].x >> shift) & (bins - 1), bits, item[k].x >= 0, s_count + wave * bins);
     __syncthreads();
     for (int b = tid; b < bins; b += blockDim.x) {
       int p = next[b];
@@ -383,10 +375,9 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(const Id* __rest
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      if (key[k] < 0) continue;
-      const int to = s_count[wave * bins + ((key[k] >> shift) & (bins - 1))] + place[k];
-      keys_out[to] = key[k];
-      pos_out[to] = per_bag > 1 ? (int)((unsigned)from[k] / (unsigned)per_bag) : from[k];
+      if (item[k].x < 0) continue;
+      const int to = s_count[wave * bins + ((item[k].x >> shift) & (bins - 1))] + place[k];
+      out[to] = make_int2(item[k].x, per_bag > 1 ? (int)((unsigned)item[k].y / (unsigned)per_bag) : item[k].y);
     }
     __syncthreads();
   }
@@ -394,8 +385,7 @@ __global__ __launch_bounds__(256) void embedding_scatter_kernel(const Id* __rest
 
 // ------------------------------------------------------------------------------------------------ gradient
 struct GradArgs {
-  const int* keys;                      // [n] sorted ids; rows: no gradient
-  const int* pos;                       // [n] the bag that each came from
+  const int2* items;                    // [n] sorted ids (rows: no gradient), and the bag that each came from
   const float* factor;                  // [bags] or null: scale for all
   int* first;                           // [rows] where a row's run begins, -1: no occurrence
   int* last;                            // [rows] where it ends (rows with an occurrence)
@@ -427,8 +417,8 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, c
   const int lo = (int)begin, hi = a.n - lo < (1 << a.chunk_log2) ? a.n : lo + (1 << a.chunk_log2);
   const int c = (column << a.lanes_log2) + lane;
   const bool on = c < a.dim / E, scribe = lane == 0 && column == 0;
-  int row = a.keys[lo], start = lo;
-  bool began_before = lo > 0 && a.keys[lo - 1] == row;
+  int row = a.items[lo].x, start = lo;
+  bool began_before = lo > 0 && a.items[lo - 1].x == row;
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -449,13 +439,10 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, c
       put_row<T, E, STREAM>(static_cast<T*>(a.out) + (long)row * a.dim + (long)c * E, v);
     }
   };
-  int next_key[8], next_bag[8];
+  int2 next[8];
   const auto load_ids = [&](int i) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      next_key[k] = i + k < hi ? a.keys[i + k] : a.rows;
-      next_bag[k] = i + k < hi ? a.pos[i + k] : 0;
-    }
+    for (int k = 0; k < 8; ++k) next[k] = i + k < hi ? a.items[i + k] : make_int2(a.rows, 0);
   };
   load_ids(lo);
   for (int i = lo; i < hi; i += 8) {
@@ -464,11 +451,11 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, c
     float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      key[k] = next_key[k];
+      key[k] = next[k].x;
       if (key[k] < a.rows && on) {
-        const T* at = grad + (long)next_bag[k] * a.dim + (long)c * E;
+        const T* at = grad + (long)next[k].y * a.dim + (long)c * E;
         raw[k] = ONCE ? load_raw_stream<T, E>(at) : load_raw<T, E>(at);
-        f[k] = a.factor ? a.factor[next_bag[k]] : 1.f;
+        f[k] = a.factor ? a.factor[next[k].y] : 1.f;
       }
     }
     if (i + 8 < hi) load_ids(i + 8);                            // under way with the rows
@@ -491,7 +478,7 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, c
       }
     }
   }
-  finish(hi, hi < a.n && a.keys[hi] == row);
+  finish(hi, hi < a.n && a.items[hi].x == row);
 }
 
 // Adds the partial sums of a run from sorted position s to e: that of its first chunk and those of the chunks behind it, the
@@ -556,8 +543,8 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const GradArgs a, i
   // the run of the last occurrence of chunk q, if it begins there and goes on
   const long border = (((long)blockIdx.x * groups + group) + 1) << a.chunk_log2;
   if (border < a.n) {
-    const int row = a.keys[border - 1];
-    if (row < a.rows && a.keys[border] == row) {
+    const int row = a.items[border - 1].x;
+    if (row < a.rows && a.items[border].x == row) {
       const int s = a.first[row], e = a.last[row];
       if ((long)s >= border - (1l << a.chunk_log2)) {
         if (((e - 1) >> a.chunk_log2) - (s >> a.chunk_log2) >= LONG_RUN) {
@@ -615,7 +602,7 @@ int pack_elems(int dtype, int dim, long ld, const void* p, const void* q) {
 }
 
 struct Sizes {
-  long keys, pos, keys2, pos2, counts, factor, first, last, parts, total;   // byte offsets
+  long items, items2, counts, factor, first, last, parts, total;   // byte offsets
   int tiles, pitch, subs, digit, passes, bits, chunk_log2;
 };
 
@@ -639,11 +626,9 @@ Sizes sizes_of(long n, long bags, long rows, int dim, bool mean) {
   while (s.chunk_log2 < (n <= (1 << 20) ? 6 : 7) && (2l << s.chunk_log2) * 131072 <= n * lanes) ++s.chunk_log2;
   long at = 0;
   auto take = [&at](long bytes) { const long p = at; at += (bytes + 255) / 256 * 256; return p; };
-  s.keys = take(4 * n);
-  s.pos = take(4 * n);
+  s.items = take(8 * n);
   const bool large = n > SMALL_SORT;
-  s.keys2 = take(large ? 4 * n : 0);
-  s.pos2 = take(large ? 4 * n : 0);
+  s.items2 = take(large ? 8 * n : 0);
   s.counts = take(large ? 4l * (s.pitch + 1) << s.digit : 0);
   s.factor = take(mean ? 4 * bags : 0);
   s.first = take(n > 0 ? 4 * rows : 0);
@@ -686,39 +671,36 @@ int launch_lookup_ids(const void* table, long ld, int rows, int dim, const void*
 }
 
 template <typename Id, bool FIRST>
-int launch_pass(const Id* ids, const int* keys, const int* pos, long n, int rows, const Sizes& s, int shift, int per_bag, const Prepare& prep,
-                int extra, int* counts, int* keys_out, int* pos_out, hipStream_t stream) {
+int launch_pass(const Id* ids, const int2* items, long n, int rows, const Sizes& s, int shift, int per_bag, const Prepare& prep,
+                int extra, int* counts, int2* out, hipStream_t stream) {
   const size_t lds = (5 * (size_t)(1 << s.digit) + 16) * sizeof(int);     // at most 10 bits: 20 KB
   int* totals = s.tiles > 32 ? counts + ((long)s.pitch << s.digit) : nullptr;
-  embedding_digits_kernel<Id, FIRST><<<s.tiles + extra, 256, sizeof(int) << s.digit, stream>>>(ids, keys, (int)n, rows, s.tiles, s.subs, shift,
+  embedding_digits_kernel<Id, FIRST><<<s.tiles + extra, 256, sizeof(int) << s.digit, stream>>>(ids, items, (int)n, rows, s.tiles, s.subs, shift,
                                                                                                      s.digit, s.pitch, prep, counts);
   if (totals) embedding_scan_kernel<<<1 << s.digit, 64, 0, stream>>>(counts, s.tiles, s.pitch, totals);
-  embedding_scatter_kernel<Id, FIRST><<<s.tiles, 256, lds, stream>>>(ids, keys, pos, (int)n, rows, s.subs, shift, s.digit, s.pitch, per_bag,
-                                                                           counts, totals, keys_out, pos_out);
+  embedding_scatter_kernel<Id, FIRST><<<s.tiles, 256, lds, stream>>>(ids, items, (int)n, rows, s.subs, shift, s.digit, s.pitch, per_bag,
+                                                                           counts, totals, out);
   return (int)hipGetLastError();
 }
 
 template <typename Id>
-int launch_sort(const Id* ids, long n, int rows, const Sizes& s, char* ws, const Prepare& prep, int** keys, int** pos, hipStream_t stream) {
-  int* k[2] = {(int*)(ws + s.keys), (int*)(ws + s.keys2)};
-  int* p[2] = {(int*)(ws + s.pos), (int*)(ws + s.pos2)};
+int launch_sort(const Id* ids, long n, int rows, const Sizes& s, char* ws, const Prepare& prep, int2** sorted, hipStream_t stream) {
+  int2* items[2] = {(int2*)(ws + s.items), (int2*)(ws + s.items2)};
   long extra = 1 + prep.rows / 4096;                             // workgroups that prepare the rows
   if (prep.factor && extra < prep.bags / 16) extra = prep.bags / 16;
   if (extra > 2048) extra = 2048;
   if (n <= SMALL_SORT) {
-    embedding_sort_small_kernel<Id><<<1 + (unsigned)extra, 1024, 0, stream>>>(ids, (int)n, rows, s.bits, prep.tokens, prep, k[0], p[0]);
-    *keys = k[0];
-    *pos = p[0];
+    embedding_sort_small_kernel<Id><<<1 + (unsigned)extra, 1024, 0, stream>>>(ids, (int)n, rows, s.bits, prep.tokens, prep, items[0]);
+    *sorted = items[0];
     return (int)hipGetLastError();
   }
   int* counts = (int*)(ws + s.counts);
-  int rc = launch_pass<Id, true>(ids, nullptr, nullptr, n, rows, s, 0, s.passes == 1 ? prep.tokens : 1, prep, (int)extra, counts, k[0], p[0], stream);
+  int rc = launch_pass<Id, true>(ids, nullptr, n, rows, s, 0, s.passes == 1 ? prep.tokens : 1, prep, (int)extra, counts, items[0], stream);
   int from = 0;
   for (int pass = 1; pass < s.passes && rc == TFR_OK; ++pass, from ^= 1)
-    rc = launch_pass<Id, false>(ids, k[from], p[from], n, rows, s, pass * s.digit, pass + 1 == s.passes ? prep.tokens : 1, prep, 0, counts, k[from ^ 1],
-                                p[from ^ 1], stream);
-  *keys = k[from];
-  *pos = p[from];
+    rc = launch_pass<Id, false>(ids, items[from], n, rows, s, pass * s.digit, pass + 1 == s.passes ? prep.tokens : 1, prep, 0, counts, items[from ^ 1],
+                                stream);
+  *sorted = items[from];
   return rc;
 }
 
@@ -814,12 +796,11 @@ extern "C" int tfr_embedding_grad(const void* grad, int dtype, const void* ids, 
     a.first = (int*)(ws + s.first);
     a.last = (int*)(ws + s.last);
     const Prepare prep = {a.first, factor, bags, a.rows, tokens, scale};
-    int *keys = nullptr, *pos = nullptr;
-    rc = id_type == TFR_IDS_I32 ? launch_sort<int32_t>((const int32_t*)ids, n, a.rows, s, ws, prep, &keys, &pos, st)
-                                : launch_sort<int64_t>((const int64_t*)ids, n, a.rows, s, ws, prep, &keys, &pos, st);
+    int2* items = nullptr;
+    rc = id_type == TFR_IDS_I32 ? launch_sort<int32_t>((const int32_t*)ids, n, a.rows, s, ws, prep, &items, st)
+                                : launch_sort<int64_t>((const int64_t*)ids, n, a.rows, s, ws, prep, &items, st);
     if (rc != TFR_OK) return rc;
-    a.keys = keys;
-    a.pos = pos;
+    a.items = items;
     a.parts = (float*)(ws + s.parts);
     a.chunk_log2 = s.chunk_log2;
   }
