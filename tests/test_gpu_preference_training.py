@@ -124,7 +124,7 @@ def test_training_step_in_a_graph():
             with torch.cuda.graph(graph):
                 out = step()
         losses = []
-        for k in range(4):
+        for k in range(10):                                                # 0, 1 and 3 hold no pair: those steps only decay
             for h, t in zip(held, batch(vocab, 4, 2, 11, k)):
                 h.copy_(t)
             if captured:
@@ -136,6 +136,45 @@ def test_training_step_in_a_graph():
         results.append((losses, table.detach().clone(), weight.detach().clone()))
     assert results[0][0] == results[1][0]
     assert torch.equal(results[0][1], results[1][1]) and torch.equal(results[0][2], results[1][2])
+
+
+def test_autograd_in_a_graph():
+    """Forward and autograd.grad captured together (every graph before it is gone), replayed on new batches = eager."""
+    from ranking_amd import preference
+    from ranking_amd.embedding import embedding_lookup
+    from ranking_amd.keras.losses import PreferenceLoss
+    vocab, dim = 97, 16
+    g = torch.Generator().manual_seed(3)
+    table, weight = ((torch.randn(vocab, dim, generator=g) * 0.2).to(DEV).requires_grad_() for _ in range(2))
+    loss_fn = PreferenceLoss(beta=0.5)
+    held = [t.to(DEV) for t in batch(vocab, 4, 2, 11, 0)]
+
+    def step():
+        logits = embedding_lookup(table, held[0], 4.0) @ weight.t()
+        loss = loss_fn(held[3], preference.token_log_probs(logits, held[1]), mask=held[2])
+        return [loss.detach(), *torch.autograd.grad(loss, [table, weight])]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    pairs = 0
+    for k in range(10):
+        new = batch(vocab, 4, 2, 11, k)
+        for h, t in zip(held, new):
+            h.copy_(t)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        y = new[3]
+        has = bool(((y[:, 0] != y[:, 1]) & (y >= 0).all(1)).any())          # without a pair the loss is 0 and so are its gradients
+        assert all(torch.equal(a, b) for a, b in zip(out, want)) and bool(want[1].any()) == bool(want[2].any()) == has
+        pairs += has
+    assert pairs >= 3
 
 
 def work_of(seed, dtype):
