@@ -272,23 +272,23 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise ValueError('AdamW does not take sparse gradients')
                 s = self._state_of(p, group)
-                if group['capturable']:
-                    t = 1
-                else:
-                    t = s['step'] = s['step'] + 1
+                t = 1 if group['capturable'] else s['step'] + 1
                 m, v = s['exp_avg'], s['exp_avg_sq']
-                runs.setdefault(t, []).append((p, p.grad.contiguous(), (m, s['exp_avg_scale']) if eight else m,
+                runs.setdefault(t, []).append((s, p, p.grad.contiguous(), (m, s['exp_avg_scale']) if eight else m,
                                                (v, s['exp_avg_sq_scale']) if eight else v))
             if not runs:
                 continue
             lr, now = group['lr'], None
             if group['capturable']:
-                now = self._advance(group, next(iter(runs.values()))[0][0].device)
+                now = self._advance(group, next(iter(runs.values()))[0][1].device)
             elif torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: a step inside a stream capture needs capturable=True (the step count would be frozen)')
             for t, items in runs.items():
-                p, g, m, v = zip(*items)
+                states, p, g, m, v = zip(*items)
                 adamw_step(p, g, m, v, step=t, lr=lr, betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'], now=now)
+                if not group['capturable']:
+                    for s in states:                           # counted once it is launched: a step that is refused is none
+                        s['step'] = t
         return loss
 
     def _advance(self, group, device):

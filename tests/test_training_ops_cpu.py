@@ -234,3 +234,30 @@ def test_plain_adamw_against_torch():
         opt.step()
         mine, m, v, *_ = T.adamw(mine, grad, m, v, step, 0.01, (0.8, 0.99), 1e-8, 0.1)
         assert torch.allclose(mine, theirs.detach(), rtol=1e-12, atol=1e-14)
+
+
+# ---------------------------------------------------------------- the optimizer's state
+def held_state(p, step, bits=32):
+    """The state of a parameter that took `step` steps, on the parameter's device (init_state() makes it on a GPU only)."""
+    if bits == 32:
+        return {'exp_avg': torch.full(p.shape, 0.5), 'exp_avg_sq': torch.full(p.shape, 0.25), 'step': step}
+    codes, blocks = optim.quantized_size(p.numel())
+    return {'exp_avg': torch.full((codes,), 3, dtype=torch.int8), 'exp_avg_sq': torch.full((codes,), 5, dtype=torch.uint8),
+            'exp_avg_scale': torch.full((blocks,), 0.5), 'exp_avg_sq_scale': torch.full((blocks,), 0.25), 'step': step}
+
+
+def test_a_refused_step_is_not_counted(monkeypatch):
+    """A step that raises before it is launched (tensors that are refused, a capture that would freeze the count) leaves the
+    counts: the next step's corrections are those of the steps that were taken."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = optim.AdamW([p])
+    opt.state[p] = held_state(p, 2)
+    p.grad = torch.ones(3)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    with pytest.raises(_lib.TfrHipError):                                   # not on a GPU
+        opt.step()
+    assert opt.state[p]['step'] == 2
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(RuntimeError, match='capturable'):
+        opt.step()
+    assert opt.state[p]['step'] == 2
