@@ -688,6 +688,16 @@ int tfr_adamw8(int dtype, int count, void* const* params_host, const void* const
  * lr_device when given: a step that is replayed from a hipGraph keeps counting and follows its learning rate. */
 int tfr_adamw_advance(int64_t* step, const float* lr_device, double lr, double beta1, double beta2, double weight_decay,
                       float* now, void* stream);
+/* Both with a count on the device for every tensor: steps_host holds device pointers, one int64 a tensor, no two the same; `all`
+ * (nullable) is one more count that is advanced once.  now [3 * count]: device workspace, 4-byte aligned. */
+int tfr_adamw_counted(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+                      void* const* exp_avg_sqs_host, const int64_t* sizes_host, int64_t* const* steps_host, int64_t* all,
+                      const float* lr_device, double lr, double beta1, double beta2, double eps, double weight_decay, float* now,
+                      void* stream);
+int tfr_adamw8_counted(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+                       float* const* exp_avg_scales_host, void* const* exp_avg_sqs_host, float* const* exp_avg_sq_scales_host,
+                       const int64_t* sizes_host, int64_t* const* steps_host, int64_t* all, const float* lr_device, double lr,
+                       double beta1, double beta2, double eps, double weight_decay, float* now, void* stream);
 /* out[i] = codes[i] * scale (square: its square): what the 8-bit moments stand for; n a multiple of TFR_ADAMW_QBLOCK. */
 int tfr_adamw_dequantize(const void* codes, const float* scales, long n, int square, float* out, void* stream);
 

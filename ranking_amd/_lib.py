@@ -190,6 +190,8 @@ _SIGNATURES = {
                   + [ctypes.c_int64] + [ctypes.c_void_p] * 2),
     'tfr_adamw8': (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_void_p] * 7 + [ctypes.c_double] * 5
                    + [ctypes.c_int64] + [ctypes.c_void_p] * 2),
+    'tfr_adamw_counted': (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_void_p] * 8 + [ctypes.c_double] * 5 + [ctypes.c_void_p] * 2),
+    'tfr_adamw8_counted': (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_void_p] * 10 + [ctypes.c_double] * 5 + [ctypes.c_void_p] * 2),
     'tfr_adamw_advance': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_double] * 4 + [ctypes.c_void_p] * 2),
     'tfr_adamw_dequantize': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_long, ctypes.c_int] + [ctypes.c_void_p] * 2),
 }

@@ -27,6 +27,7 @@ struct Coef {
   double b1, c1, b2, c2;               // beta and 1 - beta
   float decay, step, root, eps;        // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   const float* now;                    // device (decay, step, root) of a step that is counted on the device, or null
+  int stride;                          // 3: the launch's tensors have their own, one after the other; 0: one for all
 };
 
 template <int CAP, bool Q>
@@ -57,9 +58,12 @@ __device__ __forceinline__ int tensor_of(const Tab& t, int block) {
 }
 
 struct Now { float decay, step, root; };
-__device__ __forceinline__ Now now_of(const Coef& c) {
+__device__ __forceinline__ Now now_of(const Coef& c, int tensor) {
   Now w = {c.decay, c.step, c.root};
-  if (c.now) w = {c.now[0], c.now[1], c.now[2]};
+  if (c.now) {
+    const float* n = c.now + c.stride * tensor;
+    w = {n[0], n[1], n[2]};
+  }
   return w;
 }
 
@@ -90,7 +94,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Table32 t) {
   const T* __restrict__ g = (const T*)t.g[i] + base;
   float* __restrict__ m = (float*)t.m[i] + base;
   float* __restrict__ v = (float*)t.v[i] + base;
-  const Now w = now_of(t.coef);
+  const Now w = now_of(t.coef, i);
   const float b1 = (float)t.coef.b1, c1 = (float)t.coef.c1, b2 = (float)t.coef.b2, c2 = (float)t.coef.c2, eps = t.coef.eps;
   const int left = (int)(n - base < BLOCK32 ? n - base : BLOCK32);
   const bool wide = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0;
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const Table8 t) {
   uint8_t* __restrict__ v = (uint8_t*)t.v[i];
   float* __restrict__ ms = t.ms[i];
   float* __restrict__ vs = t.vs[i];
-  const Now w = now_of(t.coef);
+  const Now w = now_of(t.coef, i);
   const double c1 = t.coef.c1, c2 = t.coef.c2;
   const float eps = t.coef.eps;
   const bool tiny_eps = eps < 1e-12f;                          // the fast root takes v below 2^-126 as 0: far below any other eps
@@ -317,14 +321,32 @@ __global__ __launch_bounds__(256) void adamw_dequantize_kernel(const uint8_t* __
 }
 
 // One more step, counted on the device: coefficients of the launch behind it.
-__global__ void adamw_advance_kernel(long* __restrict__ count, const float* __restrict__ lr_now, double lr, double b1, double b2, double decay,
-                                     float* __restrict__ now) {
+__device__ __forceinline__ void advance(long* __restrict__ count, const float* __restrict__ lr_now, double lr, double b1, double b2, double decay,
+                                        float* __restrict__ now) {
   const long t = count[0] + 1;
   count[0] = t;
   if (lr_now) lr = (double)lr_now[0];
   now[0] = (float)(1.0 - lr * decay);
   now[1] = (float)(lr / (1.0 - pow(b1, (double)t)));
   now[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+}
+__global__ void adamw_advance_kernel(long* __restrict__ count, const float* __restrict__ lr_now, double lr, double b1, double b2, double decay,
+                                     float* __restrict__ now) {
+  advance(count, lr_now, lr, b1, b2, decay, now);
+}
+
+// The same where every tensor of the launch has a count of its own (a thread each): a parameter that gets its first gradient late is
+// corrected by the steps that it took.  `all` (or null) counts the steps of them together.
+struct Counts {
+  long* at[TFR_ADAMW_MAX_TENSORS];
+};
+constexpr int COUNT_THREADS = 128;
+static_assert(TFR_ADAMW_MAX_TENSORS <= COUNT_THREADS && TFR_ADAMW8_MAX_TENSORS <= TFR_ADAMW_MAX_TENSORS, "a thread a tensor");
+__global__ __launch_bounds__(COUNT_THREADS) void adamw_advance_each_kernel(const Counts counts, int n, long* __restrict__ all, const float* __restrict__ lr_now,
+                                                                           double lr, double b1, double b2, double decay, float* __restrict__ now) {
+  const int i = threadIdx.x;
+  if (i == 0 && all) all[0] += 1;
+  if (i < n) advance(counts.at[i], lr_now, lr, b1, b2, decay, now + 3 * i);
 }
 
 constexpr long kCache = 256l << 20;
@@ -344,7 +366,7 @@ bool bad_betas(double b1, double b2) { return !(b1 >= 0.0 && b1 < 1.0 && b2 >= 0
 
 template <typename Tab, int PER>
 int fill(Tab& t, int cap, int count, void* const* p, const void* const* g, void* const* m, void* const* v, const int64_t* n, double lr,
-         double b1, double b2, double eps, double decay, int64_t step, const float* now) {
+         double b1, double b2, double eps, double decay, int64_t step, const float* now, int stride) {
   if (count < 1 || count > cap || !p || !g || !m || !v || !n || bad_betas(b1, b2)) return TFR_EINVAL;
   if (!now && step < 1) return TFR_EINVAL;
   t.coef.b1 = b1;
@@ -353,6 +375,7 @@ int fill(Tab& t, int cap, int count, void* const* p, const void* const* g, void*
   t.coef.c2 = 1.0 - b2;
   t.coef.eps = (float)eps;
   t.coef.now = now;
+  t.coef.stride = stride;
   t.coef.decay = (float)(1.0 - lr * decay);
   t.coef.step = now ? 0.f : (float)(lr / (1.0 - __builtin_pow(b1, (double)step)));
   t.coef.root = now ? 0.f : (float)(1.0 / __builtin_sqrt(1.0 - __builtin_pow(b2, (double)step)));
@@ -373,6 +396,51 @@ int fill(Tab& t, int cap, int count, void* const* p, const void* const* g, void*
   return TFR_OK;
 }
 
+template <typename Tab, int PER>
+int fill_scales(Tab& t, int cap, int count, void* const* p, const void* const* g, void* const* m, float* const* ms, void* const* v, float* const* vs,
+                const int64_t* n, double lr, double b1, double b2, double eps, double decay, int64_t step, const float* now, int stride) {
+  if (!ms || !vs) return TFR_EINVAL;
+  const int rc = fill<Tab, PER>(t, cap, count, p, g, m, v, n, lr, b1, b2, eps, decay, step, now, stride);
+  if (rc != TFR_OK) return rc;
+  for (int i = 0; i < count; ++i) {
+    t.ms[i] = ms[i];
+    t.vs[i] = vs[i];
+    if (n[i] > 0 && (!ms[i] || !vs[i] || (((uintptr_t)m[i] | (uintptr_t)v[i]) & 7))) return TFR_EINVAL;
+  }
+  return TFR_OK;
+}
+
+int run(const Table32& t, int dtype, hipStream_t st) {
+  const int blocks = t.first[t.count];
+  if (blocks == 0) return TFR_OK;
+  if (dtype == TFR_DTYPE_F32) launch32<float>(t, blocks, st);
+  else if (dtype == TFR_DTYPE_BF16) launch32<__bf16>(t, blocks, st);
+  else launch32<_Float16>(t, blocks, st);
+  return (int)hipGetLastError();
+}
+int run(const Table8& t, int dtype, hipStream_t st) {
+  const int blocks = t.first[t.count];
+  if (blocks == 0) return TFR_OK;
+  if (dtype == TFR_DTYPE_F32) launch8<float>(t, blocks, st);
+  else if (dtype == TFR_DTYPE_BF16) launch8<__bf16>(t, blocks, st);
+  else launch8<_Float16>(t, blocks, st);
+  return (int)hipGetLastError();
+}
+
+// The counts of a table's tensors are advanced, then the table's launch reads its coefficients.
+template <typename Tab>
+int run_counted(const Tab& t, int dtype, int64_t* const* steps, int64_t* all, const float* lr_device, double lr, double b1, double b2,
+                double decay, float* now, hipStream_t st) {
+  Counts counts = {};
+  for (int i = 0; i < t.count; ++i) {
+    if (!steps[i]) return TFR_EINVAL;
+    counts.at[i] = (long*)steps[i];
+  }
+  adamw_advance_each_kernel<<<1, COUNT_THREADS, 0, st>>>(counts, t.count, (long*)all, lr_device, lr, b1, b2, decay, now);
+  const int rc = (int)hipGetLastError();
+  return rc != TFR_OK ? rc : run(t, dtype, st);
+}
+
 }  // namespace
 
 extern "C" int tfr_adamw(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
@@ -381,38 +449,41 @@ extern "C" int tfr_adamw(int dtype, int count, void* const* params_host, const v
   if (!elem_known(dtype)) return TFR_EINVAL;
   Table32 t;
   const int rc = fill<Table32, BLOCK32>(t, TFR_ADAMW_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_sqs_host, sizes_host,
-                                        lr, beta1, beta2, eps, weight_decay, step, now);
-  if (rc != TFR_OK) return rc;
-  const int blocks = t.first[count];
-  if (blocks == 0) return TFR_OK;
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == TFR_DTYPE_F32) launch32<float>(t, blocks, st);
-  else if (dtype == TFR_DTYPE_BF16) launch32<__bf16>(t, blocks, st);
-  else launch32<_Float16>(t, blocks, st);
-  return (int)hipGetLastError();
+                                        lr, beta1, beta2, eps, weight_decay, step, now, 0);
+  return rc != TFR_OK ? rc : run(t, dtype, (hipStream_t)stream);
 }
 
 extern "C" int tfr_adamw8(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
                           float* const* exp_avg_scales_host, void* const* exp_avg_sqs_host, float* const* exp_avg_sq_scales_host,
                           const int64_t* sizes_host, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
                           const float* now, void* stream) {
-  if (!elem_known(dtype) || !exp_avg_scales_host || !exp_avg_sq_scales_host) return TFR_EINVAL;
+  if (!elem_known(dtype)) return TFR_EINVAL;
   Table8 t;
-  const int rc = fill<Table8, BLOCK8>(t, TFR_ADAMW8_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_sqs_host, sizes_host,
-                                      lr, beta1, beta2, eps, weight_decay, step, now);
-  if (rc != TFR_OK) return rc;
-  for (int i = 0; i < count; ++i) {
-    t.ms[i] = exp_avg_scales_host[i];
-    t.vs[i] = exp_avg_sq_scales_host[i];
-    if (t.n[i] > 0 && (!t.ms[i] || !t.vs[i] || (((uintptr_t)t.m[i] | (uintptr_t)t.v[i]) & 7))) return TFR_EINVAL;
-  }
-  const int blocks = t.first[count];
-  if (blocks == 0) return TFR_OK;
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == TFR_DTYPE_F32) launch8<float>(t, blocks, st);
-  else if (dtype == TFR_DTYPE_BF16) launch8<__bf16>(t, blocks, st);
-  else launch8<_Float16>(t, blocks, st);
-  return (int)hipGetLastError();
+  const int rc = fill_scales<Table8, BLOCK8>(t, TFR_ADAMW8_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_scales_host, exp_avg_sqs_host,
+                                             exp_avg_sq_scales_host, sizes_host, lr, beta1, beta2, eps, weight_decay, step, now, 0);
+  return rc != TFR_OK ? rc : run(t, dtype, (hipStream_t)stream);
+}
+
+extern "C" int tfr_adamw_counted(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+                                 void* const* exp_avg_sqs_host, const int64_t* sizes_host, int64_t* const* steps_host, int64_t* all,
+                                 const float* lr_device, double lr, double beta1, double beta2, double eps, double weight_decay, float* now,
+                                 void* stream) {
+  if (!elem_known(dtype) || !steps_host || !now) return TFR_EINVAL;
+  Table32 t;
+  const int rc = fill<Table32, BLOCK32>(t, TFR_ADAMW_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_sqs_host, sizes_host,
+                                        lr, beta1, beta2, eps, weight_decay, 0, now, 3);
+  return rc != TFR_OK ? rc : run_counted(t, dtype, steps_host, all, lr_device, lr, beta1, beta2, weight_decay, now, (hipStream_t)stream);
+}
+
+extern "C" int tfr_adamw8_counted(int dtype, int count, void* const* params_host, const void* const* grads_host, void* const* exp_avgs_host,
+                                  float* const* exp_avg_scales_host, void* const* exp_avg_sqs_host, float* const* exp_avg_sq_scales_host,
+                                  const int64_t* sizes_host, int64_t* const* steps_host, int64_t* all, const float* lr_device, double lr,
+                                  double beta1, double beta2, double eps, double weight_decay, float* now, void* stream) {
+  if (!elem_known(dtype) || !steps_host || !now) return TFR_EINVAL;
+  Table8 t;
+  const int rc = fill_scales<Table8, BLOCK8>(t, TFR_ADAMW8_MAX_TENSORS, count, params_host, grads_host, exp_avgs_host, exp_avg_scales_host, exp_avg_sqs_host,
+                                             exp_avg_sq_scales_host, sizes_host, lr, beta1, beta2, eps, weight_decay, 0, now, 3);
+  return rc != TFR_OK ? rc : run_counted(t, dtype, steps_host, all, lr_device, lr, beta1, beta2, weight_decay, now, (hipStream_t)stream);
 }
 
 extern "C" int tfr_adamw_advance(int64_t* step, const float* lr_device, double lr, double beta1, double beta2, double weight_decay, float* now,

@@ -123,8 +123,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
     ``params`` / ``grads``: dense tensors of one type (float32, bfloat16, float16) a pair.  ``exp_avgs`` / ``exp_avg_sqs``:
     float32 tensors of the parameter's size, or all of them pairs ``(codes, scales)``: int8 / uint8 codes and float32 scales
-    of ``quantized_size(param.numel())`` elements.  ``step`` counts from 1.  ``now``: float32 ``[3]`` on the device, written
-    by ``AdamW`` when the step is counted there (``step`` and ``lr`` are then not used)."""
+    of ``quantized_size(param.numel())`` elements.  ``step`` counts from 1.  ``now``: float32 ``[3]`` on the device, the
+    coefficients of a step that is counted there, as ``tfr_adamw_advance`` writes them (``step`` and ``lr`` are then not used)."""
     n = len(params)
     if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n):
         raise ValueError('lists of %d params, %d grads, %d exp_avgs and %d exp_avg_sqs' % (n, len(grads), len(exp_avgs), len(exp_avg_sqs)))
@@ -141,32 +141,61 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         _check_dense(now, params[0], 3, torch.float32, 'now')
         if any(p.get_device() != now.get_device() for p in params):
             raise ValueError('now is on %s: a step that is counted on a device takes the parameters of that device' % (now.device,))
+    tail = (lr, betas[0], betas[1], eps, weight_decay, step, None if now is None else now.data_ptr())
+    for launch, name, device, args, _ in _launches(params, grads, exp_avgs, exp_avg_sqs, False):
+        with _ops.device_of(device):
+            rc = launch(*args, *tail, _raw_stream(device))
+        if rc:
+            _lib.check(rc, name)
+    _changed(params)
+
+
+def _launches(params, grads, exp_avgs, exp_avg_sqs, counted):
+    """(C entry point, its name, device, first arguments, addresses of the parameters) of every launch of a step."""
     eight = isinstance(exp_avgs[0], (tuple, list))
     groups = _uniform(params, grads, exp_avgs, exp_avg_sqs, eight) or _grouped(params, grads, exp_avgs, exp_avg_sqs, eight)
     cap = _MAX_TENSORS_8 if eight else _MAX_TENSORS
-    lib = _lib.load()
-    launch, name = (lib.tfr_adamw8, 'tfr_adamw8') if eight else (lib.tfr_adamw, 'tfr_adamw')
+    name = ('tfr_adamw8' if eight else 'tfr_adamw') + ('_counted' if counted else '')
+    launch = getattr(_lib.load(), name)
     for (device, dtype), rows in groups.items():
         size_of = [row[-1] for row in rows]
-        with _ops.device_of(device):
-            tail = (lr, betas[0], betas[1], eps, weight_decay, step, None if now is None else now.data_ptr(), _raw_stream(device))
-            at = 0
-            while at < len(rows):
-                end = min(at + cap, len(rows))
-                while sum(size_of[at:end]) >= _MAX_LAUNCH:
-                    end -= 1
-                columns = list(zip(*rows[at:end]))
-                addresses = ctypes.c_void_p * (end - at)
-                rc = launch(_DTYPES[dtype], end - at, *[addresses(*c) for c in columns[:-1]], (ctypes.c_int64 * (end - at))(*columns[-1]), *tail)
-                if rc:
-                    _lib.check(rc, name)
-                at = end
-    try:                                                       # a graph that saved a parameter must not go backward any more
+        at = 0
+        while at < len(rows):
+            end = min(at + cap, len(rows))
+            while sum(size_of[at:end]) >= _MAX_LAUNCH:
+                end -= 1
+            columns = list(zip(*rows[at:end]))
+            addresses = ctypes.c_void_p * (end - at)
+            yield launch, name, device, (_DTYPES[dtype], end - at, *[addresses(*c) for c in columns[:-1]], (ctypes.c_int64 * (end - at))(*columns[-1])), columns[0]
+            at = end
+
+
+def _changed(params):
+    """A graph that saved a parameter must not go backward any more."""
+    try:
         torch.autograd.graph.increment_version(params)
     except RuntimeError:                                       # inference tensors have no version
         for p in params:
             if not p.is_inference():
                 torch.autograd.graph.increment_version(p)
+
+
+def _counted_step(params, grads, exp_avgs, exp_avg_sqs, steps, all_steps, lr, betas, eps, weight_decay):
+    """``adamw_step`` with the step counts on the device: ``steps`` one int64 tensor a parameter, ``all_steps`` one that counts
+    the calls; ``lr`` a number or a float32 tensor of one element there."""
+    lr_device = lr.data_ptr() if torch.is_tensor(lr) else None
+    tail = (0.0 if lr_device else lr, betas[0], betas[1], eps, weight_decay)
+    count_of = {p.data_ptr(): t.data_ptr() for p, t in zip(params, steps)}
+    every = all_steps.data_ptr()
+    for launch, name, device, args, addresses in _launches(params, grads, exp_avgs, exp_avg_sqs, True):
+        with _ops.device_of(device):
+            now = torch.empty(3 * len(addresses), dtype=torch.float32, device=all_steps.device)
+            counts = (ctypes.c_void_p * len(addresses))(*[count_of[a] for a in addresses])
+            rc = launch(*args, counts, every, lr_device, *tail, now.data_ptr(), _raw_stream(device))
+        if rc:
+            _lib.check(rc, name)
+        every = None
+    _changed(params)
 
 
 def _dequantize(codes, scales, dtype, square):
@@ -199,9 +228,10 @@ class AdamW(torch.optim.Optimizer):
     ``TFR_ADAMW_MAX_TENSORS`` tensors.
 
     ``state_bits=8`` holds the moments in 8 bits (2.06 bytes an element for both instead of 8).  ``capturable=True`` counts the
-    step on the device (one small launch more), so that a step recorded in a hipGraph keeps counting when it is replayed;
-    ``lr`` may then be a float32 device tensor of one element.  The state is made by the first eager step (or by
-    ``init_state()``); a capture needs it to be there."""
+    steps on the device (one small launch more), so that a step recorded in a hipGraph keeps counting when it is replayed;
+    ``lr`` may then be a float32 device tensor of one element.  Either way every parameter has its own count
+    (``state[p]['step']``): one that gets its first gradient late is corrected by the steps that it took itself.  The state is
+    made by the first eager step (or by ``init_state()``); a capture needs it to be there."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
@@ -222,32 +252,33 @@ class AdamW(torch.optim.Optimizer):
 
     def _state_of(self, p, group):
         s = self.state[p]
-        if 'exp_avg' in s:
+        there = torch.is_tensor(s.get('step'))                 # counted on the device
+        if 'exp_avg' in s and there == group['capturable']:
             return s
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('AdamW: the state must be there before a stream capture (run a step or init_state() first)')
         require_device(p, 'params')
-        if group['state_bits'] == 32:
-            s['exp_avg'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            s['exp_avg_sq'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-        else:
-            codes, blocks = quantized_size(p.numel())
-            s['exp_avg'] = torch.zeros(codes, dtype=torch.int8, device=p.device)
-            s['exp_avg_sq'] = torch.zeros(codes, dtype=torch.uint8, device=p.device)
-            s['exp_avg_scale'] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-            s['exp_avg_sq_scale'] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-        if not group['capturable']:
-            s['step'] = 0
+        if 'exp_avg' not in s:
+            if group['state_bits'] == 32:
+                s['exp_avg'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                s['exp_avg_sq'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:
+                codes, blocks = quantized_size(p.numel())
+                s['exp_avg'] = torch.zeros(codes, dtype=torch.int8, device=p.device)
+                s['exp_avg_sq'] = torch.zeros(codes, dtype=torch.uint8, device=p.device)
+                s['exp_avg_scale'] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+                s['exp_avg_sq_scale'] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        taken = int(s.get('step', 0))                          # `capturable` may have been switched
+        s['step'] = torch.full((1,), taken, dtype=torch.int64, device=p.device) if group['capturable'] else taken
         return s
 
     def _counter(self, group, device):
-        """(step count, coefficients) on the device, of a capturable group."""
+        """The steps of a capturable group, on the device (its parameters count their own)."""
         if group.get('step_count') is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: the state must be there before a stream capture (run a step or init_state() first)')
             group['step_count'] = torch.zeros(1, dtype=torch.int64, device=device)
-            group['coefficients'] = torch.zeros(3, dtype=torch.float32, device=device)
-        return group['step_count'], group['coefficients']
+        return group['step_count']
 
     def init_state(self) -> None:
         """Makes the state of every parameter (before a stream capture without an eager step)."""
@@ -272,48 +303,41 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise ValueError('AdamW does not take sparse gradients')
                 s = self._state_of(p, group)
-                t = 1 if group['capturable'] else s['step'] + 1
+                t = 0 if group['capturable'] else s['step'] + 1
                 m, v = s['exp_avg'], s['exp_avg_sq']
                 runs.setdefault(t, []).append((s, p, p.grad.contiguous(), (m, s['exp_avg_scale']) if eight else m,
                                                (v, s['exp_avg_sq_scale']) if eight else v))
             if not runs:
                 continue
-            lr, now = group['lr'], None
-            if group['capturable']:
-                now = self._advance(group, next(iter(runs.values()))[0][1].device)
-            elif torch.cuda.is_current_stream_capturing():
+            how = dict(lr=group['lr'], betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'])
+            if group['capturable']:                            # all in one list: the launches read the counts on the device
+                states, p, g, m, v = zip(*runs[0])
+                count = self._counter(group, p[0].device)
+                if any(q.device != count.device for q in group['params']):
+                    raise ValueError('AdamW: a capturable group lives on one device')
+                lr = group['lr']
+                if torch.is_tensor(lr) and not (lr.is_cuda and lr.dtype == torch.float32 and lr.numel() == 1 and lr.device == count.device):
+                    raise ValueError('lr must be a float32 tensor of one element on %s' % (count.device,))
+                _check_hyper(**how)
+                _counted_step(p, g, m, v, [s['step'] for s in states], count, **how)
+                continue
+            if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('AdamW: a step inside a stream capture needs capturable=True (the step count would be frozen)')
             for t, items in runs.items():
                 states, p, g, m, v = zip(*items)
-                adamw_step(p, g, m, v, step=t, lr=lr, betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'], now=now)
-                if not group['capturable']:
-                    for s in states:                           # counted once it is launched: a step that is refused is none
-                        s['step'] = t
+                adamw_step(p, g, m, v, step=t, **how)
+                for s in states:                               # counted once it is launched: a step that is refused is none
+                    s['step'] = t
         return loss
-
-    def _advance(self, group, device):
-        count, now = self._counter(group, device)
-        if any(p.device != count.device for p in group['params']):
-            raise ValueError('AdamW: a capturable group lives on one device')
-        lr, lr_device = group['lr'], None
-        if torch.is_tensor(lr):
-            if not (lr.is_cuda and lr.dtype == torch.float32 and lr.numel() == 1 and lr.device == count.device):
-                raise ValueError('lr must be a float32 tensor of one element on %s' % (count.device,))
-            lr, lr_device = 0.0, lr
-        with torch.cuda.device(count.device):
-            rc = _lib.load().tfr_adamw_advance(_ptr(count), _ptr(lr_device), float(lr), group['betas'][0], group['betas'][1],
-                                               group['weight_decay'], _ptr(now), _stream())
-        _lib.check(rc, 'tfr_adamw_advance')
-        return now
 
     def load_state_dict(self, state_dict) -> None:
         """Loads what ``state_dict`` gave.  Moments keep their own types (the base class would cast them to the
         parameter's), and tensors that are there already are filled in place: a captured step goes on with them."""
         mine = {p: dict(s) for p, s in self.state.items()}
-        counters = [(g.get('step_count'), g.get('coefficients')) for g in self.param_groups]
+        counters = [g.get('step_count') for g in self.param_groups]
         saved = [(g.get('step_count'), g['params']) for g in state_dict['param_groups']]
         super().load_state_dict(state_dict)
-        for group, (count, ids), (old, coef) in zip(self.param_groups, saved, counters):
+        for group, (count, ids), old in zip(self.param_groups, saved, counters):
             for p, i in zip(group['params'], ids):
                 given = state_dict['state'].get(i)
                 if given is None:
@@ -321,11 +345,13 @@ class AdamW(torch.optim.Optimizer):
                 codes, blocks = quantized_size(p.numel())
                 sizes = {'exp_avg': codes, 'exp_avg_sq': codes, 'exp_avg_scale': blocks, 'exp_avg_sq_scale': blocks}
                 s = self.state[p] = {}
+                if count is not None and 'step' not in given:      # counted by group alone: each of its parameters took them all
+                    given = dict(given, step=count)
                 for key, value in given.items():
                     if not torch.is_tensor(value):
                         s[key] = value
                         continue
-                    want = sizes.get(key) if group['state_bits'] == 8 else p.numel()
+                    want = 1 if key == 'step' else sizes.get(key) if group['state_bits'] == 8 else p.numel()
                     if value.numel() != want:
                         raise ValueError('state %s of %d elements does not fit a parameter of %d' % (key, value.numel(), p.numel()))
                     have = mine.get(p, {}).get(key)
@@ -336,4 +362,4 @@ class AdamW(torch.optim.Optimizer):
             if count is not None and group['params']:
                 device = group['params'][0].device
                 group['step_count'] = count.to(device, copy=True) if old is None else old.copy_(count)
-                group['coefficients'] = torch.zeros(3, dtype=torch.float32, device=device) if coef is None else coef
+                group.pop('coefficients', None)                # of a state that counted by group alone

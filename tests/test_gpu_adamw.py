@@ -403,3 +403,103 @@ def test_stale_graphs_are_refused():
         a, b = torch.ones(3, device=DEV), torch.zeros(3, device=DEV)
         O().adamw_step([a], [torch.ones_like(a)], [b], [torch.zeros_like(a)], step=1, lr=0.1, weight_decay=0.0)
         assert torch.allclose(a, torch.full_like(a, 0.9), atol=1e-6)
+
+
+# ---------------------------------------------------------------- counts of a capturable group
+@pytest.mark.parametrize('bits', [8, 32])
+@pytest.mark.parametrize('replayed', [False, True])
+def test_counts_on_the_device_are_a_parameters_own(bits, replayed):
+    """A parameter that is frozen at first, or for a while, is corrected by the number of its own steps, as it is where the host
+    counts: lr (m / (1 - beta1)) / sqrt(v / (1 - beta2)) = lr at its first step, not 3.2 lr.  `replayed`: the steps of all parameters
+    are a graph that was captured before any was missed."""
+    runs = []
+    for capturable in (True, False):
+        ps = params()
+        held = [torch.zeros_like(p) for p in ps]
+        opt = O().AdamW(ps, lr=0.01, weight_decay=0.1, state_bits=bits, capturable=capturable)
+        graph = None
+        if capturable and replayed:
+            for p, h in zip(ps, held):
+                p.grad = h
+            opt.init_state()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
+        for step in range(12):
+            g = torch.Generator().manual_seed(step)
+            for h in held:
+                h.copy_(torch.randn(h.shape, generator=g))
+            missing = {2} if step < 6 else {0, 3} if step in (7, 8) else set()
+            for k, (p, h) in enumerate(zip(ps, held)):
+                p.grad = None if k in missing else h
+            before = ps[2].detach().clone()
+            if graph is not None and not missing:
+                graph.replay()
+            else:
+                opt.step()
+            if step == 6:                                      # the late one's first step: every element moves by lr, and decays
+                moved = (ps[2] - before * (1 - 0.01 * 0.1)).abs()
+                assert (moved - 0.01).abs().max() < 1e-4 * 0.01 + 4 * T.U * before.abs().max()
+        torch.cuda.synchronize()
+        assert [int(opt.state[p]['step']) for p in ps] == [10, 12, 6, 10]
+        runs.append((ps, [opt.state[p] for p in ps]))
+    for a, b in zip(runs[0][0], runs[1][0]):
+        # the coefficients come from pow() of the host and of the device: a rounding a step
+        assert torch.allclose(a, b, rtol=0, atol=12 * 20 * T.U * (b.abs().max() + 1).item())
+    for a, b in zip(runs[0][1], runs[1][1]):
+        for key in ('exp_avg', 'exp_avg_sq'):
+            assert torch.equal(a[key], b[key])                 # the moments do not hang on the count
+
+
+def test_counts_of_many_tensors_and_types():
+    """More tensors than a launch holds, two types in a group, one empty: as where the host counts."""
+    runs = []
+    for capturable in (True, False):
+        g = torch.Generator().manual_seed(1)
+        ps = [torch.nn.Parameter(torch.randn(n % 13, generator=g).to(torch.bfloat16 if n % 3 == 0 else torch.float32).to(DEV)) for n in range(1, 200)]
+        opt = O().AdamW(ps, lr=0.01, capturable=capturable)
+        for step in range(3):
+            for k, p in enumerate(ps):
+                grad = torch.randn(p.shape, generator=g).to(p.dtype).to(DEV)
+                p.grad = grad if (k + step) % 5 or step == 2 else None
+            opt.step()
+        runs.append((ps, [int(opt.state[p]['step']) for p in ps]))
+    assert all(a == b for a, b, p in zip(runs[0][1], runs[1][1], runs[0][0]) if p.numel())
+    for a, b in zip(runs[0][0], runs[1][0]):
+        assert torch.allclose(a.float(), b.float(), rtol=0 if a.dtype == torch.float32 else 2 ** -8, atol=3 * 20 * T.U * 5)
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_counts_are_saved_and_loaded(bits):
+    """A saved capturable state goes on bit for bit, with the counts of its parameters; one that holds the group's count alone gives
+    it to each; and a group whose `capturable` is switched keeps its counts."""
+    import copy
+    ps = params()
+    opt = O().AdamW(ps, state_bits=bits, capturable=True, **HYPER)
+    for step in range(4):
+        grads(ps, step)
+        if step < 3:
+            ps[1].grad = None
+        opt.step()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    again = O().AdamW(qs, state_bits=bits, capturable=True, lr=1.0)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert [int(again.state[q]['step']) for q in qs] == [4, 1, 4, 4] and again.param_groups[0]['step_count'].item() == 4
+    grads(ps, 9), grads(qs, 9)
+    opt.step(), again.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    old = copy.deepcopy(opt.state_dict())
+    for s in old['state'].values():
+        del s['step']
+    again.load_state_dict(old)
+    assert [int(again.state[q]['step']) for q in qs] == [5] * 4
+    for group in opt.param_groups:
+        group['capturable'] = False
+    grads(ps, 10)
+    opt.step()
+    assert [opt.state[p]['step'] for p in ps] == [6, 3, 6, 6]
+    for group in opt.param_groups:
+        group['capturable'] = True
+    opt.step()
+    assert [int(opt.state[p]['step']) for p in ps] == [7, 4, 7, 7]

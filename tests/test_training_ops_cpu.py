@@ -261,3 +261,19 @@ def test_a_refused_step_is_not_counted(monkeypatch):
     with pytest.raises(RuntimeError, match='capturable'):
         opt.step()
     assert opt.state[p]['step'] == 2
+
+
+def test_counted_adamw_arguments_are_checked_before_any_launch():
+    lib = _lib.load()
+    ptr, size = (ctypes.c_void_p * 1)(256), (ctypes.c_int64 * 1)(4)
+
+    def call(steps=ptr, n=size, now=one, b1=0.9, count=1, dtype=0):
+        return lib.tfr_adamw_counted(dtype, count, ptr, ptr, ptr, ptr, n, steps, None, None, 1e-3, b1, 0.999, 1e-8, 0.0, now, None)
+
+    def call8(steps=ptr, n=size, now=one, scales=ptr, m=ptr):
+        return lib.tfr_adamw8_counted(0, 1, ptr, ptr, m, scales, ptr, ptr, n, steps, None, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, now, None)
+    for f in (call, call8):
+        assert f(steps=None) == -1 and f(steps=(ctypes.c_void_p * 1)(None)) == -1 and f(now=None) == -1
+        assert f(n=(ctypes.c_int64 * 1)(-1)) == -1 and f(n=(ctypes.c_int64 * 1)(1 << 40)) == -1
+    assert call(b1=1.0) == -1 and call(count=0) == -1 and call(count=89) == -1 and call(dtype=3) == -1
+    assert call8(scales=None) == -1 and call8(m=(ctypes.c_void_p * 1)(260)) == -1
