@@ -330,36 +330,72 @@ class AdamW(torch.optim.Optimizer):
                     s['step'] = t
         return loss
 
+    def _moments(self, p, group):
+        """(type, elements) of what the state of a parameter holds beside its count."""
+        if group['state_bits'] == 32:
+            return {'exp_avg': (torch.float32, p.numel()), 'exp_avg_sq': (torch.float32, p.numel())}
+        codes, blocks = quantized_size(p.numel())
+        return {'exp_avg': (torch.int8, codes), 'exp_avg_sq': (torch.uint8, codes), 'exp_avg_scale': (torch.float32, blocks),
+                'exp_avg_sq_scale': (torch.float32, blocks)}
+
+    @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        """Loads what ``state_dict`` gave.  Moments keep their own types (the base class would cast them to the
-        parameter's), and tensors that are there already are filled in place: a captured step goes on with them."""
-        mine = {p: dict(s) for p, s in self.state.items()}
-        counters = [g.get('step_count') for g in self.param_groups]
-        saved = [(g.get('step_count'), g['params']) for g in state_dict['param_groups']]
+        """Loads what ``state_dict`` gave; a state that does not fit raises and changes nothing.  Moments keep their own types
+        (the base class would cast them to the parameter's).  Tensors that are there already -- moments, counts, a learning
+        rate on the device -- stay and are filled, with zeros where the loaded state holds none: a captured step goes on with
+        them, and a group that is capturable stays so."""
+        saved, mine = state_dict['param_groups'], [dict(g) for g in self.param_groups]
+        held = {p: dict(s) for p, s in self.state.items()}
+        for group, given in zip(mine, saved):
+            if group['capturable'] and given['state_bits'] != group['state_bits'] and any(held.get(p) for p in group['params']):
+                raise ValueError('a state of %d bits does not fit one of %d that a captured step may hold' % (given['state_bits'], group['state_bits']))
+            for p, i in zip(group['params'], given['params']):
+                for key, (dtype, numel) in self._moments(p, given).items() if i in state_dict['state'] else ():
+                    value = state_dict['state'][i].get(key)
+                    if not torch.is_tensor(value) or value.numel() != numel or (value.dtype != dtype if given['state_bits'] == 8 else not value.is_floating_point()):
+                        raise ValueError('state %s does not fit a parameter of %d elements: %d of %s are wanted' % (key, p.numel(), numel, dtype))
         super().load_state_dict(state_dict)
-        for group, (count, ids), old in zip(self.param_groups, saved, counters):
-            for p, i in zip(group['params'], ids):
-                given = state_dict['state'].get(i)
-                if given is None:
-                    continue
-                codes, blocks = quantized_size(p.numel())
-                sizes = {'exp_avg': codes, 'exp_avg_sq': codes, 'exp_avg_scale': blocks, 'exp_avg_sq_scale': blocks}
-                s = self.state[p] = {}
-                if count is not None and 'step' not in given:      # counted by group alone: each of its parameters took them all
-                    given = dict(given, step=count)
-                for key, value in given.items():
-                    if not torch.is_tensor(value):
-                        s[key] = value
-                        continue
-                    want = 1 if key == 'step' else sizes.get(key) if group['state_bits'] == 8 else p.numel()
-                    if value.numel() != want:
-                        raise ValueError('state %s of %d elements does not fit a parameter of %d' % (key, value.numel(), p.numel()))
-                    have = mine.get(p, {}).get(key)
-                    if have is not None and have.dtype == value.dtype and have.shape == value.shape:
-                        s[key] = have.copy_(value)
-                    else:
-                        s[key] = value.to(p.device, copy=True)
-            if count is not None and group['params']:
-                device = group['params'][0].device
-                group['step_count'] = count.to(device, copy=True) if old is None else old.copy_(count)
-                group.pop('coefficients', None)                # of a state that counted by group alone
+        for group, old, given in zip(self.param_groups, mine, saved):
+            group['capturable'] = there = bool(group['capturable'] or old['capturable'])
+            count = given.get('step_count')
+            for p, i in zip(group['params'], given['params']):
+                self._fill_state(p, group, held.get(p, {}), state_dict['state'].get(i), count)
+            if not group['params']:
+                continue
+            device = group['params'][0].device
+            group.pop('coefficients', None)                    # of a state that counted by group alone
+            group.pop('step_count', None)
+            if there and (count is not None or old.get('step_count') is not None):
+                group['step_count'] = _filled(old.get('step_count'), 0 if count is None else count, torch.int64, device)
+            if torch.is_tensor(old['lr']):
+                group['lr'] = _filled(old['lr'], group['lr'], old['lr'].dtype, device)
+            elif torch.is_tensor(group['lr']):
+                group['lr'] = group['lr'].to(device)
+
+    def _fill_state(self, p, group, have, given, count):
+        """The state of one parameter from the saved one (None: as before any step), in the tensors of ``have`` that fit."""
+        moments = self._moments(p, group)
+        fits = {k: t for k, t in have.items() if k in moments and torch.is_tensor(t) and (t.dtype, t.numel()) == moments[k]}
+        if given is None:
+            self.state.pop(p, None)
+            if len(fits) < len(moments):
+                return
+        s = self.state[p] = {}
+        for key, (dtype, _) in moments.items():
+            s[key] = _filled(fits.get(key), 0 if given is None else given[key], dtype, p.device)
+        # counted by group alone, each of its parameters took all of the group's steps
+        taken = 0 if given is None else given.get('step', 0 if count is None else count)
+        step = have.get('step')
+        s['step'] = _filled(step if torch.is_tensor(step) else None, taken, torch.int64, p.device) if group['capturable'] else int(taken)
+        for key, value in (given or {}).items():
+            if key not in s:
+                s[key] = value
+
+
+def _filled(have, value, dtype, device):
+    """``value`` (a tensor or a number) in the tensor ``have``, or in a new one where there is none."""
+    if not torch.is_tensor(value):
+        return torch.full((1,), value, dtype=dtype, device=device) if have is None else have.fill_(value)
+    if have is None:
+        return value.to(device=device, dtype=dtype, copy=True)
+    return have.copy_(value.reshape(have.shape))

@@ -503,3 +503,54 @@ def test_counts_are_saved_and_loaded(bits):
         group['capturable'] = True
     opt.step()
     assert [int(opt.state[p]['step']) for p in ps] == [7, 4, 7, 7]
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_a_captured_step_goes_on_after_loading(bits):
+    """Saved (to the host), loaded again and loaded with a state from before any step, a captured step with its learning rate on the
+    device is replayed: bit for bit the eager run that loads the same."""
+    import copy
+    import io
+    runs = []
+    for captured in (True, False):
+        ps = params()
+        held = [torch.zeros_like(p) for p in ps]
+        for p, h in zip(ps, held):
+            p.grad = h
+        opt = O().AdamW(ps, lr=torch.tensor(0.01, device=DEV), weight_decay=0.1, state_bits=bits, capturable=True)
+        fresh = copy.deepcopy(opt.state_dict())
+        opt.init_state()
+        step = opt.step
+        if captured:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
+            step = graph.replay
+        seen = []
+
+        def go(n):
+            for _ in range(n):
+                g = torch.Generator().manual_seed(len(seen))
+                for h in held:
+                    h.copy_(torch.randn(h.shape, generator=g))
+                step()
+                torch.cuda.synchronize()
+                seen.append([p.detach().clone() for p in ps])
+                torch.randn(1 << 16, device=DEV)                           # takes what was given back to the allocator
+        go(3)
+        buf = io.BytesIO()
+        torch.save(opt.state_dict(), buf)
+        opt.param_groups[0]['lr'].fill_(0.5)
+        go(2)
+        buf.seek(0)
+        opt.load_state_dict(torch.load(buf, weights_only=True, map_location='cpu'))
+        go(3)
+        assert opt.param_groups[0]['step_count'].item() == 6 and opt.param_groups[0]['lr'].item() == pytest.approx(0.01)
+        opt.param_groups[0]['lr'].fill_(0.02)
+        opt.load_state_dict(fresh)
+        go(2)
+        assert opt.param_groups[0]['step_count'].item() == 2 and [int(opt.state[p]['step']) for p in ps] == [2] * 4
+        runs.append(seen)
+    for a, b in zip(*runs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

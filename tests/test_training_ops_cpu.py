@@ -277,3 +277,74 @@ def test_counted_adamw_arguments_are_checked_before_any_launch():
         assert f(n=(ctypes.c_int64 * 1)(-1)) == -1 and f(n=(ctypes.c_int64 * 1)(1 << 40)) == -1
     assert call(b1=1.0) == -1 and call(count=0) == -1 and call(count=89) == -1 and call(dtype=3) == -1
     assert call8(scales=None) == -1 and call8(m=(ctypes.c_void_p * 1)(260)) == -1
+
+
+def same_places(before, s):
+    return all(s[k] is t for k, t in before.items() if torch.is_tensor(t))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_loading_fills_what_a_captured_step_holds(bits):
+    """A captured step reads and writes the tensors that were there: a learning rate on the device, counts and moments keep their
+    places, whatever the loaded state holds of them."""
+    import copy
+    ps = [torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(200))]
+    lr = torch.tensor(0.25)
+    opt = optim.AdamW(ps, lr=lr, capturable=True, state_bits=bits)
+    fresh = copy.deepcopy(opt.state_dict())                                 # before any step: no moments, no counts
+    for k, p in enumerate(ps):
+        opt.state[p] = held_state(p, torch.tensor([4 + k]), bits)
+    opt.param_groups[0]['step_count'] = torch.tensor([5])
+    count, held = opt.param_groups[0]['step_count'], [dict(opt.state[p]) for p in ps]
+    saved = copy.deepcopy(opt.state_dict())
+    lr.fill_(0.5)
+    count.fill_(9)
+    for s in held:
+        for t in s.values():
+            t.zero_()
+
+    def check(rate, counts, all_steps, moment):
+        g = opt.param_groups[0]
+        assert g['lr'] is lr and lr.item() == pytest.approx(rate) and g['step_count'] is count and count.item() == all_steps
+        for p, s, n in zip(ps, held, counts):
+            assert same_places(s, opt.state[p]) and set(s) == set(opt.state[p])
+            assert s['step'].item() == n and s['exp_avg'].float().eq(moment).all()
+    opt.load_state_dict(saved)
+    check(0.25, (4, 5), 5, 0.5 if bits == 32 else 3)
+    other = copy.deepcopy(saved)
+    other['param_groups'][0]['lr'] = 0.125                                  # saved where the rate was a number
+    opt.load_state_dict(other)
+    check(0.125, (4, 5), 5, 0.5 if bits == 32 else 3)
+    opt.load_state_dict(fresh)                                              # as at the start: nothing but zeros, in place
+    check(0.25, (0, 0), 0, 0)
+    partly = copy.deepcopy(saved)
+    del partly['state'][1]
+    opt.load_state_dict(partly)
+    assert [s['step'].item() for s in held] == [4, 0] and not held[1]['exp_avg'].any() and held[0]['exp_avg'].any()
+    assert all(same_places(s, opt.state[p]) for s, p in zip(held, ps))
+
+
+def test_a_state_that_does_not_fit_changes_nothing():
+    import copy
+    ps = [torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(200))]
+    opt = optim.AdamW(ps, lr=0.1)
+    for k, p in enumerate(ps):
+        opt.state[p] = held_state(p, 4 + k)
+    bad = copy.deepcopy(opt.state_dict())
+    bad['state'][0]['exp_avg'] = torch.ones(3)
+    bad['state'][1]['exp_avg'] = torch.ones(199)
+    bad['param_groups'][0]['lr'] = 7.0
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
+    assert opt.param_groups[0]['lr'] == 0.1 and opt.state[ps[0]]['exp_avg'].eq(0.5).all() and opt.state[ps[1]]['step'] == 5
+
+
+def test_a_learning_rate_on_the_device_follows_its_parameters():
+    """Loaded into an optimizer whose rate is a number, a rate that was saved as a tensor is no part of the saved dict."""
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    lr = torch.tensor(0.25)
+    saved = optim.AdamW([p], lr=lr, capturable=True).state_dict()
+    opt = optim.AdamW([q], lr=0.5, capturable=True)
+    opt.load_state_dict(saved)
+    got = opt.param_groups[0]['lr']
+    assert torch.is_tensor(got) and got is not lr and got.item() == 0.25 and got.device == q.device
