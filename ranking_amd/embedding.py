@@ -10,6 +10,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import _ops
@@ -112,6 +113,12 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: int, s
     return out
 
 
+def _differentiated(t) -> bool:
+    """Whether autograd has to see a call on ``t``: a gradient is wanted, or ``t`` carries a forward-mode tangent (which the autograd
+    functions here refuse; the kernels, called on its address, would drop it)."""
+    return torch.is_tensor(t) and ((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None)
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, combiner):
@@ -133,6 +140,6 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
     are added (averaged over the ids that are not padding), in fp32, and rounded once: ``ids.shape[:-1] + (dim,)``.
     Ids below 0 are padding: zeros, no gradient.  An id beyond the table gives NaN and no gradient.  Differentiable with
     respect to ``table``; the gradient is a dense tensor of the table's type."""
-    if torch.is_grad_enabled() and torch.is_tensor(table) and table.requires_grad:
+    if _differentiated(table):
         return _EmbeddingFn.apply(table, ids, scale, combiner)
     return _lookup(table, ids, scale, combiner)

@@ -13,7 +13,7 @@ import torch
 from . import _lib
 from . import _ops
 from ._ops import _raw_stream, require_device
-from .embedding import _device_of, _dtype_code
+from .embedding import _device_of, _differentiated, _dtype_code
 
 KINDS = {'logistic': 0, 'hinge': 1, 'squared': 2}                          # TFR_PREFERENCE_*
 MAX_ANSWERS = 64
@@ -115,7 +115,7 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, temperature: fl
     """``log softmax(logits / temperature)[targets]``: logits ``[..., vocab]`` (float32, bfloat16, float16; rows of any
     stride), targets ``[...]`` -> float32 ``[...]``.  A target below 0 is no target: 0, no gradient, its row is not read.
     A target beyond the vocabulary gives NaN.  Differentiable with respect to ``logits``."""
-    if torch.is_grad_enabled() and torch.is_tensor(logits) and logits.requires_grad:
+    if _differentiated(logits):
         return _TokenLogProbsFn.apply(logits, targets, temperature)
     return _log_probs(logits, targets, temperature, False)[0]
 

@@ -260,3 +260,26 @@ def test_pipeline_with_embedded_features(tmp_path, optimizer, loss):
     assert torch.isfinite(torch.tensor(history['loss'] + history['val_loss'])).all()
     table = pipe.model.scorer._embeddings['tokens'].weight
     assert table.grad is not None and table.grad.abs().sum() > 0 and torch.isfinite(table).all()
+
+
+def test_forward_mode_is_refused():
+    """None of the operators has a forward-mode derivative: a tensor that carries a tangent is refused, with and without gradients
+    (the call used to give a result without one)."""
+    import torch.autograd.forward_ad as fwAD
+    from ranking_amd import preference
+    from ranking_amd.embedding import embedding_lookup
+    from ranking_amd.keras.losses import PreferenceLoss
+    x, ids, y = torch.randn(6, 8, device=DEV), torch.tensor([1, 5, -1], device=DEV), torch.ones(6, 8, device=DEV)
+    calls = (lambda t: embedding_lookup(t, ids), lambda t: embedding_lookup(t, ids.view(1, 3), combiner='mean'),
+             lambda t: preference.token_log_probs(t[:3], ids), lambda t: PreferenceLoss()(y, t))
+    plain = [call(x) for call in calls]
+    with fwAD.dual_level():
+        assert all(torch.equal(call(x), want) for call, want in zip(calls, plain))      # a level alone changes nothing
+        dual = fwAD.make_dual(x, torch.ones_like(x))
+        for call in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call(dual)
+    for call in calls[:3]:
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
