@@ -409,7 +409,8 @@ __device__ __forceinline__ void put_row(T* __restrict__ p, const float (&v)[E]) 
 template <typename T, int E, bool ONCE, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_runs_kernel(const GradArgs a, const T* __restrict__ grad) {
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
-  const long job = (long)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const long block = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  const long job = block * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
   const long q = job / a.steps;
   const int column = (int)(job - q * a.steps);
   const long begin = q << a.chunk_log2;
@@ -585,6 +586,8 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const GradArgs a, i
 }
 
 // ------------------------------------------------------------------------------------------------ host
+constexpr long kMostBlocks = (1l << 24) - 1;                    // workgroups of 256 along an axis: no grid of 2^32 threads
+
 int log2_ceil(long n) {
   int k = 0;
   while ((1l << k) < n) ++k;
@@ -645,11 +648,15 @@ int launch_lookup(const T* table, long ld, int rows, int dim, const Id* ids, lon
   const int lg = log2_ceil(packs < 64 ? packs : 64);
   const int groups = 256 >> lg;
   if (combiner == TFR_COMBINER_NONE) {
-    const long steps = (packs + (1 << lg) - 1) >> lg, jobs = bags * steps;
-    if ((jobs + groups - 1) / groups >= (1l << 24)) return TFR_EINVAL;    // no grid of 2^32 threads
+    const long steps = (packs + (1 << lg) - 1) >> lg;
     const bool stream_out = bags * dim * (long)sizeof(T) > (32l << 20);    // eight L2 caches of 4 MB
     const auto kernel = stream_out ? embedding_lookup_kernel<T, E, Id, true> : embedding_lookup_kernel<T, E, Id, false>;
-    kernel<<<(unsigned)((jobs + groups - 1) / groups), 256, 0, stream>>>(table, ld, rows, dim, ids, (unsigned)jobs, (unsigned)steps, lg, scale, out);
+    const long most = kMostBlocks * groups / steps;            // lookups of a launch: steps < 2^25, so at least one
+    for (long b = 0; b < bags; b += most) {
+      const long jobs = (bags - b < most ? bags - b : most) * steps;
+      kernel<<<(unsigned)((jobs + groups - 1) / groups), 256, 0, stream>>>(table, ld, rows, dim, ids + b, (unsigned)jobs, (unsigned)steps, lg, scale,
+                                                                           out + b * dim);
+    }
   } else {
     int split = 0;                       // few bags: share a bag's tokens among groups, at least eight tokens each
     while ((2 << split) <= groups && (bags << split) * (packs >> lg > 0 ? packs >> lg : 1) < 8192 && (tokens >> (split + 1)) >= 8) ++split;
@@ -718,9 +725,11 @@ int launch_rows(GradArgs a, const void* grad, bool once, hipStream_t stream) {
   if (chunks > 0) {
     a.steps = (packs + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
     const long blocks = (chunks * a.steps + groups - 1) / groups;
-    if (blocks >= (1l << 24)) return TFR_EINVAL;                // no grid of 2^32 threads
-    if (once) embedding_runs_kernel<T, E, true, STREAM><<<(unsigned)blocks, 256, 0, stream>>>(a, (const T*)grad);
-    else embedding_runs_kernel<T, E, false, STREAM><<<(unsigned)blocks, 256, 0, stream>>>(a, (const T*)grad);
+    const long y = (blocks + kMostBlocks - 1) / kMostBlocks, x = (blocks + y - 1) / y;    // the last ones may find nothing to do
+    if (y > 65535) return TFR_EINVAL;                           // its partial sums would be 2^51 bytes
+    const dim3 grid((unsigned)x, (unsigned)y);
+    if (once) embedding_runs_kernel<T, E, true, STREAM><<<grid, 256, 0, stream>>>(a, (const T*)grad);
+    else embedding_runs_kernel<T, E, false, STREAM><<<grid, 256, 0, stream>>>(a, (const T*)grad);
   }
   const unsigned joins = chunks > 1 ? (unsigned)((chunks - 1 + groups - 1) / groups) : 0;
   embedding_rows_kernel<T, E, STREAM><<<joins + (unsigned)((a.rows + 4l * wr - 1) / (4l * wr)), 256, 0, stream>>>(a, (int)joins);

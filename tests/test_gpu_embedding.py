@@ -256,3 +256,34 @@ def test_layer_in_the_scorer():
     assert torch.equal(got, plain(dense_ctx, dense, mask))
     got[mask].sum().backward()
     assert all(e.weight.grad is not None and e.weight.grad.abs().sum() > 0 for e in emb.values())
+
+
+def test_the_most_lookups_of_a_call():
+    """2^25 lookups of rows that take two column steps of a wavefront: 2^24 workgroups and more in all, in launches that hold them."""
+    n, dim, rows = 1 << 25, 65, 1000
+    table = torch.randn(rows, dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    ids = torch.randint(0, rows, (n,), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV, dtype=torch.int32)
+    ids[-1], ids[0] = 7, -1
+    out = E().embedding_lookup(table, ids)
+    assert not out[0].any()
+    for a in range(0, n, 1 << 22):
+        at = ids[a:a + (1 << 22)].long()
+        assert torch.equal(out[a:a + (1 << 22)][at >= 0], table[at[at >= 0]])
+
+
+def test_gradient_of_wide_bags():
+    """Rows of 2^20 - 1 numbers, 65 535 occurrences in 255 bags: 2^24 workgroups for the runs.  In float64 by column parts."""
+    bags, tokens, dim, rows = 255, 257, (1 << 20) - 1, 512
+    ids = make_ids((bags, tokens), rows, 5, torch.int32, pad=0.05).to(DEV)
+    up = torch.randn(bags, dim, generator=torch.Generator(device=DEV).manual_seed(6), device=DEV).to(torch.bfloat16)
+    got = E().embedding_grad(up, ids, rows, 0.5, 'sum')
+    count = torch.zeros(rows + 1, bags, dtype=torch.float64, device=DEV)
+    at = torch.where(ids >= 0, ids.long(), rows)
+    count.index_put_((at, torch.arange(bags, device=DEV).unsqueeze(1).expand_as(at)), torch.ones((), dtype=torch.float64, device=DEV), accumulate=True)
+    count = count[:-1]
+    most = count.sum(1, keepdim=True)
+    for a in range(0, dim, 1 << 17):
+        u = up[:, a:a + (1 << 17)].double()
+        want, size = 0.5 * (count @ u), 0.5 * (count @ u.abs())
+        off = (got[:, a:a + (1 << 17)].double() - want).abs() - (2.0 ** -8 * 1.001 * want.abs() + (most + 3) * T.U * size)
+        assert off.max() <= 0
