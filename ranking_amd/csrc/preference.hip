@@ -161,8 +161,8 @@ __device__ __forceinline__ void list_pairs(const PrefArgs& a, long b, float y, d
       l = log1p(e) + (h < 0.0 ? -(1.0 - a.smoothing) * h : a.smoothing > 0.f ? a.smoothing * h : 0.0);   // h may be infinite
       d = (h < 0.0 ? e * q : q) - (1.0 - a.smoothing);
     } else if (a.kind == TFR_PREFERENCE_HINGE) {
-      l = fmax(0.0, 1.0 - h);
-      d = h < 1.0 ? -1.0 : 0.0;
+      l = h >= 1.0 ? 0.0 : 1.0 - h;                             // a margin that is NaN stays one
+      d = h >= 1.0 ? 0.0 : h < 1.0 ? -1.0 : h;
     } else {
       l = (h - 0.5) * (h - 0.5);
       d = 2.0 * h - 1.0;

@@ -278,3 +278,25 @@ def test_the_scalar_of_both_paths_and_in_a_graph(B, tokens):
         total, _ = loss.loss_and_grad(y, lp, w, reference=ref, mask=mask)
         torch.cuda.synchronize()
         assert torch.equal(held, total)
+
+
+@pytest.mark.parametrize('kind', ['logistic', 'hinge', 'squared'])
+@pytest.mark.parametrize('tokens', [3, 700, 5000])
+def test_nan_of_a_token_is_seen(kind, tokens):
+    """A NaN among an answer's tokens makes its list's loss NaN and the gradients of every answer that is paired with it, for every kind;
+    other lists and answers without a pair keep theirs."""
+    y = torch.tensor([[2.0, 1.0, -1.0], [1.0, 0.0, 0.0], [1.0, 1.0, 0.0]])
+    g = torch.Generator().manual_seed(tokens)
+    lp = -torch.rand(3, 3, tokens, generator=g)
+    good = lp.clone()
+    lp[0, 1, tokens // 2] = float('nan')
+    lp[2, 0, 0] = float('nan')                                             # paired with answer 2 alone
+    loss = K().PreferenceLoss(kind=kind, reduction='none')
+    on = lambda t: t.to(DEV)                                               # noqa: E731
+    got, want = loss(on(y), on(lp)).cpu(), loss(on(y), on(good)).cpu()
+    assert got[0].isnan() and got[2].isnan() and got[1] == want[1] and want.isfinite().all()
+    total, grad = K().PreferenceLoss(kind=kind, reduction='sum').loss_and_grad(on(y), on(lp))
+    clean = K().PreferenceLoss(kind=kind, reduction='sum').loss_and_grad(on(y), on(good))[1]
+    assert total.isnan()
+    assert grad[0, :2].isnan().all() and not grad[0, 2].any() and torch.equal(grad[1], clean[1])
+    assert grad[2, 0].isnan().all() and grad[2, 2].isnan().all() and torch.equal(grad[2, 1], clean[2, 1])
