@@ -12,7 +12,7 @@ stack below with every Dense on the fp32 matrix-core kernels of
 from __future__ import annotations
 
 import math
-from typing import Callable, Dict, List, Optional, Tuple
+from typing import Callable, Dict, List, Optional, Tuple, Union
 
 import torch
 from torch import nn
@@ -88,18 +88,22 @@ class Embedding(nn.Module):
     ``combiner``: the ids of the last axis are averaged, added, or kept apart with ``combiner=None``).
 
     Ids are int32 or int64, or float32 as the parsers of ``ranking_amd.data`` deliver integer features (exact up to 2^24).
-    Below 0 they are padding: zeros, no gradient.  ``embedding_lookup`` runs it (``ranking_amd.embedding``)."""
+    Below 0 they are padding: zeros, no gradient.  ``embedding_lookup`` runs it (``ranking_amd.embedding``).  ``dtype``: of the
+    table, or its name (``'bfloat16'``), as ``get_config`` gives it where it is not float32."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, combiner: Optional[str] = 'mean', scale: float = 1.0,
-                 dtype: torch.dtype = torch.float32):
+                 dtype: Union[torch.dtype, str] = torch.float32):
         super().__init__()
         if int(num_embeddings) < 1 or int(embedding_dim) < 1:
             raise ValueError('num_embeddings and embedding_dim must be positive, got %s and %s' % (num_embeddings, embedding_dim))
         if combiner not in (None, 'sum', 'mean'):
             raise ValueError("combiner must be None, 'sum' or 'mean', got %r" % (combiner,))
+        kind = getattr(torch, dtype, None) if isinstance(dtype, str) else dtype
+        if not isinstance(kind, torch.dtype):
+            raise ValueError('dtype must be a torch dtype or its name, got %r' % (dtype,))
         self.num_embeddings, self.embedding_dim = int(num_embeddings), int(embedding_dim)
         self.combiner, self.scale = combiner, float(scale)
-        self.weight = nn.Parameter(torch.empty(self.num_embeddings, self.embedding_dim, dtype=dtype))
+        self.weight = nn.Parameter(torch.empty(self.num_embeddings, self.embedding_dim, dtype=kind))
         nn.init.normal_(self.weight, std=1.0 / math.sqrt(self.embedding_dim))
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
@@ -111,8 +115,11 @@ class Embedding(nn.Module):
         return embedding_lookup(self.weight, ids, self.scale, self.combiner)
 
     def get_config(self):
-        return {'num_embeddings': self.num_embeddings, 'embedding_dim': self.embedding_dim, 'combiner': self.combiner,
-                'scale': self.scale}
+        config = {'num_embeddings': self.num_embeddings, 'embedding_dim': self.embedding_dim, 'combiner': self.combiner,
+                  'scale': self.scale}
+        if self.weight.dtype != torch.float32:
+            config['dtype'] = str(self.weight.dtype).replace('torch.', '')
+        return config
 
 
 class FlattenList(nn.Module):

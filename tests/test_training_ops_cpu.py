@@ -348,3 +348,15 @@ def test_a_learning_rate_on_the_device_follows_its_parameters():
     opt.load_state_dict(saved)
     got = opt.param_groups[0]['lr']
     assert torch.is_tensor(got) and got is not lr and got.item() == 0.25 and got.device == q.device
+
+
+def test_embedding_config_keeps_the_type():
+    import json
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        e = layers.Embedding(10, 4, combiner='sum', scale=2.0, dtype=dtype)
+        again = layers.Embedding(**json.loads(json.dumps(e.get_config())))
+        assert again.weight.dtype == dtype and again.get_config() == e.get_config()
+        assert layers.Embedding(10, 4).to(dtype).get_config() == layers.Embedding(10, 4, dtype=dtype).get_config()
+    for bad in ('other', 'nn', None, 2):
+        with pytest.raises(ValueError):
+            layers.Embedding(10, 4, dtype=bad)
