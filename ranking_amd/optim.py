@@ -72,15 +72,16 @@ def _uniform(params, grads, exp_avgs, exp_avg_sqs, eight):
         columns = [list(map(T.data_ptr, ts)) for ts in lists]
     except (TypeError, AttributeError):
         return None
-    if (device < 0 or dtype not in _DTYPES or min(sizes) == 0 or max(sizes) >= _MAX_LAUNCH or len(set(columns[0])) != len(columns[0])
+    if (device < 0 or dtype not in _DTYPES or min(sizes) == 0 or max(sizes) >= _MAX_LAUNCH
+            or len(set().union(columns[0], *columns[2:])) != len(sizes) * (len(columns) - 1)
             or (eight and any((a | b) & 7 for a, b in zip(columns[2], columns[4])))):
         return None
-    return {(device, dtype): list(zip(*columns, sizes))}
+    return {(device, dtype): columns + [sizes]}
 
 
 def _grouped(params, grads, exp_avgs, exp_avg_sqs, eight):
-    """By (device, type), the addresses of every tensor that holds something: param, grad, exp_avg, exp_avg_sq (8 bits: codes
-    and scales of both), and its number of elements."""
+    """By (device, type), the addresses of every tensor that holds something: columns of params, grads, exp_avgs, exp_avg_sqs (8
+    bits: codes and scales of both), and of their numbers of elements."""
     groups, seen = {}, set()
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
         device, dtype, numel = p.get_device(), p.dtype, p.numel()
@@ -109,11 +110,11 @@ def _grouped(params, grads, exp_avgs, exp_avg_sqs, eight):
         if numel >= _MAX_LAUNCH:
             raise ValueError('params of at most %d elements, got %d' % (_MAX_LAUNCH - 1, numel))
         if numel:
-            if row[0] in seen:
-                raise ValueError('the same parameter twice')
-            seen.add(row[0])
+            if not seen.isdisjoint(row[2:-1] + row[:1]) or len(set(row[2:-1] + row[:1])) < len(row) - 2:
+                raise ValueError('the same parameter or moment twice')
+            seen.update(row[2:-1] + row[:1])
             groups.setdefault((device, dtype), []).append(row)
-    return groups
+    return {key: list(zip(*rows)) for key, rows in groups.items()}
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence, exp_avg_sqs: Sequence, *, step: int,
@@ -123,8 +124,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
     ``params`` / ``grads``: dense tensors of one type (float32, bfloat16, float16) a pair.  ``exp_avgs`` / ``exp_avg_sqs``:
     float32 tensors of the parameter's size, or all of them pairs ``(codes, scales)``: int8 / uint8 codes and float32 scales
-    of ``quantized_size(param.numel())`` elements.  ``step`` counts from 1.  ``now``: float32 ``[3]`` on the device, the
-    coefficients of a step that is counted there, as ``tfr_adamw_advance`` writes them (``step`` and ``lr`` are then not used)."""
+    of ``quantized_size(param.numel())`` elements.  Parameters and moments are written: no two may share memory (two that begin
+    at one address are refused).  ``step`` counts from 1.  ``now``: float32 ``[3]`` on the device, the coefficients of a step
+    that is counted there, as ``tfr_adamw_advance`` writes them (``step`` and ``lr`` are then not used)."""
     n = len(params)
     if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n):
         raise ValueError('lists of %d params, %d grads, %d exp_avgs and %d exp_avg_sqs' % (n, len(grads), len(exp_avgs), len(exp_avg_sqs)))
@@ -157,16 +159,15 @@ def _launches(params, grads, exp_avgs, exp_avg_sqs, counted):
     cap = _MAX_TENSORS_8 if eight else _MAX_TENSORS
     name = ('tfr_adamw8' if eight else 'tfr_adamw') + ('_counted' if counted else '')
     launch = getattr(_lib.load(), name)
-    for (device, dtype), rows in groups.items():
-        size_of = [row[-1] for row in rows]
-        at = 0
-        while at < len(rows):
-            end = min(at + cap, len(rows))
-            while sum(size_of[at:end]) >= _MAX_LAUNCH:
+    for (device, dtype), columns in groups.items():
+        sizes, at = columns[-1], 0
+        while at < len(sizes):
+            end = min(at + cap, len(sizes))
+            while sum(sizes[at:end]) >= _MAX_LAUNCH:
                 end -= 1
-            columns = list(zip(*rows[at:end]))
             addresses = ctypes.c_void_p * (end - at)
-            yield launch, name, device, (_DTYPES[dtype], end - at, *[addresses(*c) for c in columns[:-1]], (ctypes.c_int64 * (end - at))(*columns[-1])), columns[0]
+            yield (launch, name, device, (_DTYPES[dtype], end - at, *[addresses(*c[at:end]) for c in columns[:-1]],
+                                          (ctypes.c_int64 * (end - at))(*sizes[at:end])), columns[0][at:end])
             at = end
 
 
@@ -295,22 +296,25 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            eight = group['state_bits'] == 8
+            eight, there = group['state_bits'] == 8, group['capturable']
+            counted_by = torch.Tensor if there else int
             runs = {}                                          # by step count: parameters that were frozen for a while have their own
             for p in group['params']:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise ValueError('AdamW does not take sparse gradients')
-                s = self._state_of(p, group)
-                t = 0 if group['capturable'] else s['step'] + 1
+                s = self.state[p]
+                if type(s.get('step')) is not counted_by:
+                    s = self._state_of(p, group)
+                t = 0 if there else s['step'] + 1
                 m, v = s['exp_avg'], s['exp_avg_sq']
                 runs.setdefault(t, []).append((s, p, p.grad.contiguous(), (m, s['exp_avg_scale']) if eight else m,
                                                (v, s['exp_avg_sq_scale']) if eight else v))
             if not runs:
                 continue
             how = dict(lr=group['lr'], betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'])
-            if group['capturable']:                            # all in one list: the launches read the counts on the device
+            if there:                                          # all in one list: the launches read the counts on the device
                 states, p, g, m, v = zip(*runs[0])
                 count = self._counter(group, p[0].device)
                 if any(q.device != count.device for q in group['params']):

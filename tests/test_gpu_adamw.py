@@ -554,3 +554,26 @@ def test_a_captured_step_goes_on_after_loading(bits):
         runs.append(seen)
     for a, b in zip(*runs):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+@pytest.mark.parametrize('uniform', [True, False])
+def test_moments_in_two_places_are_refused(bits, uniform):
+    """Tensors that a step writes belong to one parameter each: shared moments would be updated by two workgroups at once."""
+    z = lambda n, d=torch.float32: torch.zeros(n, dtype=d, device=DEV)     # noqa: E731
+    ps = [z(100), z(100, torch.float32 if uniform else torch.bfloat16)]
+    gs = [torch.ones_like(p) for p in ps]
+    one = lambda kind: z(100) if bits == 32 else (z(128, kind), z(1))       # noqa: E731
+    ms, vs = [one(torch.int8) for _ in ps], [one(torch.uint8) for _ in ps]
+    step = lambda m, v: O().adamw_step(ps, gs, m, v, step=1, lr=0.1)       # noqa: E731
+    bad = [([ms[0]] * 2, vs), (ms, [vs[0]] * 2)]
+    if bits == 32:
+        bad += [([vs[0], ms[1]], vs), ([ps[0], ms[1]], vs)]
+    else:
+        bad += [([ms[0], (ms[1][0], ms[0][1])], vs), (ms, [(vs[0][0], ms[0][1]), vs[1]])]
+    for m, v in bad:
+        with pytest.raises(ValueError, match='twice'):
+            step(m, v)
+    assert not any(p.any() for p in ps)
+    step(ms, vs)
+    assert all(p.ne(0).all() for p in ps)
