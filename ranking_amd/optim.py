@@ -354,7 +354,7 @@ class AdamW(torch.optim.Optimizer):
             if group['capturable'] and given['state_bits'] != group['state_bits'] and any(held.get(p) for p in group['params']):
                 raise ValueError('a state of %d bits does not fit one of %d that a captured step may hold' % (given['state_bits'], group['state_bits']))
             for p, i in zip(group['params'], given['params']):
-                for key, (dtype, numel) in self._moments(p, given).items() if i in state_dict['state'] else ():
+                for key, (dtype, numel) in self._moments(p, given).items() if state_dict['state'].get(i) else ():
                     value = state_dict['state'][i].get(key)
                     if not torch.is_tensor(value) or value.numel() != numel or (value.dtype != dtype if given['state_bits'] == 8 else not value.is_floating_point()):
                         raise ValueError('state %s does not fit a parameter of %d elements: %d of %s are wanted' % (key, p.numel(), numel, dtype))
@@ -363,7 +363,7 @@ class AdamW(torch.optim.Optimizer):
             group['capturable'] = there = bool(group['capturable'] or old['capturable'])
             count = given.get('step_count')
             for p, i in zip(group['params'], given['params']):
-                self._fill_state(p, group, held.get(p, {}), state_dict['state'].get(i), count)
+                self._fill_state(p, group, held.get(p, {}), state_dict['state'].get(i) or None, count)
             if not group['params']:
                 continue
             device = group['params'][0].device

@@ -360,3 +360,16 @@ def test_embedding_config_keeps_the_type():
     for bad in ('other', 'nn', None, 2):
         with pytest.raises(ValueError):
             layers.Embedding(10, 4, dtype=bad)
+
+
+def test_a_state_without_moments_is_no_state():
+    """What a step that was refused leaves of a new parameter is saved and loaded as nothing."""
+    import copy
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    opt, again = optim.AdamW([p]), optim.AdamW([q])
+    p.grad = torch.ones(3)
+    with pytest.raises(_lib.TfrHipError):
+        opt.step()
+    again.state[q] = held_state(q, 4)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert again.state[q]['step'] == 0 and not again.state[q]['exp_avg'].any()
