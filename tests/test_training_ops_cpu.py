@@ -362,12 +362,13 @@ def test_embedding_config_keeps_the_type():
             layers.Embedding(10, 4, dtype=bad)
 
 
-def test_a_state_without_moments_is_no_state():
+def test_a_state_without_moments_is_no_state(monkeypatch):
     """What a step that was refused leaves of a new parameter is saved and loaded as nothing."""
     import copy
     p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
     opt, again = optim.AdamW([p]), optim.AdamW([q])
     p.grad = torch.ones(3)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
     with pytest.raises(_lib.TfrHipError):
         opt.step()
     again.state[q] = held_state(q, 4)
