@@ -577,3 +577,29 @@ def test_moments_in_two_places_are_refused(bits, uniform):
     assert not any(p.any() for p in ps)
     step(ms, vs)
     assert all(p.ne(0).all() for p in ps)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_8_bits_a_lost_element_changes_no_other(dtype):
+    """NaN and infinite gradients, in a block whose scales do not hang on those elements: every other parameter, code and scale is bit
+    for bit that of the run in which those elements have no moments and no gradient."""
+    n, lost = 384, [3, 40, 255, 300]
+    p, g = (t[0] for t in make([n], dtype)[:2])
+    state = quantized([p])[0]
+    for k in lost:
+        state[0][k] = state[2][k] = 0
+    bad, good = g.clone(), g.clone()
+    bad[3], bad[40], bad[255], bad[300] = float('nan'), float('inf'), float('-inf'), float('nan')
+    good[lost] = 0.0
+    runs = []
+    for grad in (bad, good):
+        P, S = p.to(DEV), [x.clone().to(DEV) for x in state]
+        for step in (7, 8, 9):                                              # lost in the first step, and not found again
+            O().adamw_step([P], [(grad if step == 7 else good).to(DEV)], [(S[0], S[1])], [(S[2], S[3])], step=step, **HYPER)
+        runs.append([P.cpu()] + [s.cpu() for s in S])
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[lost] = False
+    for a, b, what in zip(runs[0], runs[1], ('param', 'exp_avg', 'exp_avg scale', 'exp_avg_sq', 'exp_avg_sq scale')):
+        rest = slice(None) if 'scale' in what else keep
+        assert torch.equal(a[rest], b[rest]) and torch.isfinite(a[rest].float()).all(), what
+    assert runs[0][1][lost].eq(-128).all() and runs[0][0][lost].isnan().all() and torch.isfinite(runs[1][0].float()).all()

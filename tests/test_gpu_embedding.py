@@ -287,3 +287,119 @@ def test_gradient_of_wide_bags():
         want, size = 0.5 * (count @ u), 0.5 * (count @ u.abs())
         off = (got[:, a:a + (1 << 17)].double() - want).abs() - (2.0 ** -8 * 1.001 * want.abs() + (most + 3) * T.U * size)
         assert off.max() <= 0
+
+
+# ---------------------------------------------------------------- sizes that take other paths
+def runs_of(lengths, seed, pad=0):
+    """Ids in a random order: token 2 k + 1 occurs lengths[k] times, `pad` more are padding."""
+    ids = torch.cat([torch.full((c,), 2 * k + 1, dtype=torch.int32) for k, c in enumerate(lengths)] + [torch.full((pad,), -1, dtype=torch.int32)])
+    return ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(seed))].to(DEV)
+
+
+def borders(chunk, n):
+    """Run lengths of n occurrences in all: runs that begin and end on, before and behind borders of chunks of `chunk`, one of 16 chunks
+    and more, many of one and two."""
+    runs = [chunk, chunk - 1, chunk + 1, 1, chunk - 1, 2 * chunk, 2 * chunk + 1, chunk - 2, 1, 16 * chunk, 15 * chunk, 17 * chunk + 3, 40 * chunk - 3]
+    left = n - sum(runs)
+    assert left > 0
+    runs += [left // 4] + [2, 1] * (left // 8) + [5] * (left // 32)
+    return runs + [n - sum(runs)]
+
+
+@pytest.mark.parametrize('dim,dtype', [(300, torch.float32), (300, torch.bfloat16), (1001, torch.float32), (1001, torch.bfloat16), (1024, torch.float16)])
+def test_gradient_of_long_runs_in_wide_rows(dim, dtype):
+    """Runs of 16 chunks and more, joined by a whole workgroup, in rows of several column steps; the same bits on repeat."""
+    lengths = [16 * 16 + 1, 15 * 16, 3, 17 * 16 - 1, 700, 1, 5]
+    ids = runs_of(lengths, 1, pad=9)
+    up = torch.randn(len(ids), dim, generator=torch.Generator().manual_seed(dim)).to(dtype).to(DEV)
+    rows = 2 * len(lengths) + 1
+    first = check_grad(up, ids, rows, 1.5, None)
+    assert torch.equal(first, E().embedding_grad(up, ids, rows, 1.5))
+    bags = len(ids) // 4
+    check_grad(up[:bags], ids[:4 * bags].view(bags, 4), rows, 1.5, 'mean')
+
+
+# a chunk doubles while the next length times 131 072 is within n times the lanes of a row: 32 from 65 536 occurrences of 64 lanes on,
+# 64 from 131 072, 128 beyond 2^20 occurrences
+@pytest.mark.parametrize('chunk,n,dim', [(16, 65535, 256), (32, 65537, 256), (64, 131073, 256), (64, 140001, 260), (128, 1100003, 64), (128, 1100003, 100)])
+def test_gradient_of_long_chunks(chunk, n, dim):
+    """Every length of a chunk: small integers, whose sums fp32 holds exactly, against the same sums in float64."""
+    lengths = borders(chunk, n - 777)
+    ids, rows = runs_of(lengths, chunk, pad=777), 2 * len(lengths) + 1
+    up = torch.randint(-8, 9, (n, dim), generator=torch.Generator(device=DEV).manual_seed(n), device=DEV).float()
+    got = E().embedding_grad(up, ids, rows)
+    at = torch.where(ids >= 0, ids.long(), rows)
+    want = torch.zeros(rows + 1, dim, dtype=torch.float64, device=DEV).index_add_(0, at, up.double())[:-1]
+    assert torch.equal(got.double(), want)
+    if dim == 256:                                                          # bf16: sums in fp32, one rounding
+        assert torch.equal(E().embedding_grad(up.to(torch.bfloat16), ids, rows), want.to(torch.bfloat16))
+    bags = n // 11
+    pooled = E().embedding_grad(up[:bags], ids[:bags * 11].view(bags, 11), rows, combiner='sum')
+    want = torch.zeros(rows + 1, dim, dtype=torch.float64, device=DEV).index_add_(0, at[:bags * 11], up[:bags].double().repeat_interleave(11, 0))[:-1]
+    assert torch.equal(pooled.double(), want)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [512, 514, 513])
+def test_lookup_beyond_the_caches(dtype, dim):
+    """Results of more than 32 MB go past the caches: 16-byte, 4-byte and single elements a lane; the same bits as row by row."""
+    n, rows = 70001, 3001
+    table = torch.randn(rows, dim, generator=torch.Generator(device=DEV).manual_seed(dim), device=DEV).to(dtype)
+    ids = make_ids((n,), rows, dim).to(DEV)
+    ids[5] = rows
+    assert n * dim * table.element_size() > 32 << 20
+    out = E().embedding_lookup(table, ids, 0.5)
+    want = (table.float()[ids.clamp(0, rows - 1)] * 0.5).to(dtype)
+    want[ids < 0] = 0
+    assert out[5].isnan().all()
+    keep = torch.arange(n, device=DEV) != 5
+    assert torch.equal(out[keep], want[keep])
+    assert torch.equal(out[:1000][keep[:1000]], E().embedding_lookup(table, ids[:1000], 0.5)[keep[:1000]])
+
+
+@pytest.mark.parametrize('dim,dtype', [(1024, torch.bfloat16), (1022, torch.bfloat16), (1023, torch.bfloat16), (640, torch.float32)])
+def test_gradient_table_beyond_the_caches(dim, dtype):
+    """A table of more than 256 MB, written past the caches, of many lookups; small integers as above."""
+    rows, n = 140001, 90001
+    ids = make_ids((n,), rows, dim, torch.int32, common=0.1).to(DEV)
+    up = torch.randint(-8, 9, (n, dim), generator=torch.Generator(device=DEV).manual_seed(dim), device=DEV).to(dtype)
+    assert rows * dim * up.element_size() > 256 << 20
+    got = E().embedding_grad(up, ids, rows)
+    at = torch.where(ids >= 0, ids.long(), rows)
+    want = torch.zeros(rows + 1, dim, device=DEV).index_add_(0, at, up.float())[:-1]      # exact: integers below 2^24 in any order
+    assert torch.equal(got, want.to(dtype))
+
+
+@pytest.mark.parametrize('padded', [False, True])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_layer_in_front_of_the_fused_tower(dtype, padded):
+    """DNNScorer's bf16 tower behind embedded example features: logits and table gradients are those of the same tower fed with the
+    embedded columns, the columns' gradient brought to the table by embedding_grad."""
+    import ranking_amd as ra
+    from ranking_amd.tower import FusedTower
+    torch.manual_seed(0)
+    L, M = ra.keras.layers, ra.keras.model
+    emb = {'d': L.Embedding(60, 24, 'mean', dtype=dtype), 'k': L.Embedding(9, 8, None, dtype=dtype)}
+    kw = dict(input_dim=24 + 8 * 3, hidden_layer_dims=[64, 32], dropout=0.0, compute_dtype=torch.bfloat16)
+    scorer, plain = M.DNNScorer(embeddings=emb, **kw).to(DEV), M.DNNScorer(**kw).to(DEV)
+    assert isinstance(scorer._tower, FusedTower)
+    plain._tower.load_state_dict(scorer._tower.state_dict())
+    ids = {'d': make_ids((16, 20, 5), 60, 2).to(DEV), 'k': make_ids((16, 20, 3), 9, 3, torch.int32).to(DEV)}
+    mask = torch.ones(16, 20, dtype=torch.bool, device=DEV)
+    if padded:
+        mask[:, 13:] = False
+        mask[3, 2:] = False
+    up = torch.randn(16, 20, generator=torch.Generator().manual_seed(4)).to(DEV) * mask
+    got = scorer({}, ids, mask)
+    got.backward(up)
+    dense = {k: emb[k](v).detach().flatten(2).requires_grad_() for k, v in ids.items()}
+    want = plain({}, dense, mask)
+    want.backward(up)
+    assert torch.equal(got, want) and got[mask].abs().sum() > 0
+    for k, combiner in (('d', 'mean'), ('k', None)):
+        g = dense[k].grad if combiner else dense[k].grad.view(16, 20, 3, 8)
+        wide, size, count = T.embedding_gradient(g, ids[k], emb[k].num_embeddings, 1.0, combiner)
+        assert wide.abs().sum() > 0
+        # padded lists: rows that are scored several times are added by atomics, in any order: 20 roundings of fp32, or of a bf16 step
+        again = (20 * T.U if dtype == torch.float32 else 2 * T.half(dtype)) * size if padded else 0.0
+        T.assert_within(emb[k].weight.grad, wide, T.half(dtype) * wide.abs() * 1.001 + (count.unsqueeze(1) + 3) * T.U * size + again + T.tiny(dtype), k)
