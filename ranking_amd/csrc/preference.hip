@@ -6,8 +6,10 @@
 //   loss  = w / P sum_{(i, j) : y_i > y_j >= 0} l(s_i - s_j),   P = number of such pairs (0 pairs: loss 0)
 //   l(h)  = (1 - a) softplus(-h) + a softplus(h)   |   max(0, 1 - h)   |   (h - 1/2)^2
 //   dloss/dlp_it = m_it f_i sum over the pairs of i of +-l'(h) w / P,   f_i = beta (/ length)
-// 9 bytes a token are read (4 + 4 + the mask's 1) and, with the mask once more, 4 written: HBM-bound for long answers (512 lists x 6
-// x 8192 tokens: 31 us for the sums = 7.2 TB/s, 19 for the gradient = 6.6, 6 for the pairs), launch-bound for short ones.
+// 9 bytes a token are read (4 + 4 + the mask's 1), those of absent answers are not, and, with the mask once more, 4 written for every
+// token: HBM-bound for long answers (512 lists x 6 x 8192 tokens, a sixth of the answers absent: 31 us for the sums = 6.1 TB/s, 19 for the
+// gradient = 6.6, 6 for the pairs), launch-bound for a few short ones, and bound by the fp64 exponentials of the pairs and single-token
+// reads for very many (282 574 lists x 3 x 13: 105 us with the gradient, 29 by its bytes).
 // Sums over tokens are fp64: a margin is the difference of two sums of thousands of tokens.  What stands in masked places or
 // in answers with y < 0 is never used (NaN there does no harm).
 #include "common.h"

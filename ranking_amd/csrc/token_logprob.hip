@@ -206,7 +206,8 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(const T* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
-// out[lo, hi) of one row by THREADS threads; aligned stores, the loads wide as well where x lies on the same offset.
+// out[lo, hi) of one row by THREADS threads: 16-byte accesses where x and out lie on the same offset from their boundaries, one element
+// at a time where they do not (8192 x 50 021 bf16: 364 us for rows that lie so, 566 for the same rows sliced from longer ones).
 template <typename T, int THREADS, bool STREAM>
 __device__ __forceinline__ void grad_row(const T* __restrict__ x, T* __restrict__ out, int lo, int hi, int tid, long y, float g, float m,
                                          float over_s, float c) {
