@@ -369,8 +369,9 @@ class AdamW(torch.optim.Optimizer):
             device = group['params'][0].device
             group.pop('coefficients', None)                    # of a state that counted by group alone
             group.pop('step_count', None)
-            if there and (count is not None or old.get('step_count') is not None):
-                group['step_count'] = _filled(old.get('step_count'), 0 if count is None else count, torch.int64, device)
+            have = old.get('step_count')
+            if there and (count is not None or have is not None):
+                group['step_count'] = _filled(have if have is not None and have.device == device else None, 0 if count is None else count, torch.int64, device)
             if torch.is_tensor(old['lr']):
                 group['lr'] = _filled(old['lr'], group['lr'], old['lr'].dtype, device)
             elif torch.is_tensor(group['lr']):
@@ -379,7 +380,8 @@ class AdamW(torch.optim.Optimizer):
     def _fill_state(self, p, group, have, given, count):
         """The state of one parameter from the saved one (None: as before any step), in the tensors of ``have`` that fit."""
         moments = self._moments(p, group)
-        fits = {k: t for k, t in have.items() if k in moments and torch.is_tensor(t) and (t.dtype, t.numel()) == moments[k]}
+        have = {k: t for k, t in have.items() if torch.is_tensor(t) and t.device == p.device}
+        fits = {k: t for k, t in have.items() if k in moments and (t.dtype, t.numel()) == moments[k]}
         if given is None:
             self.state.pop(p, None)
             if len(fits) < len(moments):
@@ -389,8 +391,7 @@ class AdamW(torch.optim.Optimizer):
             s[key] = _filled(fits.get(key), 0 if given is None else given[key], dtype, p.device)
         # counted by group alone, each of its parameters took all of the group's steps
         taken = 0 if given is None else given.get('step', 0 if count is None else count)
-        step = have.get('step')
-        s['step'] = _filled(step if torch.is_tensor(step) else None, taken, torch.int64, p.device) if group['capturable'] else int(taken)
+        s['step'] = _filled(have.get('step'), taken, torch.int64, p.device) if group['capturable'] else int(taken)
         for key, value in (given or {}).items():
             if key not in s:
                 s[key] = value

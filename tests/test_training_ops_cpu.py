@@ -374,3 +374,17 @@ def test_a_state_without_moments_is_no_state(monkeypatch):
     again.state[q] = held_state(q, 4)
     again.load_state_dict(copy.deepcopy(opt.state_dict()))
     assert again.state[q]['step'] == 0 and not again.state[q]['exp_avg'].any()
+
+
+def test_loading_follows_parameters_that_moved():
+    """State that is on another device than its parameter is replaced, not filled."""
+    import copy
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = optim.AdamW([p], capturable=True)
+    opt.state[p], opt.param_groups[0]['step_count'] = held_state(p, torch.tensor([4])), torch.tensor([4])
+    saved = copy.deepcopy(opt.state_dict())
+    opt.state[p] = {k: t.to('meta') for k, t in opt.state[p].items()}
+    opt.param_groups[0]['step_count'] = opt.param_groups[0]['step_count'].to('meta')
+    opt.load_state_dict(saved)
+    assert all(t.device == p.device for t in opt.state[p].values()) and opt.state[p]['step'].item() == 4
+    assert opt.param_groups[0]['step_count'].item() == 4 and opt.state[p]['exp_avg'].eq(0.5).all()
